@@ -305,6 +305,107 @@ int uk_cuda_decode_rmsnorm_gemm_f16(const float* X, const float* gamma, float ep
                                     uint16_t* const* Y_list, int n_y, int64_t ldy, int B, int N_shard, int K,
                                     int64_t col_offset, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- paged key-value cache ---------------------------------------------------
+ * The keys and values that the decode layer's attention reads, in pages of a
+ * pool.  A sequence owns the pages its row of a block table names, in order:
+ * position p of sequence b is offset p % page_size of page
+ * block_table[b * table_stride + p / page_size].  A row is one head's `dim`
+ * values of one position, contiguous; the three strides (in elements, the same
+ * for k and v) lay the rows out, so [page][token][head][dim] and
+ * [page][head][token][dim] pools both pass as they are.
+ *   UK_KV_F16   rows of binary16.
+ *   UK_KV_E4M3  rows of 8-bit e4m3 codes (4 exponent and 3 mantissa bits, no
+ *               infinity) and one exponent byte e per row, in k_exp / v_exp
+ *               [pages][heads][page_size]: value = code * 2^(e - 127).  e - 127
+ *               is within [-24, 15].
+ * Any page_size >= 1; dim a multiple of 8 (e4m3: of 16) from 8 to 128; pools
+ * 16-byte aligned, strides multiples of 16 bytes.
+ * Page ids and lengths are device memory and are not trusted: a page id outside
+ * the pool or a position beyond max_pages pages is treated as absent (nothing is
+ * written there; it reads as zeros; attention does not see it) and sets bit 64
+ * of uk_cuda_pipeline_fault.  Lengths below zero count as zero.
+ * The reference has no counterpart (its op set ends at softmax,
+ * src/codegen_hip.cpp:1985-2009). */
+#define UK_KV_F16 0
+#define UK_KV_E4M3 1
+typedef struct uk_kv_cache {
+  void* k;
+  void* v;
+  uint8_t* k_exp; /* e4m3; NULL for f16 */
+  uint8_t* v_exp;
+  int64_t page_stride, token_stride, head_stride;
+  int64_t pages;
+  int page_size, heads, dim, kind;
+} uk_kv_cache;
+
+/* Append packed rows K, V [total][heads][dim] (binary16, strides in elements)
+ * to the cache.  Sequence b brings rows cu_new[b] .. cu_new[b + 1] - 1, which
+ * become its LAST positions of seq_lens[b] (the lengths after the append):
+ * row j of n goes to position seq_lens[b] - n + j; rows that would land below
+ * position 0 are dropped.  cu_new [n_seq + 1] is non-decreasing; rows of K and
+ * V before cu_new[0] and from cu_new[n_seq] on (padding) are not read, pages
+ * not named are not touched.  The sequences of one call must not share a
+ * position that is written.
+ * e4m3: values are clamped to +-61440 (the largest multiple of 2^8 with an
+ * e4m3 significand that binary16 holds; at most 2^-4 off), e - 127 is the
+ * smallest integer >= -15 with max |x| <= 448 * 2^(e - 127), codes are
+ * x * 2^(127 - e) rounded to nearest even; NaN stays NaN. */
+int uk_cuda_kv_append_f16(const uint16_t* K, int64_t k_token_stride, int64_t k_head_stride, const uint16_t* V,
+                          int64_t v_token_stride, int64_t v_head_stride, int64_t total, const uk_kv_cache* cache,
+                          const int32_t* block_table, int64_t table_stride, int max_pages, const int32_t* cu_new,
+                          const int32_t* seq_lens, int n_seq, void* stream);
+
+/* The inverse: the last cu_out[b + 1] - cu_out[b] of the seq_lens[b] positions
+ * of each sequence, as packed binary16 rows K, V [total][heads][dim] (exact
+ * values of the codes).  Positions below 0 and absent pages give zeros; rows
+ * outside cu_out[0] .. cu_out[n_seq] - 1 are left as they were. */
+int uk_cuda_kv_gather_f16(const uk_kv_cache* cache, const int32_t* block_table, int64_t table_stride, int max_pages,
+                          const int32_t* cu_out, const int32_t* seq_lens, int n_seq, uint16_t* K,
+                          int64_t k_token_stride, int64_t k_head_stride, uint16_t* V, int64_t v_token_stride,
+                          int64_t v_head_stride, int64_t total, void* stream);
+
+/* ---- attention -----------------------------------------------------------------
+ * Attention of one new token per sequence over its cached positions (the decode
+ * layer's scores, softmax and value product in one pass over the cache):
+ *   O[b][h] = sum_p softmax_p(scale * Q[b][h] . K[p][g]) V[p][g],
+ *   p < seq_lens[b], g = h / (heads_q / cache->heads);
+ * LSE[b][h] = log sum_p exp(scale * Q[b][h] . K[p][g]) (fp32; NULL to leave it
+ * out).  A sequence of length zero gives zeros and -inf.  Q, O binary16
+ * [n_seq][heads_q][dim], strides in elements (multiples of 8, 16-byte aligned).
+ * Scores, softmax statistics and sums are fp32; the softmax weights enter the
+ * value product as binary16, one rounding into O.  A NaN or an infinity among
+ * the values seen makes that column's outputs NaN or infinite.
+ * Deterministic.  The workspace (its size depends on the current device, the
+ * heads and dim, not on lengths or n_seq) may be reused by later calls on the
+ * same stream; calls that can overlap need one each. */
+size_t uk_cuda_attn_decode_workspace_size(int heads_q, int heads_kv, int dim);
+int uk_cuda_attn_decode_f16(const uint16_t* Q, int64_t q_seq_stride, int64_t q_head_stride, const uk_kv_cache* cache,
+                            const int32_t* block_table, int64_t table_stride, int max_pages,
+                            const int32_t* seq_lens, int n_seq, int heads_q, float scale, uint16_t* O,
+                            int64_t o_seq_stride, int64_t o_head_stride, float* LSE, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
+/* Attention over packed prompts: sequence b has query rows cu_q[b] ..
+ * cu_q[b + 1] - 1 of Q [total_q][heads_q][dim] and key rows cu_k[b] ..
+ * cu_k[b + 1] - 1 of K, V [total_k][heads_kv][dim] (binary16; strides in
+ * elements, multiples of 8, 16-byte aligned; dim a multiple of 8 from 8 to
+ * 128).  causal != 0: with n query and m key rows, query i sees keys 0 ..
+ * m - n + i (the queries are the last n positions); else all m.
+ *   O[i][h] = sum_j softmax_j(scale * Q[i][h] . K[j][g]) V[j][g]
+ * over the keys it sees, whatever the others hold (infinities and NaN too);
+ * LSE [total_q][heads_q] as above, or NULL.  A query that sees no key gives
+ * zeros and -inf.  Rows of O and LSE outside cu_q[0] .. cu_q[n_seq] - 1 are left
+ * as they were.  cu_q and cu_k are device memory, non-decreasing within
+ * [0, total_q] and [0, total_k]; values outside are clamped.  fp32 scores,
+ * statistics and sums; the softmax weights enter the value product as binary16.
+ * Deterministic. */
+int uk_cuda_attn_prompt_f16(const uint16_t* Q, int64_t q_token_stride, int64_t q_head_stride, const uint16_t* K,
+                            int64_t k_token_stride, int64_t k_head_stride, const uint16_t* V, int64_t v_token_stride,
+                            int64_t v_head_stride, const int32_t* cu_q, const int32_t* cu_k, int n_seq,
+                            int64_t total_q, int64_t total_k, int heads_q, int heads_kv, int dim, float scale,
+                            int causal, uint16_t* O, int64_t o_token_stride, int64_t o_head_stride, float* LSE,
+                            void* stream);
+
 /* ---- multi-GPU from a C/C++ host, over NCCL (one process per GPU) ----------
  * NCCL is resolved at run time (the process's loaded libnccl, else
  * libnccl.so.2); these calls return UK_ECUDA when it is absent.
@@ -372,7 +473,8 @@ int uk_cuda_peer_barrier(unsigned* const* flag_list, int n, int rank, unsigned e
 /* Fault word of the tensor-core pipelines: 0 when no bounded wait inside a
  * kernel of this library expired since the last call, otherwise a bit mask
  * (1 producer, 2 MMA issuer, 4 epilogue, 8 teardown, 16 self-test, 32 peer
- * wait).  Synchronises with the device and clears the word.  A kernel whose
+ * wait; and 64, not a wait: a page id or a position outside the pool or the
+ * block table was skipped by a cache or attention call).  Synchronises with the device and clears the word.  A kernel whose
  * wait expires unwinds and leaves its outputs undefined instead of hanging.
  * No reference counterpart (the reference has no device-side waits). */
 unsigned uk_cuda_pipeline_fault(void);

@@ -1,0 +1,480 @@
+"""Attention over a paged cache (one new token per sequence) and over packed
+prompts on the GPU, against the definition in 64 bits; bounds in attn_testutil."""
+import math
+
+import pytest
+import torch
+
+from attn_testutil import Pool, assert_close, attention_f64, same_bits
+
+pytestmark = pytest.mark.gpu
+
+
+def abi():
+    import unikern_b200.abi as a
+    assert torch.cuda.is_available()
+    return a
+
+
+def i32(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def prefix(v):
+    out = [0]
+    for x in v:
+        out.append(out[-1] + x)
+    return out
+
+
+def fault():
+    torch.cuda.synchronize()
+    return abi().lib().uk_cuda_pipeline_fault()
+
+
+def randn(*shape, seed=0, mul=1.0):
+    return (torch.randn(shape, generator=torch.Generator("cuda").manual_seed(seed), device="cuda") * mul).half()
+
+
+# ---- one new token over a paged cache -----------------------------------------------
+
+def check_decode(pool, q, o, lse, scale, values=None, gone=None):
+    """gone: per sequence a set of positions that do not count."""
+    heads_q, group = q.shape[1], q.shape[1] // pool.heads
+    for b, n in enumerate(pool.lens):
+        k, v = (values or pool.values)[b]
+        seen = torch.ones(group, n, dtype=torch.bool, device="cuda")
+        if gone:
+            seen[:, sorted(gone[b])] = False
+        for g in range(pool.heads):
+            rows = slice(g * group, (g + 1) * group)
+            ro, rl, to, tl = attention_f64(q[b, rows], k[:, g], v[:, g], scale, seen)
+            assert_close(o[b, rows], ro, to, "sequence %d heads of %d: o" % (b, g))
+            if lse is not None:
+                assert_close(lse[b, rows], rl, tl, "sequence %d heads of %d: lse" % (b, g))
+
+
+DECODE = [  # kind, layout, heads_kv, group, dim, page_size, lengths
+    ("f16", "nhd", 1, 1, 8, 1, [1]),
+    ("f16", "hnd", 2, 3, 24, 3, [0, 1, 2, 5, 0]),
+    ("f16", "hnd", 8, 4, 128, 16, [500]),
+    ("f16", "nhd", 2, 8, 64, 16, [15, 16, 17, 63, 64, 65, 127, 128, 129, 0, 1]),
+    ("f16", "hnd", 1, 12, 128, 32, [1000, 31, 2049]),
+    ("f16", "nhd", 2, 16, 96, 7, [333, 64]),
+    ("f16", "hnd", 1, 20, 80, 256, [1500]),
+    ("f16", "hnd", 1, 40, 120, 5, [77, 0, 200]),
+    ("f16", "hnd", 3, 5, 104, 64, [400, 1]),
+    ("e4m3", "hnd", 1, 1, 16, 1, [1, 2, 0]),
+    ("e4m3", "nhd", 3, 4, 48, 5, [9, 40, 0, 333]),
+    ("e4m3", "hnd", 8, 4, 128, 16, [700, 12]),
+    ("e4m3", "hnd", 2, 7, 64, 32, [31, 32, 33, 95, 96, 97, 255, 256, 257, 1, 0]),
+    ("e4m3", "nhd", 1, 16, 112, 24, [2000]),
+    ("e4m3", "hnd", 1, 9, 80, 64, [129, 4097]),
+    ("e4m3", "hnd", 1, 33, 32, 128, [300, 20]),
+]
+
+
+@pytest.mark.parametrize("kind,layout,heads,group,dim,page,lens", DECODE)
+def test_decode(kind, layout, heads, group, dim, page, lens):
+    a = abi()
+    fault()
+    pool = Pool(kind, layout, heads, dim, page, lens, seed=3)
+    q = randn(len(lens), heads * group, dim, seed=5)
+    o, lse = torch.full_like(q, math.nan), torch.full(q.shape[:2], math.nan, device="cuda")
+    a.attn_decode(q, pool.cache, pool.table, pool.lens_t, o, lse=lse)
+    assert fault() == 0
+    check_decode(pool, q, o, lse, dim ** -0.5)
+    # the same again: same bits; without lse; strided rows of a wider tensor
+    wide = torch.full((len(lens), 3, heads * group, dim), 7.0, dtype=torch.float16, device="cuda")
+    wide[:, 0] = q
+    a.attn_decode(wide[:, 0], pool.cache, pool.table, pool.lens_t, wide[:, 2])
+    assert same_bits(wide[:, 2], o) and (wide[:, 1] == 7).all() and same_bits(wide[:, 0], q)
+
+
+@pytest.mark.parametrize("kind", ["f16", "e4m3"])
+@pytest.mark.parametrize("lens", [[8191], [3000] * 9, [1] * 700, [0] * 5, [0, 0, 5000, 0, 1, 0, 640, 0, 0],
+                                  [i * 13 % 700 for i in range(300)]])
+def test_decode_work_split(kind, lens):
+    """Lengths that the split of the work cuts in every way: within a
+    sequence, between sequences, more sequences than blocks, none at all."""
+    a = abi()
+    pool = Pool(kind, "hnd", 2, 64, 16, lens, seed=1, table_pad=0 if max(lens) else 1)
+    q = randn(len(lens), 8, 64, seed=2)
+    o, lse = torch.full_like(q, math.nan), torch.full(q.shape[:2], math.nan, device="cuda")
+    a.attn_decode(q, pool.cache, pool.table, pool.lens_t, o, lse=lse)
+    check_decode(pool, q, o, lse, 64 ** -0.5)
+
+
+@pytest.mark.parametrize("kind", ["f16", "e4m3"])
+def test_decode_long(kind):
+    """One long sequence, one key head: many parts joined; a strong first key
+    in front of a long weak tail (weights far below the first one's)."""
+    a = abi()
+    n, dim = 131071, 128
+    pool = Pool(kind, "nhd", 1, dim, 64, [n], seed=1)
+    q = randn(1, 16, dim, seed=2)
+    strong = (q[0, 0] * 2).view(1, 1, dim)  # score of head 0 about 2 |q|^2 / sqrt(dim) = 22
+    first = pool.put(0, 0, 0, strong)
+    k, v = pool.values[0]
+    k[0:1] = first
+    o, lse = torch.empty_like(q), torch.empty(1, 16, device="cuda")
+    a.attn_decode(q, pool.cache, pool.table, pool.lens_t, o, lse=lse)
+    check_decode(pool, q, o, lse, dim ** -0.5)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3, 1.0, 40.0])
+def test_decode_scales(scale):
+    """Uniform weights, negative scales, and scores of some hundreds that rise
+    along the sequence (every tile raises the maximum)."""
+    a = abi()
+    for kind in ("f16", "e4m3"):
+        pool = Pool(kind, "hnd", 1, 64, 16, [1000, 70], seed=1)
+        q = randn(2, 4, 64, seed=2)
+        if scale == 40.0:
+            for b, n in enumerate(pool.lens):
+                up = q[b, 0].float() * torch.arange(n, device="cuda").view(n, 1, 1) / n / q[b, 0].float().norm()
+                pool.values[b] = (pool.put(0, b, 0, up.half()), pool.values[b][1])
+        o, lse = torch.empty_like(q), torch.empty(2, 4, device="cuda")
+        a.attn_decode(q, pool.cache, pool.table, pool.lens_t, o, scale=scale, lse=lse)
+        check_decode(pool, q, o, lse, scale)
+
+
+def test_decode_infinities_and_nan():
+    """Held NaN and infinities reach exactly the heads and columns they should;
+    a key of the type's lowest value takes no weight."""
+    a = abi()
+    pool = Pool("f16", "hnd", 2, 32, 16, [40, 40, 40], seed=1)
+    q = randn(3, 4, 32, seed=2).abs() + 0.1
+    low = torch.full((1, 2, 32), -65504.0, dtype=torch.float16, device="cuda")
+    pool.values[0] = (pool.values[0][0].clone(), pool.values[0][1])
+    pool.values[0][0][7:8] = pool.put(0, 0, 7, low)
+    v = pool.values[1][1].half()
+    v[20, 1, 3], v[30, 1, 5] = math.inf, math.nan
+    pool.values[1] = (pool.values[1][0], pool.put(1, 1, 0, v))
+    k = pool.values[2][0].half()
+    k[11, 0, 2] = math.nan
+    pool.values[2] = (pool.put(0, 2, 0, k), pool.values[2][1])
+    o, lse = torch.empty_like(q), torch.empty(3, 4, device="cuda")
+    a.attn_decode(q, pool.cache, pool.table, pool.lens_t, o, lse=lse)
+    assert torch.isfinite(o[0]).all()
+    assert torch.isfinite(o[1, :2]).all() and not torch.isfinite(o[1, 2:, 3]).any() and torch.isnan(o[1, 2:, 5]).all()
+    rest = [c for c in range(32) if c not in (3, 5)]
+    assert torch.isfinite(o[1][:, rest]).all()
+    assert torch.isnan(o[2, :2]).all() and torch.isfinite(o[2, 2:]).all()
+    pool.lens = [40]
+    check_decode(pool, q, o, lse, 32 ** -0.5)
+
+
+def test_decode_absent_pages():
+    a = abi()
+    fault()
+    for kind in ("f16", "e4m3"):
+        pool = Pool(kind, "hnd", 2, 64, 8, [50, 50, 50, 50], seed=1)
+        table = pool.table.clone()
+        table[0, 2] = -1
+        table[1, 6] = pool.pages
+        table[2, :] = 2147483647
+        gone = [set(range(16, 24)), {48, 49}, set(range(50)), set()]
+        q = randn(4, 4, 64, seed=2)
+        o, lse = torch.empty_like(q), torch.empty(4, 4, device="cuda")
+        lens = pool.lens_t.clone()
+        a.attn_decode(q, pool.cache, table, lens, o, lse=lse)
+        assert fault() == 64
+        check_decode(pool, q, o, lse, 0.125, gone=gone)
+        # lengths behind the table stop at it (the pad entries are bad ids), negative ones are empty
+        lens[0], lens[3] = 2147483647, -4
+        a.attn_decode(q, pool.cache, pool.table, lens, o, lse=lse)
+        assert fault() == 64
+        assert (o[3] == 0).all() and (lse[3] == -math.inf).all()
+        far = pool.table.shape[1] * 8
+        assert far > 50  # positions 50 .. 55 are held by nobody: all bits set, NaN
+        full = Pool(kind, "hnd", 2, 64, 8, [56], seed=1, table_pad=0)
+        ln = i32([2147483647])
+        qq = q[:1].contiguous()
+        o1, l1 = torch.empty_like(qq), torch.empty(1, 4, device="cuda")
+        a.attn_decode(qq, full.cache, full.table, ln, o1, lse=l1)
+        assert fault() == 64
+        check_decode(full, qq, o1, l1, 0.125)
+
+
+def test_decode_offsets_past_32_bits():
+    a = abi()
+    heads, dim, ps = 2, 64, 16
+    stride = (1 << 31) // 2 + 64
+    k, v = (torch.empty(4 * stride + ps * heads * dim, dtype=torch.float16, device="cuda")
+            .as_strided((5, ps, heads, dim), (stride, heads * dim, dim, 1)) for _ in "kv")
+    x = [randn(40, heads, dim, seed=i) for i in range(2)]
+    table = i32([[4, 0, 3]])
+    cache = a.KvCache(k, v)
+    a.kv_append(x[0], x[1], cache, table, i32([0, 40]), i32([40]))
+    q = randn(1, 6, dim, seed=7)
+    o = torch.empty_like(q)
+    a.attn_decode(q, cache, table, i32([40]), o)
+    seen = torch.ones(3, 40, dtype=torch.bool, device="cuda")
+    for g in range(heads):
+        ro, _, to, _ = attention_f64(q[0, 3 * g:3 * g + 3], x[0][:, g], x[1][:, g], dim ** -0.5, seen)
+        assert_close(o[0, 3 * g:3 * g + 3], ro, to, "o")
+
+
+# ---- packed prompts -------------------------------------------------------------------
+
+def check_prompt(q, k, v, cu_q, cu_k, o, lse, scale, causal):
+    group = q.shape[1] // k.shape[1]
+    for b in range(len(cu_q) - 1):
+        n, m = cu_q[b + 1] - cu_q[b], cu_k[b + 1] - cu_k[b]
+        if n == 0:
+            continue
+        i, j = torch.arange(n, device="cuda")[:, None], torch.arange(m, device="cuda")[None]
+        seen = (j <= i + m - n) if causal else (j >= 0).expand(n, m)
+        qs, ks = slice(cu_q[b], cu_q[b + 1]), slice(cu_k[b], cu_k[b + 1])
+        for h in range(q.shape[1]):
+            ro, rl, to, tl = attention_f64(q[qs, h], k[ks, h // group], v[ks, h // group], scale, seen)
+            assert_close(o[qs, h], ro, to, "sequence %d head %d: o" % (b, h))
+            assert_close(lse[qs, h], rl, tl, "sequence %d head %d: lse" % (b, h))
+
+
+PROMPT = [  # heads_kv, group, dim, query lengths, key lengths (None: the same)
+    (1, 1, 8, [1], None),
+    (1, 1, 128, [128], None),
+    (2, 2, 64, [1, 2, 0, 3, 127, 128, 129], None),
+    (1, 3, 128, [255, 256, 257], None),
+    (2, 4, 128, [77], None),
+    (1, 5, 80, [300, 5], None),
+    (3, 1, 72, [64, 200], None),
+    (1, 2, 128, [1, 1, 5, 130, 128], [1, 500, 5, 1000, 129]),
+    (1, 2, 64, [10, 200, 130, 7, 3], [4, 100, 0, 7, 260]),
+    (2, 3, 24, [40, 0, 17, 140], [0, 30, 400, 139]),
+    (1, 8, 96, [513], [700]),
+    (1, 1, 128, [1] * 40, [i * 7 for i in range(40)]),
+]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("heads,group,dim,nq,nk", PROMPT)
+def test_prompt(heads, group, dim, nq, nk, causal):
+    a = abi()
+    fault()
+    nk = nq if nk is None else nk
+    # NaN rows before the first, behind the last and between nothing: they belong to nobody
+    lead, tail = 5, 133
+    cu_q, cu_k = [lead + c for c in prefix(nq)], [lead + c for c in prefix(nk)]
+    tq, tk = cu_q[-1] + tail, cu_k[-1] + tail
+    q = randn(tq, heads * group, dim, seed=1)
+    kv = randn(tk, 2 * heads, dim, seed=2)  # keys beside values: strided heads
+    for x, cu in ((q, cu_q), (kv, cu_k)):
+        x[:lead], x[cu[-1]:] = math.nan, math.nan
+    k, v = kv[:, :heads], kv[:, heads:]
+    o = torch.full((tq, heads * group, 2, dim), 7.0, dtype=torch.float16, device="cuda")
+    lse = torch.full((tq, heads * group), 7.0, device="cuda")
+    a.attn_prompt(q, k, v, i32(cu_q), i32(cu_k), o[:, :, 0], causal=causal, lse=lse)
+    assert fault() == 0
+    assert (o[:, :, 1] == 7).all()
+    for x in (o, lse):
+        assert (x[:lead] == 7).all() and (x[cu_q[-1]:] == 7).all()
+    check_prompt(q, k, v, cu_q, cu_k, o[:, :, 0], lse, dim ** -0.5, causal)
+    again = torch.empty_like(q)
+    a.attn_prompt(q, k, v, i32(cu_q), i32(cu_k), again, causal=causal)
+    rows = slice(cu_q[0], cu_q[-1])
+    assert same_bits(again[rows], o[rows, :, 0])
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.2, 1.0, 30.0])
+def test_prompt_scales(scale):
+    a = abi()
+    n, dim = 400, 64
+    q, k, v = (randn(n, 2, dim, seed=s) for s in range(3))
+    if scale == 30.0:  # scores that rise along the keys: the maximum moves in every tile
+        up = q[-1].float() / q[-1].float().norm(dim=-1, keepdim=True)
+        k = (up[None] * torch.arange(n, device="cuda")[:, None, None] / n).half()
+    o, lse = torch.empty_like(q), torch.empty(n, 2, device="cuda")
+    a.attn_prompt(q, k, v, i32([0, n]), i32([0, n]), o, scale=scale, lse=lse)
+    check_prompt(q, k, v, [0, n], [0, n], o, lse, scale, True)
+
+
+def test_prompt_weak_tail():
+    """A strong first key in front of many weak ones, whose weights together
+    still count: they must not vanish in a narrow type."""
+    a = abi()
+    n, dim = 4096, 128
+    q, k, v = (randn(n, 1, dim, seed=s, mul=m) for s, m in ((1, 1.0), (2, 0.05), (3, 1.0)))
+    q[:, 0] = q[0, 0]
+    k[0, 0] = q[0, 0] * (13.0 * math.sqrt(dim) / float(q[0, 0].float().square().sum()))  # score 13 = ln 442413
+    v[1:] += 2.0
+    o, lse = torch.empty_like(q), torch.empty(n, 1, device="cuda")
+    a.attn_prompt(q, k, v, i32([0, n]), i32([0, n]), o, lse=lse)
+    check_prompt(q, k, v, [0, n], [0, n], o, lse, dim ** -0.5, True)
+
+
+def test_prompt_rows_do_not_see_behind_their_mask():
+    """Infinities, NaN and the lowest value at later keys reach no earlier row;
+    at keys that are seen they do."""
+    a = abi()
+    n, dim = 300, 64
+    for where in ("k", "v"):
+        for value in (math.nan, math.inf, -math.inf, -65504.0):
+            q, k, v = (randn(n, 2, dim, seed=s) for s in range(3))
+            x = k if where == "k" else v
+            x[150, 0], x[299, 1] = value, value
+            o, lse = torch.empty_like(q), torch.empty(n, 2, device="cuda")
+            a.attn_prompt(q, k, v, i32([0, n]), i32([0, n]), o, lse=lse)
+            check_prompt(q[:150], k[:150], v[:150], [0, 150], [0, 150], o[:150], lse[:150], dim ** -0.5, True)
+            check_prompt(q[:299, 1:], k[:299, 1:], v[:299, 1:], [0, 299], [0, 299], o[:299, 1:], lse[:299, 1:],
+                         dim ** -0.5, True)
+            if where == "v" and value != -65504.0:
+                bad = torch.isnan(o[150:, 0]) if math.isnan(value) else torch.isinf(o[150:, 0])
+                assert bad.all()
+                assert torch.isfinite(lse).all()
+
+
+def test_prompt_bounds_of_the_length_arrays():
+    """Row bounds outside the tensors are clamped, never read."""
+    a = abi()
+    q, k, v = (randn(100, 2, 32, seed=s) for s in range(3))
+    o, lse = torch.full_like(q, 7.0), torch.full((100, 2), 7.0, device="cuda")
+    a.attn_prompt(q, k, v, i32([-5, 1000]), i32([-7, 2000]), o, causal=False, lse=lse)
+    check_prompt(q, k, v, [0, 100], [0, 100], o, lse, 32 ** -0.5, False)
+    a.attn_prompt(q, k, v, i32([0, 100]), i32([60, 20]), o, lse=lse)
+    assert (o == 0).all() and (lse == -math.inf).all()
+    assert fault() == 0
+
+
+def test_prompt_many_sequences_and_heads():
+    a = abi()
+    nq = [i % 5 for i in range(400)]
+    nk = [n + i % 3 for i, n in enumerate(nq)]
+    cu_q, cu_k = prefix(nq), prefix(nk)
+    q, k, v = randn(cu_q[-1], 6, 16, seed=1), randn(cu_k[-1], 3, 16, seed=2), randn(cu_k[-1], 3, 16, seed=3)
+    o, lse = torch.empty_like(q), torch.empty(cu_q[-1], 6, device="cuda")
+    a.attn_prompt(q, k, v, i32(cu_q), i32(cu_k), o, lse=lse)
+    check_prompt(q, k, v, cu_q, cu_k, o, lse, 0.25, True)
+
+
+def test_prompt_long():
+    a = abi()
+    n, dim = 3001, 128
+    q, k, v = randn(n, 4, dim, seed=1), randn(n, 2, dim, seed=2), randn(n, 2, dim, seed=3)
+    o, lse = torch.empty_like(q), torch.empty(n, 4, device="cuda")
+    a.attn_prompt(q, k, v, i32([0, n]), i32([0, n]), o, lse=lse)
+    check_prompt(q, k, v, [0, n], [0, n], o, lse, dim ** -0.5, True)
+
+
+# ---- together -------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kind", ["f16", "e4m3"])
+def test_serving_run(kind):
+    """Prompts in two chunks and then single tokens, as a server runs them:
+    append, gather the context, attend over it, decode; every row against the
+    attention over what the cache holds."""
+    a = abi()
+    fault()
+    hk, group, dim, ps = 2, 4, 64, 16
+    prompts, chunk, steps = [150, 40, 0, 71], 64, 5
+    n_seq = len(prompts)
+    rows = [[randn(p + steps, h, dim, seed=10 * b + i) for i, h in enumerate((hk * group, hk, hk))]
+            for b, p in enumerate(prompts)]
+    pool = Pool(kind, "hnd", hk, dim, ps, [0] * n_seq, max_len=max(prompts) + steps)
+    scale, done = dim ** -0.5, [0] * n_seq
+    out = [torch.zeros(p + steps, hk * group, dim, device="cuda", dtype=torch.float16) for p in prompts]
+    lses = [torch.zeros(p + steps, hk * group, device="cuda") for p in prompts]
+    while any(d < p for d, p in zip(done, prompts)):
+        new = [min(chunk, p - d) for d, p in zip(done, prompts)]
+        lens = [d + n for d, n in zip(done, new)]
+        q, k, v = (torch.cat([rows[b][i][done[b]:lens[b]] for b in range(n_seq)]) for i in range(3))
+        cu_q, cu_k = i32(prefix(new)), i32(prefix(lens))
+        a.kv_append(k, v, pool.cache, pool.table, cu_q, i32(lens))
+        ck, cv = (torch.empty(sum(lens), hk, dim, dtype=torch.float16, device="cuda") for _ in "kv")
+        a.kv_gather(pool.cache, pool.table, cu_k, i32(lens), ck, cv)
+        o, lse = torch.empty_like(q), torch.empty(q.shape[:2], device="cuda")
+        a.attn_prompt(q, ck, cv, cu_q, cu_k, o, lse=lse)
+        for b, c in enumerate(prefix(new)[:-1]):
+            out[b][done[b]:lens[b]], lses[b][done[b]:lens[b]] = o[c:c + new[b]], lse[c:c + new[b]]
+        done = lens
+    ws = a.attn_decode_workspace(pool.cache, hk * group)
+    for step in range(steps):
+        at = [d + step for d in done]
+        q, k, v = (torch.stack([rows[b][i][at[b]] for b in range(n_seq)]) for i in range(3))
+        lens = i32([p + 1 for p in at])
+        a.kv_append(k, v, pool.cache, pool.table, i32(range(n_seq + 1)), lens)
+        o, lse = torch.empty_like(q), torch.empty(q.shape[:2], device="cuda")
+        a.attn_decode(q, pool.cache, pool.table, lens, o, lse=lse, workspace=ws)
+        for b in range(n_seq):
+            out[b][at[b]], lses[b][at[b]] = o[b], lse[b]
+    assert fault() == 0
+    for b, p in enumerate(prompts):
+        n = p + steps
+        k, v = pool.get(0, b, 0, n), pool.get(1, b, 0, n)
+        check_prompt(rows[b][0], k, v, [0, n], [0, n], out[b], lses[b], scale, True)
+
+
+def test_two_streams_with_a_workspace_each():
+    a = abi()
+    pools = [Pool(kind, "hnd", 2, 128, 16, [5000, 3000], seed=s) for s, kind in enumerate(("f16", "e4m3"))]
+    q = randn(2, 8, 128, seed=1)
+    want, got = [], []
+    for p in pools:
+        want.append(torch.empty_like(q))
+        a.attn_decode(q, p.cache, p.table, p.lens_t, want[-1])
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in pools]
+    for rep in range(10):
+        for p, st in zip(pools, streams):
+            got.append(torch.empty_like(q))
+            a.attn_decode(q, p.cache, p.table, p.lens_t, got[-1], stream=st)  # its own workspace each
+    torch.cuda.synchronize()
+    for i, o in enumerate(got):
+        assert same_bits(o, want[i % 2])
+
+
+def test_captured_and_replayed():
+    """Decode and prompt in one graph, replayed with other lengths and inputs;
+    the workspace serves an eager call between replays."""
+    a = abi()
+    pool = Pool("f16", "hnd", 2, 64, 16, [900, 64, 300], seed=1)
+    q, qp = randn(3, 4, 64, seed=1), randn(260, 4, 64, seed=2)
+    kp, vp = randn(260, 2, 64, seed=3), randn(260, 2, 64, seed=4)
+    lens, cu = pool.lens_t.clone(), i32([0, 100, 260])
+    o, op = torch.empty_like(q), torch.empty_like(qp)
+    lse, lp = torch.empty(3, 4, device="cuda"), torch.empty(260, 4, device="cuda")
+    ws = a.attn_decode_workspace(pool.cache, 4)
+    graph = torch.cuda.CUDAGraph()
+    a.attn_decode(q, pool.cache, pool.table, lens, o, lse=lse, workspace=ws)
+    a.attn_prompt(qp, kp, vp, cu, cu, op, lse=lp)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        a.attn_decode(q, pool.cache, pool.table, lens, o, lse=lse, workspace=ws)
+        a.attn_prompt(qp, kp, vp, cu, cu, op, lse=lp)
+    other = torch.empty_like(q)
+    for step, (ln, c) in enumerate((([900, 64, 300], [0, 100, 260]), ([1, 0, 299], [3, 259, 259]),
+                                    ([890, 1, 0], [0, 0, 128]))):
+        lens.copy_(i32(ln))
+        cu.copy_(i32(c))
+        qp.copy_(randn(260, 4, 64, seed=20 + step))
+        q.copy_(randn(3, 4, 64, seed=30 + step))
+        graph.replay()
+        a.attn_decode(q, pool.cache, pool.table, pool.lens_t, other, workspace=ws)
+        torch.cuda.synchronize()
+        pool.lens = ln
+        vals = [tuple(x[:n] for x in kv) for kv, n in zip(pool.values, ln)]
+        check_decode(pool, q, o, lse, 0.125, values=vals)
+        check_prompt(qp, kp, vp, c, c, op, lp, 0.125, True)
+    del graph
+
+
+def test_large_grids():
+    """More rows than one dimension of a grid holds."""
+    a = abi()
+    n = 70000
+    q, k, v = randn(n, 1, 8, seed=1), randn(n, 1, 8, seed=2), randn(n, 1, 8, seed=3)
+    cu = torch.arange(n + 1, dtype=torch.int32, device="cuda")
+    o = torch.empty_like(q)
+    a.attn_prompt(q, k, v, cu, cu, o)
+    assert same_bits(o, v)  # one key: weight one
+    pool = torch.empty(n, 1, 1, 8, dtype=torch.float16, device="cuda"), torch.empty(n, 1, 1, 8, dtype=torch.float16,
+                                                                                device="cuda")
+    cache = a.KvCache(*pool)
+    table = torch.arange(n, dtype=torch.int32, device="cuda").flip(0).view(n, 1)
+    ones = torch.ones(n, dtype=torch.int32, device="cuda")
+    a.kv_append(k, v, cache, table, cu, ones)
+    a.attn_decode(q, cache, table, ones, o.zero_())
+    assert same_bits(o, v)
+    assert fault() == 0

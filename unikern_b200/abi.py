@@ -17,6 +17,16 @@ _PATH = Path(os.environ.get("UNIKERN_CUDA_LIB") or Path(__file__).resolve().pare
 
 vp, i64, i32, f32, sz = C.c_void_p, C.c_int64, C.c_int, C.c_float, C.c_size_t
 
+
+
+class KvCacheStruct(C.Structure):
+    """uk_kv_cache."""
+    _fields_ = [("k", vp), ("v", vp), ("k_exp", vp), ("v_exp", vp), ("page_stride", i64), ("token_stride", i64),
+                ("head_stride", i64), ("pages", i64), ("page_size", i32), ("heads", i32), ("dim", i32), ("kind", i32)]
+
+
+_kv = C.POINTER(KvCacheStruct)
+
 # name -> (restype, argtypes); must match include/unikern_cuda.h
 PROTOTYPES = {
     "uk_cuda_last_error": (C.c_char_p, []),
@@ -67,6 +77,13 @@ PROTOTYPES = {
     "uk_cuda_tile_plan": (i32, [i32, i32, C.POINTER(C.c_int64), i32, C.POINTER(C.c_int)]),
     "uk_cuda_solve_plan": (i32, [i32, i32, C.POINTER(C.c_int64), i32, i32, C.POINTER(C.c_int)]),
     "uk_cuda_last_launch": (i32, [C.POINTER(C.c_int)]),
+    "uk_cuda_kv_append_f16": (i32, [vp, i64, i64, vp, i64, i64, i64, _kv, vp, i64, i32, vp, vp, i32, vp]),
+    "uk_cuda_kv_gather_f16": (i32, [_kv, vp, i64, i32, vp, vp, i32, vp, i64, i64, vp, i64, i64, i64, vp]),
+    "uk_cuda_attn_decode_workspace_size": (sz, [i32, i32, i32]),
+    "uk_cuda_attn_decode_f16": (i32, [vp, i64, i64, _kv, vp, i64, i32, vp, i32, i32, f32, vp, i64, i64, vp, vp, sz,
+                                      vp]),
+    "uk_cuda_attn_prompt_f16": (i32, [vp, i64, i64, vp, i64, i64, vp, i64, i64, vp, vp, i32, i64, i64, i32, i32, i32,
+                                      f32, i32, vp, i64, i64, vp, vp]),
     "uk_nccl_unique_id_size": (sz, []),
     "uk_nccl_get_unique_id": (i32, [vp]),
     "uk_nccl_comm_init": (i32, [vp, i32, i32, C.c_uint64, C.POINTER(vp)]),
@@ -320,6 +337,148 @@ def conv2d_f16(X, Wt, Y, N, H, W, Cc, Kh, Kw, Oc, pad=0, scale=None, layout=UK_C
     nbytes = ws.numel() * ws.element_size() if ws is not None else 0
     check(lib().uk_cuda_conv2d_f16(_p(X), _p(Wt), _p(Y), N, H, W, Cc, Kh, Kw, Oc, pad, _p(scale), layout,
                                    _p(ws), nbytes, _stream(stream)))
+
+
+# ---- paged key-value cache and attention ----------------------------------------
+
+UK_KV_F16, UK_KV_E4M3 = 0, 1
+
+
+def _need(ok, *msg):
+    if not ok:
+        raise UkError(2, " ".join(str(m) for m in msg))
+
+
+class KvCache:
+    """A paged key-value cache over the caller's pools.
+
+    k, v: [pages, page_size, heads, dim] tensors of the same strides (a pool
+    kept as [pages, heads, page_size, dim] passes as its transpose(1, 2)),
+    float16, or float8_e4m3fn with k_exp, v_exp: uint8 [pages, heads,
+    page_size], contiguous (value = code * 2^(exp - 127))."""
+
+    def __init__(self, k, v, k_exp=None, v_exp=None):
+        import torch
+        _need(k.dim() == 4 and k.shape == v.shape and k.stride() == v.stride() and k.dtype == v.dtype,
+              "KvCache: k and v must be [pages, page_size, heads, dim] tensors of one type, shape and strides")
+        _need(k.stride(3) == 1 or k.shape[3] == 1, "KvCache: a row's values must be contiguous")
+        _need(k.dtype in (torch.float16, torch.float8_e4m3fn), "KvCache: float16 or float8_e4m3fn, got", k.dtype)
+        pages, page_size, heads, dim = k.shape
+        e4m3 = k.dtype == torch.float8_e4m3fn
+        for e in (k_exp, v_exp):
+            if e4m3:
+                _need(e is not None and e.dtype == torch.uint8 and tuple(e.shape) == (pages, heads, page_size)
+                      and e.is_contiguous(), "KvCache: exponents must be contiguous uint8 [pages, heads, page_size]")
+            else:
+                _need(e is None, "KvCache: exponents belong to an e4m3 cache")
+        self.tensors = (k, v, k_exp, v_exp)  # kept alive
+        self.heads, self.dim, self.page_size, self.pages = heads, dim, page_size, pages
+        self.struct = KvCacheStruct(_p(k), _p(v), _p(k_exp), _p(v_exp), k.stride(0), k.stride(1), k.stride(2), pages,
+                                    page_size, heads, dim, UK_KV_E4M3 if e4m3 else UK_KV_F16)
+        self.ref = C.byref(self.struct)
+
+
+def _index(t, n, name):
+    import torch
+    _need(t.dtype is torch.int32 and t.dim() == 1 and t.shape[0] == n and (n <= 1 or t.stride(0) == 1), name,
+          "must be a contiguous int32 tensor of", n)
+
+
+def _table(table):
+    import torch
+    _need(table.dtype is torch.int32 and table.dim() == 2 and (table.shape[1] <= 1 or table.stride(1) == 1),
+          "block_table must be an int32 [sequences, pages] tensor with contiguous rows")
+    return table.shape
+
+
+def _rows(t, name, heads, dim):
+    import torch
+    _need(t.dtype is torch.float16 and t.dim() == 3 and t.shape[1] == heads and t.shape[2] == dim
+          and t.stride(2) == 1, name, "must be a float16 [tokens, %d, %d] tensor with contiguous rows" % (heads, dim))
+    return t.shape[0]
+
+
+def _lse(lse, n, heads):
+    import torch
+    _need(lse is None or (lse.dtype is torch.float32 and lse.shape == (n, heads) and lse.is_contiguous()),
+          "lse must be a contiguous float32 [%d, %d] tensor" % (n, heads))
+
+
+def kv_append(K, V, cache, block_table, cu_new, seq_lens, stream=None):
+    """Append packed rows K, V [tokens, heads, dim] to a paged cache: rows
+    cu_new[b] .. cu_new[b + 1] - 1 become the last of sequence b's seq_lens[b]
+    positions (the lengths after the append)."""
+    n_seq, pages = _table(block_table)
+    total = _rows(K, "K", cache.heads, cache.dim)
+    _need(_rows(V, "V", cache.heads, cache.dim) == total, "K and V must have the same rows")
+    _index(cu_new, n_seq + 1, "cu_new")
+    _index(seq_lens, n_seq, "seq_lens")
+    check(lib().uk_cuda_kv_append_f16(_p(K), K.stride(0), K.stride(1), _p(V), V.stride(0), V.stride(1), total,
+                                      cache.ref, _p(block_table), block_table.stride(0), pages, _p(cu_new),
+                                      _p(seq_lens), n_seq, _stream(stream)))
+
+
+def kv_gather(cache, block_table, cu_out, seq_lens, K, V, stream=None):
+    """Read the last cu_out[b + 1] - cu_out[b] of each sequence's seq_lens[b]
+    cached positions back into packed rows K, V [tokens, heads, dim]."""
+    n_seq, pages = _table(block_table)
+    total = _rows(K, "K", cache.heads, cache.dim)
+    _need(_rows(V, "V", cache.heads, cache.dim) == total, "K and V must have the same rows")
+    _index(cu_out, n_seq + 1, "cu_out")
+    _index(seq_lens, n_seq, "seq_lens")
+    check(lib().uk_cuda_kv_gather_f16(cache.ref, _p(block_table), block_table.stride(0), pages, _p(cu_out),
+                                      _p(seq_lens), n_seq, _p(K), K.stride(0), K.stride(1), _p(V), V.stride(0),
+                                      V.stride(1), total, _stream(stream)))
+
+
+def attn_decode_workspace(cache, heads_q, stream=None):
+    """The decode attention's workspace for this cache (a torch uint8 tensor of
+    `stream`, by default the current one); calls that can overlap need one each."""
+    import torch
+    n = lib().uk_cuda_attn_decode_workspace_size(heads_q, cache.heads, cache.dim)
+    with torch.cuda.stream(stream):
+        return torch.empty(n, dtype=torch.uint8, device="cuda")
+
+
+def attn_decode(Q, cache, block_table, seq_lens, O, scale=None, lse=None, workspace=None, stream=None):
+    """O[b] = softmax(scale Q[b] K^T) V over sequence b's seq_lens[b] cached
+    positions; Q, O [sequences, heads_q, dim], scale 1 / sqrt(dim) by default,
+    lse [sequences, heads_q] gets the log of the softmax's sum.  Allocates its
+    workspace through torch when none is passed."""
+    n_seq, pages = _table(block_table)
+    heads_q = Q.shape[1] if Q.dim() == 3 else 0
+    _need(_rows(Q, "Q", heads_q, cache.dim) == n_seq, "Q must have one row per sequence")
+    _need(_rows(O, "O", heads_q, cache.dim) == n_seq, "O must have one row per sequence")
+    _index(seq_lens, n_seq, "seq_lens")
+    _lse(lse, n_seq, heads_q)
+    # a workspace of the call's own stream: freed here, it can only be handed
+    # out again to work behind this call
+    ws = workspace if workspace is not None else attn_decode_workspace(cache, heads_q, stream)
+    check(lib().uk_cuda_attn_decode_f16(_p(Q), Q.stride(0), Q.stride(1), cache.ref, _p(block_table),
+                                        block_table.stride(0), pages, _p(seq_lens), n_seq, heads_q,
+                                        cache.dim ** -0.5 if scale is None else scale, _p(O), O.stride(0), O.stride(1),
+                                        _p(lse), _p(ws), ws.numel() * ws.element_size(), _stream(stream)))
+
+
+def attn_prompt(Q, K, V, cu_q, cu_k, O, scale=None, causal=True, lse=None, stream=None):
+    """Attention over packed prompts: sequence b has query rows cu_q[b] ..
+    cu_q[b + 1] - 1 of Q [tokens, heads_q, dim] and key rows cu_k[b] ..
+    cu_k[b + 1] - 1 of K, V [tokens, heads_kv, dim]; causal aligns the last
+    query with the last key."""
+    _need(Q.dim() == 3 and K.dim() == 3, "Q and K must be [tokens, heads, dim] tensors")
+    heads_q, dim, heads_kv = Q.shape[1], Q.shape[2], K.shape[1]
+    total_q, total_k = _rows(Q, "Q", heads_q, dim), _rows(K, "K", heads_kv, dim)
+    _need(_rows(V, "V", heads_kv, dim) == total_k, "K and V must have the same rows")
+    _need(_rows(O, "O", heads_q, dim) == total_q, "O must have Q's rows")
+    n_seq = cu_q.shape[0] - 1
+    _need(n_seq >= 0, "cu_q must have one value more than there are sequences")
+    _index(cu_q, n_seq + 1, "cu_q")
+    _index(cu_k, n_seq + 1, "cu_k")
+    _lse(lse, total_q, heads_q)
+    check(lib().uk_cuda_attn_prompt_f16(_p(Q), Q.stride(0), Q.stride(1), _p(K), K.stride(0), K.stride(1), _p(V),
+                                        V.stride(0), V.stride(1), _p(cu_q), _p(cu_k), n_seq, total_q, total_k, heads_q,
+                                        heads_kv, dim, dim ** -0.5 if scale is None else scale, int(causal), _p(O),
+                                        O.stride(0), O.stride(1), _p(lse), _stream(stream)))
 
 
 # ---- KML runner (host side) -----------------------------------------------------

@@ -17,6 +17,7 @@
 #define UK_FAULT_TEARDOWN 0x8u
 #define UK_FAULT_SELFTEST 0x10u
 #define UK_FAULT_PEER 0x20u
+#define UK_FAULT_PAGE 0x40u  // not a wait: a page id or position outside the pool was skipped
 
 __device__ __forceinline__ uint32_t uk_smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
