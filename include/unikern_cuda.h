@@ -319,7 +319,8 @@ int uk_cuda_decode_rmsnorm_gemm_f16(const float* X, const float* gamma, float ep
  *               [pages][heads][page_size]: value = code * 2^(e - 127).  e - 127
  *               is within [-24, 15].
  * Any page_size >= 1; dim a multiple of 8 (e4m3: of 16) from 8 to 128; pools
- * 16-byte aligned, strides multiples of 16 bytes.
+ * 16-byte aligned, strides multiples of 16 bytes; max_pages * page_size below
+ * 2^31 - 4096.
  * Page ids and lengths are device memory and are not trusted: a page id outside
  * the pool or a position beyond max_pages pages is treated as absent (nothing is
  * written there; it reads as zeros; attention does not see it) and sets bit 64

@@ -1,9 +1,40 @@
 // attn_decode.cu -- attention of one new token per sequence over a paged cache:
 //   O[b][h] = sum_p w_p V[p][g],  w = softmax(scale * Q[b][h] . K[p][g]),
 // p < seq_lens[b], g = h / (query heads per key head), in one pass over the
-// cache with the running maximum m and sum l of the softmax:
-//   m' = max(m, s),  l' = l 2^(m - m') + 2^(s - m'),  o' = o 2^(m - m') + 2^(s - m') v
-// (scores s carry scale * log2 e, so every exponential is a power of two).
+// cache with a running reference m, sum l and product o per head:
+//   l = sum 2^(s_p - m),  o = sum 2^(s_p - m) v_p,  s = score * scale * log2 e;
+// m moves (l and o scaled by 2^(m - m')) only when a score passes it by 2^8, so
+// weights stay within [0, 2^15] as binary16 after a constant shift of 7.
+//
+// The work is bound by streaming the cache once: the floor is its bytes over
+// the HBM rate.  Two kernels:
+// * k_attn_decode: one resident wave of CTAs.  The (sequence, key head) pairs'
+//   lengths, cut into tiles of 64 or 128 positions, are laid end to end and
+//   every CTA takes an equal run of that line, whatever the lengths are: no
+//   tail of long sequences, no empty CTAs.  A run that covers a pair whole
+//   writes O; a pair cut by a run's end leaves (m, l, o) in the workspace, at
+//   most two per CTA (the pair that entered its run, the pair that leaves it).
+// * k_attn_join: for each pair that left a run, the sum of its parts in the
+//   order of the CTAs (deterministic); launched programmatically behind the
+//   first.
+//
+// Within a CTA each of 4 warps takes its own 16 or 32 positions of a tile and
+// never waits for another: rows go from global memory straight into the
+// registers of the mma.sync operand that needs them, with no shared memory in
+// between.  The products are S^T = K Q^T (16 positions x 8 query heads) and
+// O^T += V^T P^T, so a key head's query group fills the 8 columns instead of
+// padding 16 rows, and the fragments fit 16-byte loads by renaming the
+// contraction index:
+//   K (A operand, 16 x 16): lane (r = lane / 4, q = lane % 4) holds 16 bytes at
+//     d = 8 q (f16) or 16 q (e4m3) of positions r and r + 8; Q is loaded in the
+//     same order of d, so the sum over d is the same.
+//   V^T (A operand): lane (r, q) holds 16 bytes at d = 8 r (16 r) of positions
+//     2q, 2q + 1, 2q + 8, 2q + 9; a byte permute pairs neighbouring positions,
+//     as the operand packs them, and the row index d is renamed.
+//   P^T (B operand): the S^T accumulator has position and head exchanged; an
+//     8 x 8 transpose between lanes (movmatrix) puts that right.
+// K of the next tile loads while the softmax and V product of this one run,
+// then V of the next; page ids load one tile earlier still.
 #include "kv_cache.cuh"
 
 namespace uk {
@@ -12,8 +43,11 @@ __device__ unsigned int g_attn_decode_fault = 0;
 
 namespace {
 
-constexpr int WARPS = 4;
+constexpr int WARPS = 4, THREADS = WARPS * 32;
+constexpr int MAX_CTAS = 1024;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float GROW = 8.f;   // scores may pass the reference by 2^8 before it moves
+constexpr float SHIFT = 7.f;  // weights are held as 2^7 * 2^(s - m): up to 2^15, binary16 ends at 2^16
 
 struct Args {
   const uint16_t* q;
@@ -22,84 +56,582 @@ struct Args {
   int64_t o_seq, o_head;
   float* lse;
   const int32_t* lens;
-  int n_seq, heads_q, group;
-  float scale2;  // scale * log2 e
+  int n_seq, heads_q, group;  // group = query heads per key head
+  int chunks;                 // runs of 8 NH query heads per key head
+  float scale2;               // scale * log2 e
+  float* parts;               // [ctas][2][part_floats]
+  int4* recs;                 // [ctas]: pair left unfinished {b, pair, last CTA, -}, b = -1: none
 };
 
-// four values of a cache row as floats
-__device__ __forceinline__ float4 row4(const UkKvView& c, const uint8_t* row, const uint8_t* e, int lane) {
-  if (lane * 4 >= c.dim) return make_float4(0.f, 0.f, 0.f, 0.f);
-  uint2 h;
-  float s = 1.f;
-  if (c.kind == UK_KV_F16) {
-    h = __ldg(reinterpret_cast<const uint2*>(row) + lane);
-  } else {
-    const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(row) + lane);
-    h = make_uint2(uk_e4m3x2_to_half2(w), uk_e4m3x2_to_half2(w >> 16));
-    s = uk_exp_scale(__ldg(e));
-  }
-  const float2 a = __half22float2(*reinterpret_cast<__half2*>(&h.x)), b = __half22float2(*reinterpret_cast<__half2*>(&h.y));
-  return make_float4(a.x * s, a.y * s, b.x * s, b.y * s);
+template <int KIND, int DP>
+struct Shape {
+  static constexpr bool kF16 = KIND == UK_KV_F16;
+  static constexpr int NT = (kF16 && DP == 128) ? 1 : 2;  // 16-position groups per warp tile
+  static constexpr int WT = 16 * NT, CT = WARPS * WT;     // positions per warp and CTA tile
+  static constexpr int KC = kF16 ? DP / 32 : DP / 64;     // 16-byte loads of a K row per lane
+  static constexpr int VC = kF16 ? DP / 64 : 1;           // loads of a V row per lane
+  static constexpr int VB = kF16 ? 16 : DP / 8;           // bytes of each (8 or 16)
+  static constexpr int VW = VB / 4;                       // words of each
+  static constexpr int MV = DP / 16;                      // V products per group of positions
+};
+
+__host__ __device__ constexpr int part_floats(int dp, int nh) { return 8 * nh * (dp + 2); }
+
+__device__ __forceinline__ uint4 ldg16(const void* p, bool on) {
+  uint4 v = make_uint4(0, 0, 0, 0);
+  if (on)
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint2 ldg8(const void* p, bool on) {
+  uint2 v = make_uint2(0, 0);
+  if (on) asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
 }
 
-// One CTA per (sequence, query head); each warp takes every fourth position,
-// a lane four of the row's values.
-__global__ void __launch_bounds__(WARPS * 32) k_attn_decode(Args a, UkKvView c) {
-  __shared__ float sm[WARPS], sl[WARPS];
-  __shared__ float4 so[WARPS][32];
-  const int b = blockIdx.x / a.heads_q, h = blockIdx.x % a.heads_q, g = h / a.group;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t room = (int64_t)c.max_pages * c.page_size;
-  int len = max(__ldg(a.lens + b), 0);
-  if (len > room) {
-    if (threadIdx.x == 0) atomicOr(&uk::g_attn_decode_fault, UK_FAULT_PAGE);
-    len = (int)room;
+// D (16 x 8, fp32) += A (16 x 16, f16) B (16 x 8, f16)
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// 8 x 8 transpose of halves between the lanes of a warp
+__device__ __forceinline__ uint32_t transpose8(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
+  const __half2 r = __hmul2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// ---- the line of tiles -------------------------------------------------------------
+struct Line {
+  int64_t total;  // tiles of all pairs
+  int64_t ctas;   // CTAs that take part, each with at least one tile
+  __device__ __forceinline__ int64_t begin(int64_t c) const { return c * total / ctas; }
+  // the CTA whose run holds tile x: the last c with c * total / ctas <= x
+  __device__ __forceinline__ int64_t owner(int64_t x) const { return ((x + 1) * ctas - 1) / total; }
+};
+
+__device__ __forceinline__ int clamped_len(const Args& a, int64_t room, int b) {
+  const int len = max(__ldg(a.lens + b), 0);
+  return len > room ? (int)room : len;
+}
+
+// The line, and the sequence that holds this CTA's first tile with the number
+// of tiles (of one pair) before it.  Every thread sums a run of sequences; the
+// thread whose run holds the tile finds it there.
+template <int CT>
+__device__ Line find_begin(const Args& a, int64_t room, int pairs, int64_t* x0, int64_t* x1, int* b0, int64_t* before) {
+  __shared__ int64_t warp_sum[WARPS];
+  __shared__ int64_t s_before;
+  __shared__ int s_b;
+  const int per = (a.n_seq + THREADS - 1) / THREADS;
+  const int first = min((int)threadIdx.x * per, a.n_seq), last = min(first + per, a.n_seq);
+  int64_t mine = 0;
+  for (int b = first; b < last; ++b) mine += (clamped_len(a, room, b) + CT - 1) / CT;
+  int64_t incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t t = __shfl_up_sync(0xffffffffu, incl, o);
+    if ((threadIdx.x & 31) >= o) incl += t;
   }
-  float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (lane * 4 < c.dim) {
-    const uint2 w = __ldg(reinterpret_cast<const uint2*>(a.q + b * a.q_seq + h * a.q_head) + lane);
-    const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w.x)), y = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
-    q = make_float4(x.x, x.y, y.x, y.y);
+  if ((threadIdx.x & 31) == 31) warp_sum[threadIdx.x >> 5] = incl;
+  __syncthreads();
+  int64_t base = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) {
+    if (w < (int)(threadIdx.x >> 5)) base += warp_sum[w];
+    all += warp_sum[w];
   }
-  float m = -INFINITY, l = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int p = warp; p < len; p += WARPS) {
-    int off;
-    const int page = uk_kv_page(c, b, p, &off);
-    if (page < 0) {
-      if (lane == 0) atomicOr(&uk::g_attn_decode_fault, UK_FAULT_PAGE);
-      continue;
+  Line line{all * pairs, 0};
+  line.ctas = min((int64_t)gridDim.x, line.total);
+  *x0 = *x1 = 0;
+  if ((int64_t)blockIdx.x < line.ctas) {
+    *x0 = line.begin(blockIdx.x);
+    *x1 = line.begin(blockIdx.x + 1);
+    int64_t at = base + incl - mine;  // tiles before this thread's run
+    if (at * pairs <= *x0 && *x0 < (at + mine) * pairs) {
+      int b = first;
+      for (;; ++b) {
+        const int64_t nt = (clamped_len(a, room, b) + CT - 1) / CT;
+        if (*x0 < (at + nt) * pairs) break;  // mine bounds the sum: ends within the run
+        at += nt;
+      }
+      s_b = b;
+      s_before = at;
     }
-    const int64_t at = uk_kv_row(c, page, off, g), ea = uk_kv_exp(c, page, off, g);
-    const float4 k = row4(c, c.k + at, c.k_exp + ea, lane), v = row4(c, c.v + at, c.v_exp + ea, lane);
-    const float s = uk_warp_sum(q.x * k.x + q.y * k.y + q.z * k.z + q.w * k.w) * a.scale2;
-    const float m2 = fmaxf(m, s);
-    const float f = m2 == -INFINITY ? 1.f : exp2f(m - m2), e = m2 == -INFINITY ? 0.f : exp2f(s - m2);
-    m = m2;
-    l = l * f + e;
-    o = make_float4(o.x * f + e * v.x, o.y * f + e * v.y, o.z * f + e * v.z, o.w * f + e * v.w);
   }
-  if (lane == 0) sm[warp] = m, sl[warp] = l;
+  __syncthreads();
+  *b0 = s_b;
+  *before = s_before;
+  return line;
+}
+
+// ---- the kernel -----------------------------------------------------------------------
+template <int KIND, int DP, int NH>
+__global__ void __launch_bounds__(THREADS, NH == 1 ? 3 : 2) k_attn_decode(Args a, UkKvView c) {
+  using S = Shape<KIND, DP>;
+  constexpr int CT = S::CT, WT = S::WT, NT = S::NT;
+  __shared__ float sm_m[WARPS][8 * NH], sm_l[WARPS][8 * NH];
+  __shared__ __align__(16) float sm_o[WARPS][8 * NH][DP + 2];
+
+  uk_pdl_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, q = lane & 3;
+  const int64_t room = (int64_t)c.max_pages * c.page_size;
+  const int pairs = c.heads * a.chunks;
+
+  // sequences without positions have no tiles: their rows are written here
+  for (int b = blockIdx.x; b < a.n_seq; b += gridDim.x) {
+    const int len = __ldg(a.lens + b);
+    if (len > room && threadIdx.x == 0) atomicOr(&uk::g_attn_decode_fault, UK_FAULT_PAGE);
+    if (len > 0 && room > 0) continue;
+    for (int i = threadIdx.x; i < a.heads_q * (c.dim / 8); i += THREADS) {
+      const int h = i / (c.dim / 8), d = i % (c.dim / 8);
+      reinterpret_cast<uint4*>(a.o + b * a.o_seq + h * a.o_head)[d] = make_uint4(0, 0, 0, 0);
+    }
+    if (a.lse != nullptr)
+      for (int h = threadIdx.x; h < a.heads_q; h += THREADS) a.lse[(int64_t)b * a.heads_q + h] = -INFINITY;
+  }
+
+  int64_t x0, x1, before;
+  int b;
+  const Line line = find_begin<CT>(a, room, pairs, &x0, &x1, &b, &before);
+  if (x0 >= x1) {
+    if (threadIdx.x == 0) a.recs[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    return;
+  }
+
+  int4 rec = make_int4(-1, 0, 0, 0);
+  int64_t x = x0;
+  int len = clamped_len(a, room, b), nt = (len + CT - 1) / CT;
+  int pair = (int)((x - before * pairs) / nt);
+  while (x < x1) {
+    const int64_t start = before * pairs + (int64_t)pair * nt;
+    const int t0 = (int)(x - start), t1 = (int)min((int64_t)nt, x1 - start);
+    const int g = pair / a.chunks, h0 = g * a.group + (pair % a.chunks) * 8 * NH;
+    const int heads = min(8 * NH, (g + 1) * a.group - h0);  // query heads of this run
+
+    // Q in the operand's order of d; absent heads and d behind dim are zero
+    uint32_t qf[NH][DP / 8];
+#pragma unroll
+    for (int n = 0; n < NH; ++n) {
+      const uint16_t* qp = a.q + b * a.q_seq + (int64_t)(h0 + n * 8 + r) * a.q_head;
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i) {
+        // f16: 8 values at 32 i + 8 q; e4m3: the i-th half of 16 values at 64 (i / 2) + 16 q
+        const int d = S::kF16 ? i * 32 + q * 8 : (i / 2) * 64 + q * 16 + (i % 2) * 8;
+        const uint4 v = ldg16(qp + d, n * 8 + r < heads && d < c.dim);
+        qf[n][i * 4] = v.x;
+        qf[n][i * 4 + 1] = v.y;
+        qf[n][i * 4 + 2] = v.z;
+        qf[n][i * 4 + 3] = v.w;
+      }
+    }
+
+    float m[NH][2], l[NH][2], acc[S::MV][NH][4];
+#pragma unroll
+    for (int n = 0; n < NH; ++n) m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+    for (int j = 0; j < S::MV; ++j)
+#pragma unroll
+      for (int n = 0; n < NH; ++n) acc[j][n][0] = acc[j][n][1] = acc[j][n][2] = acc[j][n][3] = 0.f;
+
+    const int32_t* table = c.table + (int64_t)b * c.table_stride;
+    const int p0 = t0 * CT + warp * WT;                  // first position of this warp
+    const int p1 = (int)min((int64_t)t1 * CT, (int64_t)len);  // one past the run's last
+    // lane i stands for position p + i of the warp's tile: its page id, then
+    // the byte offset of its row (-1: absent) and its exponents
+    auto page_of = [&](int p) -> int {
+      const int pos = p + lane;
+      if (lane >= WT || pos >= p1) return -1;
+      return __ldg(table + c.div.div((uint32_t)pos));
+    };
+    auto row_of = [&](int p, int page, uint32_t* e) -> int64_t {
+      const int pos = p + lane;
+      *e = 127u | 127u << 8;
+      if (lane >= WT || pos >= p1) return -1;
+      if ((unsigned)page >= (uint64_t)c.pages) {
+        atomicOr(&uk::g_attn_decode_fault, UK_FAULT_PAGE);
+        return -1;
+      }
+      const int off = pos - (int)c.div.div((uint32_t)pos) * c.page_size;
+      if (!S::kF16) {
+        const int64_t at = uk_kv_exp(c, page, off, g);
+        *e = __ldg(c.k_exp + at) | (uint32_t)__ldg(c.v_exp + at) << 8;
+      }
+      return uk_kv_row(c, page, off, g);
+    };
+
+    uint4 kr[NT][2][S::KC];
+    uint32_t vr[NT][4][S::VC][S::VW];
+    unsigned seen = 0;  // bit 2 n + i: position 16 n + 8 i + r of the tile counts
+    auto load_k = [&](int64_t row) {
+      seen = 0;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int64_t at = __shfl_sync(0xffffffffu, row, n * 16 + i * 8 + r);
+          if (at >= 0) seen |= 1u << (2 * n + i);
+#pragma unroll
+          for (int k = 0; k < S::KC; ++k) {
+            const int d = S::kF16 ? k * 32 + q * 8 : k * 64 + q * 16;
+            kr[n][i][k] = ldg16(c.k + at + d * (S::kF16 ? 2 : 1), at >= 0 && d < c.dim);
+          }
+        }
+    };
+    auto load_v = [&](int64_t row) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int64_t at = __shfl_sync(0xffffffffu, row, n * 16 + (i >> 1) * 8 + 2 * q + (i & 1));
+#pragma unroll
+          for (int k = 0; k < S::VC; ++k) {
+            const int d = S::kF16 ? k * 64 + r * 8 : r * S::VB;
+            const uint8_t* p = c.v + at + d * (S::kF16 ? 2 : 1);
+            if (S::VB == 16) {
+              const uint4 v = ldg16(p, at >= 0 && d < c.dim);
+              vr[n][i][k][0] = v.x;
+              vr[n][i][k][1] = v.y;
+              vr[n][i][k][S::VW - 2] = v.z;
+              vr[n][i][k][S::VW - 1] = v.w;
+            } else {
+              const uint2 v = ldg8(p, at >= 0 && d < c.dim);
+              vr[n][i][k][0] = v.x;
+              vr[n][i][k][1] = v.y;
+            }
+          }
+        }
+    };
+
+    if (p0 < p1) {
+      uint32_t e, e_next = 0;
+      int page = page_of(p0);
+      int page_next = page_of(p0 + CT);
+      int64_t row = row_of(p0, page, &e);
+      load_k(row);
+      load_v(row);
+      for (int p = p0; p < p1; p += CT) {
+        // ---- S^T = K Q^T
+        float s[NT][NH][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int w = 0; w < NH; ++w) s[n][w][0] = s[n][w][1] = s[n][w][2] = s[n][w][3] = 0.f;
+#pragma unroll
+          for (int k = 0; k < S::KC; ++k) {
+            const uint4 x0_ = kr[n][0][k], x1_ = kr[n][1][k];
+            const uint32_t lo[4] = {x0_.x, x0_.y, x0_.z, x0_.w}, hi[4] = {x1_.x, x1_.y, x1_.z, x1_.w};
+            if (S::kF16) {
+#pragma unroll
+              for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int w = 0; w < NH; ++w)
+                  mma16816(s[n][w], lo[2 * i], hi[2 * i], lo[2 * i + 1], hi[2 * i + 1], qf[w][k * 4 + 2 * i],
+                           qf[w][k * 4 + 2 * i + 1]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const uint32_t a0 = uk_e4m3x2_to_half2(lo[i]), a1 = uk_e4m3x2_to_half2(hi[i]);
+                const uint32_t a2 = uk_e4m3x2_to_half2(lo[i] >> 16), a3 = uk_e4m3x2_to_half2(hi[i] >> 16);
+#pragma unroll
+                for (int w = 0; w < NH; ++w)
+                  mma16816(s[n][w], a0, a1, a2, a3, qf[w][k * 8 + 2 * i], qf[w][k * 8 + 2 * i + 1]);
+              }
+            }
+          }
+        }
+        const unsigned now = seen;
+        // ---- the next tile's rows and keys
+        const int64_t row_next = row_of(p + CT, page_next, &e_next);
+        page_next = page_of(p + 2 * CT);
+        load_k(row_next);
+
+        // ---- scores, reference and weights
+        float top[NH][2];
+#pragma unroll
+        for (int w = 0; w < NH; ++w) top[w][0] = top[w][1] = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float f = a.scale2;
+            if (!S::kF16) f *= uk_exp_scale(__shfl_sync(0xffffffffu, e, n * 16 + i * 8 + r) & 255u);
+            const bool on = now >> (2 * n + i) & 1u;
+#pragma unroll
+            for (int w = 0; w < NH; ++w)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                float& v = s[n][w][2 * i + h];
+                v = on ? v * f : -INFINITY;
+                top[w][h] = fmaxf(top[w][h], v);
+              }
+          }
+        bool grow = false;
+#pragma unroll
+        for (int w = 0; w < NH; ++w)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) grow |= top[w][h] > m[w][h] + GROW;
+        if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+          for (int w = 0; w < NH; ++w)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              float t = top[w][h];
+#pragma unroll
+              for (int o = 4; o < 32; o <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+              t = fmaxf(t, m[w][h]);
+              const float f = t == -INFINITY ? 1.f : ex2(m[w][h] - t);
+              m[w][h] = t;
+              l[w][h] *= f;
+#pragma unroll
+              for (int j = 0; j < S::MV; ++j) {
+                acc[j][w][h] *= f;
+                acc[j][w][2 + h] *= f;
+              }
+            }
+        }
+        uint32_t pf[NT][NH][2];
+#pragma unroll
+        for (int w = 0; w < NH; ++w) {
+          const float z0 = m[w][0] == -INFINITY ? 0.f : m[w][0] - SHIFT, z1 = m[w][1] == -INFINITY ? 0.f : m[w][1] - SHIFT;
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float a0 = ex2(s[n][w][2 * i] - z0), a1 = ex2(s[n][w][2 * i + 1] - z1);
+              l[w][0] += a0;
+              l[w][1] += a1;
+              pf[n][w][i] = transpose8(pack_half(a0, a1));
+            }
+        }
+
+        // ---- O^T += V^T P^T
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          if (S::kF16) {
+#pragma unroll
+            for (int k = 0; k < S::VC; ++k)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const uint32_t a0 = __byte_perm(vr[n][0][k][i], vr[n][1][k][i], 0x5410);
+                const uint32_t a1 = __byte_perm(vr[n][0][k][i], vr[n][1][k][i], 0x7632);
+                const uint32_t a2 = __byte_perm(vr[n][2][k][i], vr[n][3][k][i], 0x5410);
+                const uint32_t a3 = __byte_perm(vr[n][2][k][i], vr[n][3][k][i], 0x7632);
+#pragma unroll
+                for (int w = 0; w < NH; ++w) mma16816(acc[k * 4 + i][w], a0, a1, a2, a3, pf[n][w][0], pf[n][w][1]);
+              }
+          } else {
+            uint32_t sc[2];  // the scales of positions 2q, 2q + 1 and 2q + 8, 2q + 9
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t ea = __shfl_sync(0xffffffffu, e, n * 16 + i * 8 + 2 * q) >> 8;
+              const uint32_t eb = __shfl_sync(0xffffffffu, e, n * 16 + i * 8 + 2 * q + 1) >> 8;
+              sc[i] = pack_half(uk_exp_scale(ea), uk_exp_scale(eb));
+            }
+#pragma unroll
+            for (int i = 0; i < S::VW; ++i)
+#pragma unroll
+              for (int half = 0; half < 2; ++half) {
+                const uint32_t sel = half ? 0x7362 : 0x5140;
+                const uint32_t x = __byte_perm(vr[n][0][0][i], vr[n][1][0][i], sel);
+                const uint32_t y = __byte_perm(vr[n][2][0][i], vr[n][3][0][i], sel);
+                const uint32_t a0 = mul_half2(uk_e4m3x2_to_half2(x), sc[0]);
+                const uint32_t a1 = mul_half2(uk_e4m3x2_to_half2(x >> 16), sc[0]);
+                const uint32_t a2 = mul_half2(uk_e4m3x2_to_half2(y), sc[1]);
+                const uint32_t a3 = mul_half2(uk_e4m3x2_to_half2(y >> 16), sc[1]);
+#pragma unroll
+                for (int w = 0; w < NH; ++w)
+                  mma16816(acc[2 * i + half][w], a0, a1, a2, a3, pf[n][w][0], pf[n][w][1]);
+              }
+          }
+        }
+        load_v(row_next);
+        e = e_next;
+      }
+    }
+
+    // ---- the four warps' parts joined in shared memory
+#pragma unroll
+    for (int w = 0; w < NH; ++w)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float t = l[w][h];
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+        const int head = w * 8 + 2 * q + h;
+        if (r == 0) {
+          sm_m[warp][head] = m[w][h];
+          sm_l[warp][head] = t;
+        }
+#pragma unroll
+        for (int j = 0; j < S::MV; ++j) {
+          const int d = S::kF16 ? (j / 4) * 64 + r * 8 + (j % 4) * 2 : r * (DP / 8) + 2 * j;
+          *reinterpret_cast<float2*>(&sm_o[warp][head][d]) = make_float2(acc[j][w][h], acc[j][w][2 + h]);
+        }
+      }
+    __syncthreads();
+    const bool entered = t0 > 0, leaves = t1 < nt;
+    float* part = a.parts + ((int64_t)blockIdx.x * 2 + (entered ? 0 : 1)) * part_floats(DP, NH);
+    constexpr int LANES = DP / 8;  // threads per head, 8 values each
+    for (int i = threadIdx.x; i < heads * LANES; i += THREADS) {
+      const int head = i / LANES, d = (i % LANES) * 8;
+      float mm = -INFINITY, ll = 0.f, o[8];
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) mm = fmaxf(mm, sm_m[w][head]);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) o[k] = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        const float mw = sm_m[w][head];
+        // a warp without a reference has zero sums, or NaN ones that stay
+        const float f = mw == -INFINITY ? 1.f : ex2(mw - mm);
+        ll += sm_l[w][head] * f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) o[k] += sm_o[w][head][d + k] * f;
+      }
+      if (entered || leaves) {
+        if (d == 0) {
+          part[head] = mm;
+          part[8 * NH + head] = ll;
+        }
+        float4* dst = reinterpret_cast<float4*>(part + 16 * NH + head * DP + d);
+        dst[0] = make_float4(o[0], o[1], o[2], o[3]);
+        dst[1] = make_float4(o[4], o[5], o[6], o[7]);
+      } else {
+        const float inv = ll == 0.f ? 0.f : 1.f / ll;
+        if (d < c.dim)
+          *reinterpret_cast<uint4*>(a.o + b * a.o_seq + (int64_t)(h0 + head) * a.o_head + d) =
+              make_uint4(pack_half(o[0] * inv, o[1] * inv), pack_half(o[2] * inv, o[3] * inv),
+                         pack_half(o[4] * inv, o[5] * inv), pack_half(o[6] * inv, o[7] * inv));
+        if (a.lse != nullptr && d == 0)
+          a.lse[(int64_t)b * a.heads_q + h0 + head] = ll == 0.f ? -INFINITY : (mm - SHIFT + log2f(ll)) * LN2;
+      }
+    }
+    if (!entered && leaves) rec = make_int4(b, pair, (int)line.owner(start + nt - 1), 0);
+    __syncthreads();
+
+    x = start + t1;
+    if (x < x1 && ++pair == pairs) {
+      pair = 0;
+      before += nt;
+      do {
+        ++b;
+        len = clamped_len(a, room, b);
+        nt = (len + CT - 1) / CT;
+      } while (nt == 0);
+    }
+  }
+  if (threadIdx.x == 0) a.recs[blockIdx.x] = rec;
+}
+
+// One CTA per (first CTA of a cut pair, query head of its run): weights of the
+// parts, then their sum, a warp taking every fourth part.
+template <int DP, int NH>
+__global__ void __launch_bounds__(THREADS) k_attn_join(Args a, int dim) {
+  __shared__ float wt[MAX_CTAS];
+  __shared__ float red[33];
+  __shared__ float4 so[WARPS][32];
+  uk_pdl_wait();
+  const int first = blockIdx.x / (8 * NH), head = blockIdx.x % (8 * NH);
+  const int4 rec = a.recs[first];
+  const int b = rec.x, pair = rec.y, n = rec.z - first + 1;
+  if (b < 0) return;
+  const int g = pair / a.chunks, h = g * a.group + (pair % a.chunks) * 8 * NH + head;
+  if (h >= (g + 1) * a.group) return;
+  auto part = [&](int i) { return a.parts + ((int64_t)(first + i) * 2 + (i == 0 ? 1 : 0)) * part_floats(DP, NH); };
+  float mm = -INFINITY;
+  for (int i = threadIdx.x; i < n; i += THREADS) mm = fmaxf(mm, part(i)[head]);
+  mm = uk_block_max<THREADS>(mm, red);
+  float ll = 0.f;
+  for (int i = threadIdx.x; i < n; i += THREADS) {
+    const float mw = part(i)[head], f = mw == -INFINITY ? 1.f : ex2(mw - mm);
+    wt[i] = f;
+    ll += f * part(i)[8 * NH + head];
+  }
+  ll = uk_block_sum<THREADS>(ll, red);  // ends with a barrier: wt is complete
+  constexpr int LANES = DP / 4, PER = 32 / LANES;  // a warp takes PER parts at a time
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d4 = lane % LANES;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int i = warp * PER + lane / LANES; i < n; i += WARPS * PER) {
+    const float4 v = reinterpret_cast<const float4*>(part(i) + 16 * NH + head * DP)[d4];
+    const float f = wt[i];
+    o = make_float4(o.x + f * v.x, o.y + f * v.y, o.z + f * v.z, o.w + f * v.w);
+  }
   so[warp][lane] = o;
   __syncthreads();
-  if (warp != 0) return;
-  m = -INFINITY;
-  for (int w = 0; w < WARPS; ++w) m = fmaxf(m, sm[w]);
-  l = 0.f;
-  o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int w = 0; w < WARPS; ++w) {
-    const float f = sm[w] == -INFINITY ? (sl[w] != 0.f ? 1.f : 0.f) : exp2f(sm[w] - m);
-    const float4 x = so[w][lane];
-    l += sl[w] * f;
-    o = make_float4(o.x + x.x * f, o.y + x.y * f, o.z + x.z * f, o.w + x.w * f);
+  if (threadIdx.x < LANES) {
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int w = 0; w < WARPS; ++w)
+      for (int k = 0; k < PER; ++k) {
+        const float4 v = so[w][k * LANES + d4];
+        o = make_float4(o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w);
+      }
+    const float inv = ll == 0.f ? 0.f : 1.f / ll;
+    if (d4 * 4 < dim)
+      reinterpret_cast<uint2*>(a.o + b * a.o_seq + (int64_t)h * a.o_head)[d4] =
+          make_uint2(pack_half(o.x * inv, o.y * inv), pack_half(o.z * inv, o.w * inv));
+    if (a.lse != nullptr && d4 == 0)
+      a.lse[(int64_t)b * a.heads_q + h] = ll == 0.f ? -INFINITY : (mm - SHIFT + log2f(ll)) * LN2;
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  if (lane * 4 < c.dim) {
-    const __half2 x = __floats2half2_rn(o.x * inv, o.y * inv), y = __floats2half2_rn(o.z * inv, o.w * inv);
-    reinterpret_cast<uint2*>(a.o + b * a.o_seq + h * a.o_head)[lane] =
-        make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+}
+
+// ---- host side ------------------------------------------------------------------------
+
+// query heads per key head above 8 run as 16 wide: the cache is read once for
+// 16 of them, at twice the registers
+int heads_nh(int group) { return group > 8 ? 2 : 1; }
+int padded_dim(int dim) { return dim > 64 ? 128 : 64; }
+int ctas_per_sm(int nh) { return nh == 1 ? 3 : 2; }
+
+int grid_ctas(int nh) {
+  const int n = uk::sm_count() * ctas_per_sm(nh);
+  return n < MAX_CTAS ? n : MAX_CTAS;
+}
+
+size_t workspace_bytes_for(int ctas, int dp, int nh) {
+  return (size_t)ctas * (sizeof(int4) + 2 * sizeof(float) * part_floats(dp, nh));
+}
+
+template <int KIND, int DP, int NH>
+int launch(const Args& a, const UkKvView& c, int ctas, cudaStream_t st) {
+  k_attn_decode<KIND, DP, NH><<<(unsigned)ctas, THREADS, 0, st>>>(a, c);
+  if (int rc = uk::check_launch("attn_decode")) return rc;
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr{};
+  cfg.gridDim = dim3((unsigned)(ctas * 8 * NH), 1, 1);
+  cfg.blockDim = dim3(THREADS, 1, 1);
+  cfg.stream = st;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, k_attn_join<DP, NH>, a, c.dim);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return uk::fail(UK_ECUDA, "attn_decode: %s", cudaGetErrorString(e));
   }
-  if (a.lse != nullptr && lane == 0) a.lse[(int64_t)b * a.heads_q + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
+  return UK_OK;
 }
 
 }  // namespace
@@ -115,8 +647,9 @@ unsigned attn_decode_fault_take() {
 }  // namespace uk
 
 extern "C" size_t uk_cuda_attn_decode_workspace_size(int heads_q, int heads_kv, int dim) {
-  if (heads_q <= 0 || heads_kv <= 0 || dim <= 0) return 0;
-  return 16;
+  if (heads_q <= 0 || heads_kv <= 0 || dim <= 0 || dim > 128) return 0;
+  const int nh = heads_nh(heads_q / heads_kv);
+  return workspace_bytes_for(grid_ctas(nh), padded_dim(dim), nh);
 }
 
 extern "C" int uk_cuda_attn_decode_f16(const uint16_t* Q, int64_t q_seq_stride, int64_t q_head_stride,
@@ -131,18 +664,28 @@ extern "C" int uk_cuda_attn_decode_f16(const uint16_t* Q, int64_t q_seq_stride, 
   if (heads_q % cache->heads != 0)
     return uk::fail(UK_EINVAL, "attn_decode: %d query heads do not divide over %d key heads", heads_q, cache->heads);
   if (n_seq == 0) return UK_OK;
-  if ((int64_t)n_seq * heads_q > 0x7fffffff) return uk::fail(UK_EINVAL, "attn_decode: n_seq * heads_q exceeds the grid");
   if (int rc = uk::check_rows("attn_decode", "Q", Q, n_seq, heads_q, q_seq_stride, q_head_stride, 0)) return rc;
   if (int rc = uk::check_rows("attn_decode", "O", O, n_seq, heads_q, o_seq_stride, o_head_stride, cache->dim)) return rc;
   if (int rc = uk::check_device_ptr(seq_lens, "seq_lens")) return rc;
   if (LSE != nullptr)
     if (int rc = uk::check_device_ptr(LSE, "LSE")) return rc;
   if (int rc = uk::check_device_ptr(workspace, "workspace")) return rc;
-  const size_t need = uk_cuda_attn_decode_workspace_size(heads_q, cache->heads, cache->dim);
+  const int group = heads_q / cache->heads, nh = heads_nh(group), ctas = grid_ctas(nh), dp = padded_dim(cache->dim);
+  const size_t need = workspace_bytes_for(ctas, dp, nh);
   if (workspace_bytes < need || !uk::aligned16(workspace))
     return uk::fail(UK_EINVAL, "attn_decode: workspace of %zu bytes, %zu wanted, 16-byte aligned", workspace_bytes, need);
-  Args a{Q, q_seq_stride, q_head_stride, O, o_seq_stride, o_head_stride, LSE, seq_lens, n_seq, heads_q,
-         heads_q / cache->heads, scale * LOG2E};
-  k_attn_decode<<<(unsigned)(n_seq * heads_q), WARPS * 32, 0, (cudaStream_t)stream>>>(a, c);
-  return uk::check_launch("attn_decode");
+  Args a{Q, q_seq_stride, q_head_stride, O, o_seq_stride, o_head_stride, LSE, seq_lens, n_seq, heads_q, group,
+         (group + 8 * nh - 1) / (8 * nh), scale * LOG2E, nullptr, (int4*)workspace};
+  a.parts = reinterpret_cast<float*>(a.recs + ctas);
+  const cudaStream_t st = (cudaStream_t)stream;
+  switch ((cache->kind == UK_KV_E4M3 ? 4 : 0) + (dp == 128 ? 2 : 0) + (nh - 1)) {
+    case 0: return launch<UK_KV_F16, 64, 1>(a, c, ctas, st);
+    case 1: return launch<UK_KV_F16, 64, 2>(a, c, ctas, st);
+    case 2: return launch<UK_KV_F16, 128, 1>(a, c, ctas, st);
+    case 3: return launch<UK_KV_F16, 128, 2>(a, c, ctas, st);
+    case 4: return launch<UK_KV_E4M3, 64, 1>(a, c, ctas, st);
+    case 5: return launch<UK_KV_E4M3, 64, 2>(a, c, ctas, st);
+    case 6: return launch<UK_KV_E4M3, 128, 1>(a, c, ctas, st);
+    default: return launch<UK_KV_E4M3, 128, 2>(a, c, ctas, st);
+  }
 }

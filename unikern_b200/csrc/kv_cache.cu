@@ -162,7 +162,8 @@ int kv_view(const uk_kv_cache* c, const int32_t* table, int64_t table_stride, in
                 (long long)c->pages);
   if (max_pages < 0 || (n_seq > 1 && table_stride < max_pages))
     return fail(UK_EINVAL, "%s: max_pages %d, table_stride %lld", what, max_pages, (long long)table_stride);
-  if ((int64_t)max_pages * c->page_size > 0x7fffffff)
+  // kernels look some tiles ahead of the last position in 32 bits
+  if ((int64_t)max_pages * c->page_size > 0x7ffff000)
     return fail(UK_EINVAL, "%s: max_pages * page_size = %lld positions do not fit 31 bits", what,
                 (long long)max_pages * c->page_size);
   if ((c->pages > 1 && (c->page_stride < c->dim || c->page_stride % step != 0)) ||
