@@ -139,17 +139,18 @@ def test_decode_scales(scale):
         check_decode(pool, q, o, lse, scale)
 
 
-def test_decode_infinities_and_nan():
+@pytest.mark.parametrize("kind", ["f16", "e4m3"])
+def test_decode_infinities_and_nan(kind):
     """Held NaN and infinities reach exactly the heads and columns they should;
     a key of the type's lowest value takes no weight."""
     a = abi()
-    pool = Pool("f16", "hnd", 2, 32, 16, [40, 40, 40], seed=1)
+    pool = Pool(kind, "hnd", 2, 32, 16, [40, 40, 40], seed=1)
     q = randn(3, 4, 32, seed=2).abs() + 0.1
     low = torch.full((1, 2, 32), -65504.0, dtype=torch.float16, device="cuda")
     pool.values[0] = (pool.values[0][0].clone(), pool.values[0][1])
     pool.values[0][0][7:8] = pool.put(0, 0, 7, low)
     v = pool.values[1][1].half()
-    v[20, 1, 3], v[30, 1, 5] = math.inf, math.nan
+    v[20, 1, 3], v[30, 1, 5] = math.inf if kind == "f16" else math.nan, math.nan
     pool.values[1] = (pool.values[1][0], pool.put(1, 1, 0, v))
     k = pool.values[2][0].half()
     k[11, 0, 2] = math.nan

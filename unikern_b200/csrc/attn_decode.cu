@@ -25,14 +25,16 @@
 // O^T += V^T P^T, so a key head's query group fills the 8 columns instead of
 // padding 16 rows, and the fragments fit 16-byte loads by renaming the
 // contraction index:
-//   K (A operand, 16 x 16): lane (r = lane / 4, q = lane % 4) holds 16 bytes at
-//     d = 8 q (f16) or 16 q (e4m3) of positions r and r + 8; Q is loaded in the
-//     same order of d, so the sum over d is the same.
-//   V^T (A operand): lane (r, q) holds 16 bytes at d = 8 r (16 r) of positions
-//     2q, 2q + 1, 2q + 8, 2q + 9; a byte permute pairs neighbouring positions,
-//     as the operand packs them, and the row index d is renamed.
+//   K (A operand): lane (r = lane / 4, q = lane % 4) holds 16 bytes at byte
+//     16 q of positions r and r + 8; Q is loaded in the same order of d, so
+//     the sum over d is the same.
+//   V^T (A operand): lane (r, q) holds 16 bytes at byte 16 r of positions 2q,
+//     2q + 1, 2q + 8, 2q + 9; a byte permute pairs neighbouring positions, as
+//     the operand packs them, and the row index d is renamed.
 //   P^T (B operand): the S^T accumulator has position and head exchanged; an
 //     8 x 8 transpose between lanes (movmatrix) puts that right.
+// e4m3 rows are converted to binary16 in registers, exactly; the keys' scale
+// multiplies the score, the values' goes into the weight's exponent.
 // K of the next tile loads while the softmax and V product of this one run,
 // then V of the next; page ids load one tile earlier still.
 #include "kv_cache.cuh"
@@ -60,7 +62,11 @@ struct Args {
   int chunks;                 // runs of 8 NH query heads per key head
   float scale2;               // scale * log2 e
   float* parts;               // [ctas][2][part_floats]
-  int4* recs;                 // [ctas]: pair left unfinished {b, pair, last CTA, -}, b = -1: none
+  // a pair cut by the end of its first CTA's run: {b, pair, first CTA, last
+  // CTA}, b = -1: none; one per pair where there are no more pairs than CTAs
+  // (by_pair), else one per CTA
+  int4* recs;
+  int by_pair;
 };
 
 template <int KIND, int DP>
@@ -110,10 +116,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
-  const __half2 r = __hmul2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
 }
 __device__ __forceinline__ float ex2(float x) {
   float r;
@@ -186,7 +188,12 @@ __device__ Line find_begin(const Args& a, int64_t room, int pairs, int64_t* x0, 
 }
 
 // ---- the kernel -----------------------------------------------------------------------
-template <int KIND, int DP, int NH>
+// kWhole: page_size is a multiple of 16, so a group of 16 positions lies in one
+// page and its rows are one address apart; otherwise every position's row is
+// looked up by one lane and passed to the others (32 x 8192 f16 positions: 173
+// against 186 us).  e4m3 takes the second form always: its exponents are looked
+// up by position in any case (ragged 32 x 8192: 68 against 79 us with kWhole).
+template <int KIND, int DP, int NH, bool kWhole>
 __global__ void __launch_bounds__(THREADS, NH == 1 ? 3 : 2) k_attn_decode(Args a, UkKvView c) {
   using S = Shape<KIND, DP>;
   constexpr int CT = S::CT, WT = S::WT, NT = S::NT;
@@ -209,17 +216,19 @@ __global__ void __launch_bounds__(THREADS, NH == 1 ? 3 : 2) k_attn_decode(Args a
     }
     if (a.lse != nullptr)
       for (int h = threadIdx.x; h < a.heads_q; h += THREADS) a.lse[(int64_t)b * a.heads_q + h] = -INFINITY;
+    if (a.by_pair)
+      for (int i = threadIdx.x; i < pairs; i += THREADS) a.recs[b * pairs + i] = make_int4(-1, 0, 0, 0);
   }
 
   int64_t x0, x1, before;
   int b;
   const Line line = find_begin<CT>(a, room, pairs, &x0, &x1, &b, &before);
+  int4 rec = make_int4(-1, 0, 0, 0);
   if (x0 >= x1) {
-    if (threadIdx.x == 0) a.recs[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    if (threadIdx.x == 0 && !a.by_pair) a.recs[blockIdx.x] = rec;
     return;
   }
 
-  int4 rec = make_int4(-1, 0, 0, 0);
   int64_t x = x0;
   int len = clamped_len(a, room, b), nt = (len + CT - 1) / CT;
   int pair = (int)((x - before * pairs) / nt);
@@ -228,6 +237,108 @@ __global__ void __launch_bounds__(THREADS, NH == 1 ? 3 : 2) k_attn_decode(Args a
     const int t0 = (int)(x - start), t1 = (int)min((int64_t)nt, x1 - start);
     const int g = pair / a.chunks, h0 = g * a.group + (pair % a.chunks) * 8 * NH;
     const int heads = min(8 * NH, (g + 1) * a.group - h0);  // query heads of this run
+
+    const int32_t* table = c.table + (int64_t)b * c.table_stride;
+    const int p0 = t0 * CT + warp * WT;                       // first position of this warp
+    const int p1 = (int)min((int64_t)t1 * CT, (int64_t)len);  // one past the run's last
+
+    // The rows of a warp tile at p.  kWhole: group n's page id and then the
+    // byte offset of its first row, the same in every lane; else lane i's own
+    // for position p + i.  -1: absent.  e: position p + lane's exponent bytes,
+    // the key's below the value's.
+    constexpr int NR = kWhole ? NT : 1;
+    struct Where {
+      int64_t row[NR];
+    };
+    auto page_of = [&](int p, int (&page)[NR]) {
+#pragma unroll
+      for (int n = 0; n < NR; ++n) {
+        const int pos = kWhole ? p + n * 16 : p + lane;
+        page[n] = pos < p1 && (kWhole || lane < WT) ? __ldg(table + c.div.div((uint32_t)pos)) : -1;
+      }
+    };
+    auto rows_of = [&](int p, const int (&page)[NR], uint32_t* e) {
+      Where w;
+      *e = 127u | 127u << 8;
+#pragma unroll
+      for (int n = 0; n < NR; ++n) {
+        const int pos = kWhole ? p + n * 16 : p + lane;
+        w.row[n] = -1;
+        if (pos < p1 && (kWhole || lane < WT)) {
+          if ((unsigned)page[n] < (uint64_t)c.pages) {
+            const int off = pos - (int)c.div.div((uint32_t)pos) * c.page_size;
+            w.row[n] = uk_kv_row(c, page[n], off, g);
+            if (!S::kF16) {
+              const int64_t at = uk_kv_exp(c, page[n], off, g);
+              *e = __ldg(c.k_exp + at) | (uint32_t)__ldg(c.v_exp + at) << 8;
+            }
+          } else {
+            atomicOr(&uk::g_attn_decode_fault, UK_FAULT_PAGE);
+          }
+        }
+      }
+      return w;
+    };
+    // the row of position p + n * 16 + i, or -1
+    auto row_at = [&](const Where& w, int p, int n, int i) -> int64_t {
+      if (kWhole) return w.row[n] < 0 || p + n * 16 + i >= p1 ? -1 : w.row[n] + (int64_t)i * c.token_bytes;
+      return __shfl_sync(0xffffffffu, w.row[0], n * 16 + i);
+    };
+
+    uint4 kr[NT][2][S::KC];
+    uint32_t vr[NT][4][S::VC][S::VW];
+    unsigned seen = 0;  // bit 2 n + i: position 16 n + 8 i + r of the tile counts
+    auto load_k = [&](const Where& w, int p) {
+      seen = 0;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int64_t at = row_at(w, p, n, i * 8 + r);
+          if (at >= 0) seen |= 1u << (2 * n + i);
+          const uint8_t* kp = c.k + at + q * 16;
+#pragma unroll
+          for (int k = 0; k < S::KC; ++k)
+            kr[n][i][k] = ldg16(kp + k * 64, at >= 0 && (k * 64 + q * 16) / (S::kF16 ? 2 : 1) < c.dim);
+        }
+    };
+    auto load_v = [&](const Where& w, int p) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int64_t at = row_at(w, p, n, (i >> 1) * 8 + 2 * q + (i & 1));
+          const uint8_t* vp = c.v + at + r * S::VB;
+#pragma unroll
+          for (int k = 0; k < S::VC; ++k) {
+            const bool on = at >= 0 && (k * 128 + r * S::VB) / (S::kF16 ? 2 : 1) < c.dim;
+            if (S::VB == 16) {
+              const uint4 v = ldg16(vp + k * 128, on);
+              vr[n][i][k][0] = v.x;
+              vr[n][i][k][1] = v.y;
+              vr[n][i][k][S::VW - 2] = v.z;
+              vr[n][i][k][S::VW - 1] = v.w;
+            } else {
+              const uint2 v = ldg8(vp + k * 128, on);
+              vr[n][i][k][0] = v.x;
+              vr[n][i][k][1] = v.y;
+            }
+          }
+        }
+    };
+
+    // the first tile's loads go out before Q is brought into shape
+    uint32_t e, e_next = 0;
+    int page_next[NR];
+    Where rows;
+    if (p0 < p1) {
+      int page[NR];
+      page_of(p0, page);
+      page_of(p0 + CT, page_next);
+      rows = rows_of(p0, page, &e);
+      load_k(rows, p0);
+      load_v(rows, p0);
+    }
 
     // Q in the operand's order of d; absent heads and d behind dim are zero
     uint32_t qf[NH][DP / 8];
@@ -239,10 +350,7 @@ __global__ void __launch_bounds__(THREADS, NH == 1 ? 3 : 2) k_attn_decode(Args a
         // f16: 8 values at 32 i + 8 q; e4m3: the i-th half of 16 values at 64 (i / 2) + 16 q
         const int d = S::kF16 ? i * 32 + q * 8 : (i / 2) * 64 + q * 16 + (i % 2) * 8;
         const uint4 v = ldg16(qp + d, n * 8 + r < heads && d < c.dim);
-        qf[n][i * 4] = v.x;
-        qf[n][i * 4 + 1] = v.y;
-        qf[n][i * 4 + 2] = v.z;
-        qf[n][i * 4 + 3] = v.w;
+        qf[n][i * 4] = v.x, qf[n][i * 4 + 1] = v.y, qf[n][i * 4 + 2] = v.z, qf[n][i * 4 + 3] = v.w;
       }
     }
 
@@ -254,220 +362,146 @@ __global__ void __launch_bounds__(THREADS, NH == 1 ? 3 : 2) k_attn_decode(Args a
 #pragma unroll
       for (int n = 0; n < NH; ++n) acc[j][n][0] = acc[j][n][1] = acc[j][n][2] = acc[j][n][3] = 0.f;
 
-    const int32_t* table = c.table + (int64_t)b * c.table_stride;
-    const int p0 = t0 * CT + warp * WT;                  // first position of this warp
-    const int p1 = (int)min((int64_t)t1 * CT, (int64_t)len);  // one past the run's last
-    // lane i stands for position p + i of the warp's tile: its page id, then
-    // the byte offset of its row (-1: absent) and its exponents
-    auto page_of = [&](int p) -> int {
-      const int pos = p + lane;
-      if (lane >= WT || pos >= p1) return -1;
-      return __ldg(table + c.div.div((uint32_t)pos));
-    };
-    auto row_of = [&](int p, int page, uint32_t* e) -> int64_t {
-      const int pos = p + lane;
-      *e = 127u | 127u << 8;
-      if (lane >= WT || pos >= p1) return -1;
-      if ((unsigned)page >= (uint64_t)c.pages) {
-        atomicOr(&uk::g_attn_decode_fault, UK_FAULT_PAGE);
-        return -1;
+    for (int p = p0; p < p1; p += CT) {
+      // ---- S^T = K Q^T
+      float s[NT][NH][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int w = 0; w < NH; ++w) s[n][w][0] = s[n][w][1] = s[n][w][2] = s[n][w][3] = 0.f;
+        if (S::kF16) {
+#pragma unroll
+          for (int k = 0; k < S::KC; ++k) {
+            const uint4 lo = kr[n][0][k], hi = kr[n][1][k];
+#pragma unroll
+            for (int w = 0; w < NH; ++w) {
+              mma16816(s[n][w], lo.x, hi.x, lo.y, hi.y, qf[w][k * 4], qf[w][k * 4 + 1]);
+              mma16816(s[n][w], lo.z, hi.z, lo.w, hi.w, qf[w][k * 4 + 2], qf[w][k * 4 + 3]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < S::KC; ++k) {
+            const uint32_t lo[4] = {kr[n][0][k].x, kr[n][0][k].y, kr[n][0][k].z, kr[n][0][k].w};
+            const uint32_t hi[4] = {kr[n][1][k].x, kr[n][1][k].y, kr[n][1][k].z, kr[n][1][k].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t a0, a1, a2, a3;
+              uk_e4m3x4_to_half2(lo[i], &a0, &a2);
+              uk_e4m3x4_to_half2(hi[i], &a1, &a3);
+#pragma unroll
+              for (int w = 0; w < NH; ++w)
+                mma16816(s[n][w], a0, a1, a2, a3, qf[w][k * 8 + 2 * i], qf[w][k * 8 + 2 * i + 1]);
+            }
+          }
+        }
       }
-      const int off = pos - (int)c.div.div((uint32_t)pos) * c.page_size;
-      if (!S::kF16) {
-        const int64_t at = uk_kv_exp(c, page, off, g);
-        *e = __ldg(c.k_exp + at) | (uint32_t)__ldg(c.v_exp + at) << 8;
-      }
-      return uk_kv_row(c, page, off, g);
-    };
+      const unsigned now = seen;
+      // ---- the next tile's rows and keys
+      rows = rows_of(p + CT, page_next, &e_next);
+      page_of(p + 2 * CT, page_next);
+      load_k(rows, p + CT);
 
-    uint4 kr[NT][2][S::KC];
-    uint32_t vr[NT][4][S::VC][S::VW];
-    unsigned seen = 0;  // bit 2 n + i: position 16 n + 8 i + r of the tile counts
-    auto load_k = [&](int64_t row) {
-      seen = 0;
+      // ---- scores, reference and weights.  e4m3: the value row's scale 2^ev
+      // goes into the weight's exponent, t = s + ev, and the codes enter the
+      // product unscaled; l takes 2^(t - m) 2^-ev in fp32.
+      float top[NH][2], inv_ev[NT][2];
+#pragma unroll
+      for (int w = 0; w < NH; ++w) top[w][0] = top[w][1] = -INFINITY;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const int64_t at = __shfl_sync(0xffffffffu, row, n * 16 + i * 8 + r);
-          if (at >= 0) seen |= 1u << (2 * n + i);
-#pragma unroll
-          for (int k = 0; k < S::KC; ++k) {
-            const int d = S::kF16 ? k * 32 + q * 8 : k * 64 + q * 16;
-            kr[n][i][k] = ldg16(c.k + at + d * (S::kF16 ? 2 : 1), at >= 0 && d < c.dim);
+          float f = 1.f, add = 0.f;
+          if (!S::kF16) {
+            const uint32_t y = __shfl_sync(0xffffffffu, e, n * 16 + i * 8 + r);
+            f = a.scale2 * uk_exp_scale(y & 255u);
+            add = (float)((int)(y >> 8) - 127);
+            inv_ev[n][i] = uk_exp_scale(254u - (y >> 8));
           }
-        }
-    };
-    auto load_v = [&](int64_t row) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int64_t at = __shfl_sync(0xffffffffu, row, n * 16 + (i >> 1) * 8 + 2 * q + (i & 1));
-#pragma unroll
-          for (int k = 0; k < S::VC; ++k) {
-            const int d = S::kF16 ? k * 64 + r * 8 : r * S::VB;
-            const uint8_t* p = c.v + at + d * (S::kF16 ? 2 : 1);
-            if (S::VB == 16) {
-              const uint4 v = ldg16(p, at >= 0 && d < c.dim);
-              vr[n][i][k][0] = v.x;
-              vr[n][i][k][1] = v.y;
-              vr[n][i][k][S::VW - 2] = v.z;
-              vr[n][i][k][S::VW - 1] = v.w;
-            } else {
-              const uint2 v = ldg8(p, at >= 0 && d < c.dim);
-              vr[n][i][k][0] = v.x;
-              vr[n][i][k][1] = v.y;
-            }
-          }
-        }
-    };
-
-    if (p0 < p1) {
-      uint32_t e, e_next = 0;
-      int page = page_of(p0);
-      int page_next = page_of(p0 + CT);
-      int64_t row = row_of(p0, page, &e);
-      load_k(row);
-      load_v(row);
-      for (int p = p0; p < p1; p += CT) {
-        // ---- S^T = K Q^T
-        float s[NT][NH][4];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-#pragma unroll
-          for (int w = 0; w < NH; ++w) s[n][w][0] = s[n][w][1] = s[n][w][2] = s[n][w][3] = 0.f;
-#pragma unroll
-          for (int k = 0; k < S::KC; ++k) {
-            const uint4 x0_ = kr[n][0][k], x1_ = kr[n][1][k];
-            const uint32_t lo[4] = {x0_.x, x0_.y, x0_.z, x0_.w}, hi[4] = {x1_.x, x1_.y, x1_.z, x1_.w};
-            if (S::kF16) {
-#pragma unroll
-              for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int w = 0; w < NH; ++w)
-                  mma16816(s[n][w], lo[2 * i], hi[2 * i], lo[2 * i + 1], hi[2 * i + 1], qf[w][k * 4 + 2 * i],
-                           qf[w][k * 4 + 2 * i + 1]);
-            } else {
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const uint32_t a0 = uk_e4m3x2_to_half2(lo[i]), a1 = uk_e4m3x2_to_half2(hi[i]);
-                const uint32_t a2 = uk_e4m3x2_to_half2(lo[i] >> 16), a3 = uk_e4m3x2_to_half2(hi[i] >> 16);
-#pragma unroll
-                for (int w = 0; w < NH; ++w)
-                  mma16816(s[n][w], a0, a1, a2, a3, qf[w][k * 8 + 2 * i], qf[w][k * 8 + 2 * i + 1]);
-              }
-            }
-          }
-        }
-        const unsigned now = seen;
-        // ---- the next tile's rows and keys
-        const int64_t row_next = row_of(p + CT, page_next, &e_next);
-        page_next = page_of(p + 2 * CT);
-        load_k(row_next);
-
-        // ---- scores, reference and weights
-        float top[NH][2];
-#pragma unroll
-        for (int w = 0; w < NH; ++w) top[w][0] = top[w][1] = -INFINITY;
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            float f = a.scale2;
-            if (!S::kF16) f *= uk_exp_scale(__shfl_sync(0xffffffffu, e, n * 16 + i * 8 + r) & 255u);
-            const bool on = now >> (2 * n + i) & 1u;
-#pragma unroll
-            for (int w = 0; w < NH; ++w)
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                float& v = s[n][w][2 * i + h];
-                v = on ? v * f : -INFINITY;
-                top[w][h] = fmaxf(top[w][h], v);
-              }
-          }
-        bool grow = false;
-#pragma unroll
-        for (int w = 0; w < NH; ++w)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) grow |= top[w][h] > m[w][h] + GROW;
-        if (__any_sync(0xffffffffu, grow)) {
+          const bool on = now >> (2 * n + i) & 1u;
 #pragma unroll
           for (int w = 0; w < NH; ++w)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              float t = top[w][h];
-#pragma unroll
-              for (int o = 4; o < 32; o <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
-              t = fmaxf(t, m[w][h]);
-              const float f = t == -INFINITY ? 1.f : ex2(m[w][h] - t);
-              m[w][h] = t;
-              l[w][h] *= f;
-#pragma unroll
-              for (int j = 0; j < S::MV; ++j) {
-                acc[j][w][h] *= f;
-                acc[j][w][2 + h] *= f;
-              }
+              float& v = s[n][w][2 * i + h];
+              v = on ? (S::kF16 ? v * a.scale2 : fmaf(v, f, add)) : -INFINITY;
+              top[w][h] = fmaxf(top[w][h], v);
             }
         }
-        uint32_t pf[NT][NH][2];
+      bool grow = false;
 #pragma unroll
-        for (int w = 0; w < NH; ++w) {
-          const float z0 = m[w][0] == -INFINITY ? 0.f : m[w][0] - SHIFT, z1 = m[w][1] == -INFINITY ? 0.f : m[w][1] - SHIFT;
+      for (int w = 0; w < NH; ++w)
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
+        for (int h = 0; h < 2; ++h) grow |= top[w][h] > m[w][h] + GROW;
+      if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const float a0 = ex2(s[n][w][2 * i] - z0), a1 = ex2(s[n][w][2 * i + 1] - z1);
-              l[w][0] += a0;
-              l[w][1] += a1;
-              pf[n][w][i] = transpose8(pack_half(a0, a1));
+        for (int w = 0; w < NH; ++w)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float t = top[w][h];
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+            t = fmaxf(t, m[w][h]);
+            const float f = t == -INFINITY ? 1.f : ex2(m[w][h] - t);
+            m[w][h] = t;
+            l[w][h] *= f;
+#pragma unroll
+            for (int j = 0; j < S::MV; ++j) {
+              acc[j][w][h] *= f;
+              acc[j][w][2 + h] *= f;
             }
-        }
-
-        // ---- O^T += V^T P^T
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          if (S::kF16) {
-#pragma unroll
-            for (int k = 0; k < S::VC; ++k)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const uint32_t a0 = __byte_perm(vr[n][0][k][i], vr[n][1][k][i], 0x5410);
-                const uint32_t a1 = __byte_perm(vr[n][0][k][i], vr[n][1][k][i], 0x7632);
-                const uint32_t a2 = __byte_perm(vr[n][2][k][i], vr[n][3][k][i], 0x5410);
-                const uint32_t a3 = __byte_perm(vr[n][2][k][i], vr[n][3][k][i], 0x7632);
-#pragma unroll
-                for (int w = 0; w < NH; ++w) mma16816(acc[k * 4 + i][w], a0, a1, a2, a3, pf[n][w][0], pf[n][w][1]);
-              }
-          } else {
-            uint32_t sc[2];  // the scales of positions 2q, 2q + 1 and 2q + 8, 2q + 9
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const uint32_t ea = __shfl_sync(0xffffffffu, e, n * 16 + i * 8 + 2 * q) >> 8;
-              const uint32_t eb = __shfl_sync(0xffffffffu, e, n * 16 + i * 8 + 2 * q + 1) >> 8;
-              sc[i] = pack_half(uk_exp_scale(ea), uk_exp_scale(eb));
-            }
-#pragma unroll
-            for (int i = 0; i < S::VW; ++i)
-#pragma unroll
-              for (int half = 0; half < 2; ++half) {
-                const uint32_t sel = half ? 0x7362 : 0x5140;
-                const uint32_t x = __byte_perm(vr[n][0][0][i], vr[n][1][0][i], sel);
-                const uint32_t y = __byte_perm(vr[n][2][0][i], vr[n][3][0][i], sel);
-                const uint32_t a0 = mul_half2(uk_e4m3x2_to_half2(x), sc[0]);
-                const uint32_t a1 = mul_half2(uk_e4m3x2_to_half2(x >> 16), sc[0]);
-                const uint32_t a2 = mul_half2(uk_e4m3x2_to_half2(y), sc[1]);
-                const uint32_t a3 = mul_half2(uk_e4m3x2_to_half2(y >> 16), sc[1]);
-#pragma unroll
-                for (int w = 0; w < NH; ++w)
-                  mma16816(acc[2 * i + half][w], a0, a1, a2, a3, pf[n][w][0], pf[n][w][1]);
-              }
           }
-        }
-        load_v(row_next);
-        e = e_next;
       }
+      uint32_t pf[NT][NH][2];
+#pragma unroll
+      for (int w = 0; w < NH; ++w) {
+        const float z0 = m[w][0] == -INFINITY ? 0.f : m[w][0] - SHIFT, z1 = m[w][1] == -INFINITY ? 0.f : m[w][1] - SHIFT;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float a0 = ex2(s[n][w][2 * i] - z0), a1 = ex2(s[n][w][2 * i + 1] - z1);
+            l[w][0] += S::kF16 ? a0 : a0 * inv_ev[n][i];
+            l[w][1] += S::kF16 ? a1 : a1 * inv_ev[n][i];
+            pf[n][w][i] = transpose8(pack_half(a0, a1));
+          }
+      }
+
+      // ---- O^T += V^T P^T
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        if (S::kF16) {
+#pragma unroll
+          for (int k = 0; k < S::VC; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t a0 = __byte_perm(vr[n][0][k][i], vr[n][1][k][i], 0x5410);
+              const uint32_t a1 = __byte_perm(vr[n][0][k][i], vr[n][1][k][i], 0x7632);
+              const uint32_t a2 = __byte_perm(vr[n][2][k][i], vr[n][3][k][i], 0x5410);
+              const uint32_t a3 = __byte_perm(vr[n][2][k][i], vr[n][3][k][i], 0x7632);
+#pragma unroll
+              for (int w = 0; w < NH; ++w) mma16816(acc[k * 4 + i][w], a0, a1, a2, a3, pf[n][w][0], pf[n][w][1]);
+            }
+        } else {
+#pragma unroll
+          for (int i = 0; i < S::VW; ++i)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const uint32_t sel = half ? 0x7362 : 0x5140;
+              const uint32_t y0 = __byte_perm(vr[n][0][0][i], vr[n][1][0][i], sel);
+              const uint32_t y1 = __byte_perm(vr[n][2][0][i], vr[n][3][0][i], sel);
+              uint32_t a0, a1, a2, a3;
+              uk_e4m3x4_to_half2(y0, &a0, &a1);
+              uk_e4m3x4_to_half2(y1, &a2, &a3);
+#pragma unroll
+              for (int w = 0; w < NH; ++w)
+                mma16816(acc[2 * i + half][w], a0, a1, a2, a3, pf[n][w][0], pf[n][w][1]);
+            }
+        }
+      }
+      load_v(rows, p + CT);
+      e = e_next;
     }
 
     // ---- the four warps' parts joined in shared memory
@@ -527,7 +561,10 @@ __global__ void __launch_bounds__(THREADS, NH == 1 ? 3 : 2) k_attn_decode(Args a
           a.lse[(int64_t)b * a.heads_q + h0 + head] = ll == 0.f ? -INFINITY : (mm - SHIFT + log2f(ll)) * LN2;
       }
     }
-    if (!entered && leaves) rec = make_int4(b, pair, (int)line.owner(start + nt - 1), 0);
+    if (!entered) {
+      if (leaves) rec = make_int4(b, pair, blockIdx.x, (int)line.owner(start + nt - 1));
+      if (a.by_pair && threadIdx.x == 0) a.recs[b * pairs + pair] = leaves ? rec : make_int4(-1, 0, 0, 0);
+    }
     __syncthreads();
 
     x = start + t1;
@@ -541,39 +578,40 @@ __global__ void __launch_bounds__(THREADS, NH == 1 ? 3 : 2) k_attn_decode(Args a
       } while (nt == 0);
     }
   }
-  if (threadIdx.x == 0) a.recs[blockIdx.x] = rec;
+  if (threadIdx.x == 0 && !a.by_pair) a.recs[blockIdx.x] = rec;
 }
 
-// One CTA per (first CTA of a cut pair, query head of its run): weights of the
-// parts, then their sum, a warp taking every fourth part.
-template <int DP, int NH>
-__global__ void __launch_bounds__(THREADS) k_attn_join(Args a, int dim) {
+// One CTA per (cut pair, query head of its run): weights of the parts, then
+// their sum, the warps taking turns.
+template <int DP, int NH, int JT>
+__global__ void __launch_bounds__(JT) k_attn_join(Args a, int dim) {
+  constexpr int JW = JT / 32;
   __shared__ float wt[MAX_CTAS];
   __shared__ float red[33];
-  __shared__ float4 so[WARPS][32];
+  __shared__ float4 so[JW][32];
   uk_pdl_wait();
-  const int first = blockIdx.x / (8 * NH), head = blockIdx.x % (8 * NH);
-  const int4 rec = a.recs[first];
-  const int b = rec.x, pair = rec.y, n = rec.z - first + 1;
+  const int head = blockIdx.x % (8 * NH);
+  const int4 rec = a.recs[blockIdx.x / (8 * NH)];
+  const int b = rec.x, pair = rec.y, first = rec.z, n = rec.w - first + 1;
   if (b < 0) return;
   const int g = pair / a.chunks, h = g * a.group + (pair % a.chunks) * 8 * NH + head;
   if (h >= (g + 1) * a.group) return;
   auto part = [&](int i) { return a.parts + ((int64_t)(first + i) * 2 + (i == 0 ? 1 : 0)) * part_floats(DP, NH); };
   float mm = -INFINITY;
-  for (int i = threadIdx.x; i < n; i += THREADS) mm = fmaxf(mm, part(i)[head]);
-  mm = uk_block_max<THREADS>(mm, red);
+  for (int i = threadIdx.x; i < n; i += JT) mm = fmaxf(mm, part(i)[head]);
+  mm = uk_block_max<JT>(mm, red);
   float ll = 0.f;
-  for (int i = threadIdx.x; i < n; i += THREADS) {
+  for (int i = threadIdx.x; i < n; i += JT) {
     const float mw = part(i)[head], f = mw == -INFINITY ? 1.f : ex2(mw - mm);
     wt[i] = f;
     ll += f * part(i)[8 * NH + head];
   }
-  ll = uk_block_sum<THREADS>(ll, red);  // ends with a barrier: wt is complete
+  ll = uk_block_sum<JT>(ll, red);  // ends with a barrier: wt is complete
   constexpr int LANES = DP / 4, PER = 32 / LANES;  // a warp takes PER parts at a time
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d4 = lane % LANES;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-  for (int i = warp * PER + lane / LANES; i < n; i += WARPS * PER) {
+#pragma unroll 4
+  for (int i = warp * PER + lane / LANES; i < n; i += JW * PER) {
     const float4 v = reinterpret_cast<const float4*>(part(i) + 16 * NH + head * DP)[d4];
     const float f = wt[i];
     o = make_float4(o.x + f * v.x, o.y + f * v.y, o.z + f * v.z, o.w + f * v.w);
@@ -582,7 +620,9 @@ __global__ void __launch_bounds__(THREADS) k_attn_join(Args a, int dim) {
   __syncthreads();
   if (threadIdx.x < LANES) {
     o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int w = 0; w < WARPS; ++w)
+#pragma unroll
+    for (int w = 0; w < JW; ++w)
+#pragma unroll
       for (int k = 0; k < PER; ++k) {
         const float4 v = so[w][k * LANES + d4];
         o = make_float4(o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w);
@@ -613,25 +653,37 @@ size_t workspace_bytes_for(int ctas, int dp, int nh) {
   return (size_t)ctas * (sizeof(int4) + 2 * sizeof(float) * part_floats(dp, nh));
 }
 
-template <int KIND, int DP, int NH>
-int launch(const Args& a, const UkKvView& c, int ctas, cudaStream_t st) {
-  k_attn_decode<KIND, DP, NH><<<(unsigned)ctas, THREADS, 0, st>>>(a, c);
-  if (int rc = uk::check_launch("attn_decode")) return rc;
+template <int DP, int NH>
+int launch_join(const Args& a, int dim, int ctas, cudaStream_t st) {
+  const int64_t all = (int64_t)a.n_seq * (a.heads_q / a.group) * a.chunks;
+  // 16 warps where a pair can have more parts than four warps keep in flight
+  const bool wide = a.by_pair && ctas / all >= 16;
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr{};
-  cfg.gridDim = dim3((unsigned)(ctas * 8 * NH), 1, 1);
-  cfg.blockDim = dim3(THREADS, 1, 1);
+  cfg.gridDim = dim3((unsigned)((a.by_pair ? all : ctas) * 8 * NH), 1, 1);
+  cfg.blockDim = dim3(wide ? 512 : THREADS, 1, 1);
   cfg.stream = st;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, k_attn_join<DP, NH>, a, c.dim);
+  const cudaError_t e = wide ? cudaLaunchKernelEx(&cfg, k_attn_join<DP, NH, 512>, a, dim)
+                             : cudaLaunchKernelEx(&cfg, k_attn_join<DP, NH, THREADS>, a, dim);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return uk::fail(UK_ECUDA, "attn_decode: %s", cudaGetErrorString(e));
   }
   return UK_OK;
+}
+
+template <int KIND, int DP, int NH>
+int launch(const Args& a, const UkKvView& c, int ctas, cudaStream_t st) {
+  bool whole = false;
+  if constexpr (KIND == UK_KV_F16)
+    if ((whole = c.page_size % 16 == 0)) k_attn_decode<KIND, DP, NH, true><<<(unsigned)ctas, THREADS, 0, st>>>(a, c);
+  if (!whole) k_attn_decode<KIND, DP, NH, false><<<(unsigned)ctas, THREADS, 0, st>>>(a, c);
+  if (int rc = uk::check_launch("attn_decode")) return rc;
+  return launch_join<DP, NH>(a, c.dim, ctas, st);
 }
 
 }  // namespace
@@ -675,7 +727,8 @@ extern "C" int uk_cuda_attn_decode_f16(const uint16_t* Q, int64_t q_seq_stride, 
   if (workspace_bytes < need || !uk::aligned16(workspace))
     return uk::fail(UK_EINVAL, "attn_decode: workspace of %zu bytes, %zu wanted, 16-byte aligned", workspace_bytes, need);
   Args a{Q, q_seq_stride, q_head_stride, O, o_seq_stride, o_head_stride, LSE, seq_lens, n_seq, heads_q, group,
-         (group + 8 * nh - 1) / (8 * nh), scale * LOG2E, nullptr, (int4*)workspace};
+         (group + 8 * nh - 1) / (8 * nh), scale * LOG2E, nullptr, (int4*)workspace, 0};
+  a.by_pair = (int64_t)n_seq * cache->heads * a.chunks <= ctas;
   a.parts = reinterpret_cast<float*>(a.recs + ctas);
   const cudaStream_t st = (cudaStream_t)stream;
   switch ((cache->kind == UK_KV_E4M3 ? 4 : 0) + (dp == 128 ? 2 : 0) + (nh - 1)) {

@@ -95,6 +95,13 @@ __device__ __forceinline__ uint32_t uk_e4m3x2_to_half2(uint32_t codes) {
   return r;
 }
 
+// four e4m3 codes as two pairs of halves
+__device__ __forceinline__ void uk_e4m3x4_to_half2(uint32_t codes, uint32_t* lo, uint32_t* hi) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(*lo), "=r"(*hi)
+      : "r"(codes));
+}
+
 // two floats as e4m3 codes, round to nearest even, lo in the low byte
 __device__ __forceinline__ uint32_t uk_float2_to_e4m3x2(float lo, float hi) {
   uint16_t r;
