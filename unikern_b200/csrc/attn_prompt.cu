@@ -1,7 +1,39 @@
 // attn_prompt.cu -- attention over packed prompts, causal or full, with grouped
 // heads: O[i][h] = sum_j w_j V[j][g], w = softmax_j(scale * Q[i][h] . K[j][g])
-// over the keys row i sees, in one pass with the softmax's running maximum and
-// sum (scores carry scale * log2 e, so every exponential is a power of two).
+// over the keys row i sees, in one pass with a running reference m and sum l
+// per row (scores carry scale * log2 e, so every exponential is a power of two):
+//   l = sum 2^(s_j - m),  o = sum 2^(s_j - m) v_j;
+// m moves (l and o scaled by 2^(m - m')) only when a score passes it by 2^8.
+//
+// The work is bound by the tensor cores (4 dim flops per visible pair and head)
+// and, nearly as much, by the exponentials (one per pair and head; the MUFU
+// makes 16 per cycle and SM, a 128 x 128 tile's take as long as its two
+// products at dim 128).  One CTA per SM works on two tiles of 128
+// query rows of one key head at a time, so that one tile's products run while
+// the other's softmax does:
+//   warp 9     loads (TMA): both Q tiles, then K and V blocks of 128 keys through
+//              a ring in shared memory;
+//   warp 8     issues tcgen05.mma: S = Q K^T into 128 TMEM columns, O += P V with
+//              P in TMEM;
+//   warps 0-3  softmax of tile 0, a thread per row: reads its S row from TMEM,
+//              writes P (binary16) over it, rescales O when m moves, and at the
+//              end divides by l and stores; warps 4-7 the same for tile 1.
+// TMEM: S/P of tile 0 and 1 at columns 0 and 128, O at 256 and 384.  A tile's next
+// S is issued behind the product that reads its P, and the tensor core runs one
+// thread's products in order, so S arriving also says that O is up to date.
+//
+// What lies behind a row's mask: scores are replaced before the maximum, V rows
+// behind the sequence's last key are zeroed in shared memory (a zero weight
+// times a NaN would be one), and where a finite sum meets a row of O that is
+// not, the few masked keys of its last blocks are looked through; if one of
+// them holds a NaN or an infinity the row is computed again, key by key.
+//
+// Every mbarrier wait is bounded (uk_mbar_wait); a timeout sets the fault word
+// read by uk_cuda_pipeline_fault() and the CTA unwinds.
+#include <cudaTypedefs.h>
+
+#include <mutex>
+
 #include "kv_cache.cuh"
 
 namespace uk {
@@ -10,7 +42,6 @@ __device__ unsigned int g_attn_prompt_fault = 0;
 
 namespace {
 
-constexpr int WARPS = 4;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 struct Args {
@@ -33,38 +64,546 @@ __device__ __forceinline__ float4 row4(const uint16_t* row, int lane, int dim) {
 
 __device__ __forceinline__ int64_t clamp64(int64_t x, int64_t lo, int64_t hi) { return x < lo ? lo : x > hi ? hi : x; }
 
-// One warp per (query row, head), a lane four of the row's values.
-__global__ void __launch_bounds__(WARPS * 32) k_attn_prompt_rows(Args a) {
-  const int64_t w = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  const int64_t t = w / a.heads_q;
-  const int h = (int)(w - t * a.heads_q), g = h / a.group;
-  if (t >= a.total_q) return;
-  const int b = uk_find_seq(a.cu_q, a.n_seq, t);
-  if (b < 0) return;
-  const int64_t q1 = clamp64(__ldg(a.cu_q + b + 1), 0, a.total_q);
-  const int64_t k0 = clamp64(__ldg(a.cu_k + b), 0, a.total_k), k1 = clamp64(__ldg(a.cu_k + b + 1), k0, a.total_k);
-  const int64_t end = a.causal ? k1 - (q1 - 1 - t) : k1;  // one past the last key this row sees
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// One row by one warp, key by key, on CUDA cores: keys [k0, end).  A lane
+// holds four of the row's values.
+__device__ __noinline__ void attend_row(const Args& a, int64_t t, int h, int64_t k0, int64_t end) {
+  const int lane = threadIdx.x & 31, g = h / a.group;
   const float4 q = row4(a.q + t * a.q_token + h * a.q_head, lane, a.dim);
   float m = -INFINITY, l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int64_t j = k0; j < end; ++j) {
-    const float4 k = row4(a.k + j * a.k_token + g * a.k_head, lane, a.dim);
-    const float4 v = row4(a.v + j * a.v_token + g * a.v_head, lane, a.dim);
-    const float s = uk_warp_sum(q.x * k.x + q.y * k.y + q.z * k.z + q.w * k.w) * a.scale2;
-    const float m2 = fmaxf(m, s);
-    const float f = m2 == -INFINITY ? 1.f : exp2f(m - m2), e = m2 == -INFINITY ? 0.f : exp2f(s - m2);
+  constexpr int U = 4;  // keys in flight
+  for (int64_t j = k0; j < end; j += U) {
+    float4 k[U], v[U];
+    float s[U], m2 = m;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool on = j + u < end;
+      k[u] = on ? row4(a.k + (j + u) * a.k_token + g * a.k_head, lane, a.dim) : make_float4(0.f, 0.f, 0.f, 0.f);
+      v[u] = on ? row4(a.v + (j + u) * a.v_token + g * a.v_head, lane, a.dim) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      s[u] = uk_warp_sum(q.x * k[u].x + q.y * k[u].y + q.z * k[u].z + q.w * k[u].w) * a.scale2;
+      if (j + u >= end) s[u] = -INFINITY;
+      m2 = fmaxf(m2, s[u]);
+    }
+    const float z = m2 == -INFINITY ? 0.f : m2, f = m2 == -INFINITY ? 1.f : ex2(m - m2);
     m = m2;
-    l = l * f + e;
-    o = make_float4(o.x * f + e * v.x, o.y * f + e * v.y, o.z * f + e * v.z, o.w * f + e * v.w);
+    l *= f;
+    o = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float e = ex2(s[u] - z);
+      l += e;
+      o = make_float4(fmaf(e, v[u].x, o.x), fmaf(e, v[u].y, o.y), fmaf(e, v[u].z, o.z), fmaf(e, v[u].w, o.w));
+    }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  if (lane * 4 < a.dim) {
-    const __half2 x = __floats2half2_rn(o.x * inv, o.y * inv), y = __floats2half2_rn(o.z * inv, o.w * inv);
+  if (lane * 4 < a.dim)
     reinterpret_cast<uint2*>(a.o + t * a.o_token + h * a.o_head)[lane] =
-        make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
-  }
+        make_uint2(pack_half(o.x * inv, o.y * inv), pack_half(o.z * inv, o.w * inv));
   if (a.lse != nullptr && lane == 0) a.lse[t * a.heads_q + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
+}
+
+// ---- what one CTA works on -----------------------------------------------------------
+constexpr int BM = 128, BN = 128;  // query rows and keys of a tile
+constexpr float GROW = 8.f;        // scores may pass the reference by 2^8 before it moves
+constexpr float SHIFT = 7.f;       // weights are held as 2^7 * 2^(s - m): up to 2^15, binary16 ends at 2^16
+// three warpgroups: two of softmax, one of the MMA and load warps (and two idle
+// ones).  They launch with 168 registers a thread; the softmax takes 216 (a row
+// of 128 scores stays in registers) and the others keep 72.
+constexpr int NUM_THREADS = 384;
+constexpr int REGS_LAUNCH = 168, REGS_SOFTMAX = 216, REGS_OTHERS = 72;
+static_assert(2 * REGS_SOFTMAX + REGS_OTHERS <= 3 * REGS_LAUNCH, "registers of the block");
+constexpr int MMA_WARP = 8, LOAD_WARP = 9;
+constexpr uint64_t WAIT_NS = 4000000000ull;  // a row computed again may take long
+
+struct Tile {
+  int head;    // query head; -1: no tile
+  int first;   // its first row within the sequence
+  int rows;    // rows it has
+  int blocks;  // blocks of keys some row of it sees
+};
+struct Item {
+  Tile tile[2];
+  int g;             // key head
+  int q0, k0, n, m;  // the sequence: its first rows, query and key counts
+};
+
+// Item i of the list: sequences in order; in each the pairs of tiles, the
+// tiles going from the last query block to the first (the longest first where
+// causal) and through the group's heads; a key head each.
+// One warp; lanes sum runs of sequences, the lane whose run holds the item goes on.
+__device__ bool find_item(const Args& a, int64_t item, Item* out) {
+  const int lane = threadIdx.x & 31;
+  const int per = (a.n_seq + 31) / 32;
+  const int first = min(lane * per, a.n_seq), last = min(first + per, a.n_seq);
+  auto bounds = [&](int b, int64_t* q0, int64_t* q1) {
+    *q0 = clamp64(__ldg(a.cu_q + b), 0, a.total_q);
+    *q1 = clamp64(__ldg(a.cu_q + b + 1), *q0, a.total_q);
+  };
+  auto items_of = [&](int b) -> int64_t {
+    int64_t q0, q1;
+    bounds(b, &q0, &q1);
+    return (((q1 - q0 + BM - 1) / BM * a.group + 1) / 2) * a.heads_kv;
+  };
+  int64_t mine = 0;
+  for (int b = first; b < last; ++b) mine += items_of(b);
+  int64_t incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t t = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += t;
+  }
+  const bool found = item >= incl - mine && item < incl;
+  if (found) {
+    int64_t at = item - (incl - mine);
+    int b = first;
+    for (int64_t n; at >= (n = items_of(b)); ++b) at -= n;
+    int64_t q0, q1;
+    bounds(b, &q0, &q1);
+    const int64_t k0 = clamp64(__ldg(a.cu_k + b), 0, a.total_k), k1 = clamp64(__ldg(a.cu_k + b + 1), k0, a.total_k);
+    out->g = (int)(at % a.heads_kv);
+    out->q0 = (int)q0, out->k0 = (int)k0, out->n = (int)(q1 - q0), out->m = (int)(k1 - k0);
+    const int blocks = (out->n + BM - 1) / BM;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int64_t e = at / a.heads_kv * 2 + t;  // blocks * group fits 47 bits
+      Tile& tile = out->tile[t];
+      tile.head = -1, tile.first = 0, tile.rows = 0, tile.blocks = 0;
+      if (e >= (int64_t)blocks * a.group) continue;
+      tile.head = out->g * a.group + (int)(e % a.group);
+      tile.first = (blocks - 1 - (int)(e / a.group)) * BM;
+      tile.rows = min(BM, out->n - tile.first);
+      // one past the last key that its last row sees
+      const int64_t end = a.causal ? (int64_t)out->m - out->n + tile.first + tile.rows : out->m;
+      tile.blocks = end <= 0 ? 0 : (int)((end + BN - 1) / BN);
+    }
+  }
+  return __any_sync(0xffffffffu, found);
+}
+
+template <int DP>
+struct Smem {
+  static constexpr int CHUNKS = DP / 64;         // 64-wide columns of a tile, one TMA box each
+  static constexpr int BOX = 128 * 128;          // 128 rows of 128 bytes
+  static constexpr int TILE = CHUNKS * BOX;      // a Q tile, a K or a V block
+  static constexpr int STAGES = DP == 128 ? 5 : 10;
+  static constexpr size_t BYTES = 1024 + (size_t)(2 + STAGES) * TILE + 512;
+};
+
+struct Ctl {
+  uint64_t q_full;
+  uint64_t kv_full[10], kv_empty[10];
+  uint64_t s_full[2], p_full[2], o_full[2];
+  uint64_t v_landed;  // a block whose rows behind the last key are zeroed before use
+  uint64_t teardown;
+  uint32_t tmem;
+  int abort;
+  int any;
+  Item item;
+};
+static_assert(sizeof(Ctl) <= 512, "control block");
+static_assert(Smem<128>::BYTES <= 232448 && Smem<64>::BYTES <= 232448, "shared memory per block on sm_100");
+
+__device__ __forceinline__ void raise_fault(Ctl* ctl, unsigned bit) {
+  atomicOr(&uk::g_attn_prompt_fault, bit);
+  ctl->abort = 1;
+}
+
+// ---- the softmax of one tile ----------------------------------------------------------
+template <int DP>
+__device__ __forceinline__ void softmax_tile(const Args& a, Ctl* ctl, const Item& it, int t, uint32_t tmem) {
+  const Tile tile = it.tile[t];
+  if (tile.head < 0) return;
+  volatile int* abort = &ctl->abort;
+  const int lane = threadIdx.x & 31, quad = (threadIdx.x >> 5) & 3;
+  const int i = quad * 32 + lane;  // row of the tile
+  const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+  const uint32_t s_at = tmem + lanes + t * BN, o_at = tmem + lanes + 256 + t * 128;
+  // one past the last key this row sees, and the first row's of the tile
+  const int64_t shift = a.causal ? (int64_t)it.m - it.n + tile.first + 1 : it.m;
+  const int64_t end64 = a.causal ? shift + i : it.m;
+  const int end = (int)(end64 < 0 ? 0 : end64 > it.m ? it.m : end64);
+  const bool neg = a.scale2 < 0.f;
+  const float hidden = neg ? INFINITY : -INFINITY;
+
+  float m = -INFINITY, l = 0.f;
+  for (int j = 0; j < tile.blocks; ++j) {
+    if (!__all_sync(0xffffffffu, uk_mbar_wait(&ctl->s_full[t], j & 1, abort, WAIT_NS))) {
+      if (!*abort) raise_fault(ctl, UK_FAULT_EPILOGUE);
+      return;
+    }
+    uk_tc_fence_after();
+    uint32_t s[4][32];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) uk_tmem_ld32(s_at + c * 32, s[c]);
+    uk_tmem_ld_wait();
+    const int base = j * BN;
+    if ((int64_t)base + BN > (shift < it.m ? shift : it.m)) {  // some row of the tile does not see the whole block
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int k = 0; k < 32; ++k)
+          if (base + c * 32 + k >= end) s[c][k] = __float_as_uint(hidden);
+    }
+    float top[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) top[c] = hidden;
+    if (!neg) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int k = 0; k < 32; ++k) top[c] = fmaxf(top[c], __uint_as_float(s[c][k]));
+      top[0] = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+    } else {
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int k = 0; k < 32; ++k) top[c] = fminf(top[c], __uint_as_float(s[c][k]));
+      top[0] = fminf(fminf(top[0], top[1]), fminf(top[2], top[3]));
+    }
+    const float mt = top[0] * a.scale2;
+    if (__any_sync(0xffffffffu, mt > m + GROW)) {
+      const float m2 = fmaxf(m, mt);
+      const float f = m2 == -INFINITY ? 1.f : ex2(m - m2);
+      m = m2;
+      l *= f;
+      if (j > 0) {
+#pragma unroll
+        for (int c = 0; c < DP / 32; ++c) {
+          uint32_t o[32];
+          uk_tmem_ld32(o_at + c * 32, o);
+          uk_tmem_ld_wait();
+#pragma unroll
+          for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+          uk_tmem_st32(o_at + c * 32, o);
+        }
+      }
+    }
+    const float z = m == -INFINITY ? 0.f : SHIFT - m;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      uint32_t p[32];
+#pragma unroll
+      for (int k = 0; k < 32; ++k) {
+        const float x = ex2(fmaf(__uint_as_float(s[2 * c + k / 16][2 * (k % 16)]), a.scale2, z));
+        const float y = ex2(fmaf(__uint_as_float(s[2 * c + k / 16][2 * (k % 16) + 1]), a.scale2, z));
+        sum[2 * (k & 1)] += x;
+        sum[2 * (k & 1) + 1] += y;
+        p[k] = pack_half(x, y);
+      }
+      uk_tmem_st32(s_at + c * 32, p);
+    }
+    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    uk_tmem_st_wait();
+    uk_tc_fence_before();
+    __syncwarp();
+    if (lane == 0) uk_mbar_arrive(&ctl->p_full[t]);
+  }
+
+  // ---- O / l, the log of the sum
+  const bool mine = i < tile.rows;
+  const int64_t token = (int64_t)it.q0 + tile.first + i;
+  uint16_t* out = a.o + token * a.o_token + tile.head * a.o_head;
+  bool odd = false;  // a finite sum, but not a finite row
+  if (tile.blocks > 0) {
+    if (!__all_sync(0xffffffffu, uk_mbar_wait(&ctl->o_full[t], 0, abort, WAIT_NS))) {
+      if (!*abort) raise_fault(ctl, UK_FAULT_EPILOGUE);
+      return;
+    }
+    uk_tc_fence_after();
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int c = 0; c < DP / 32; ++c) {
+    uint32_t o[32];
+    if (tile.blocks > 0) {
+      uk_tmem_ld32(o_at + c * 32, o);
+      uk_tmem_ld_wait();
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      uint32_t w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float x = 0.f, y = 0.f;
+        if (tile.blocks > 0) x = __uint_as_float(o[k * 8 + 2 * e]) * inv, y = __uint_as_float(o[k * 8 + 2 * e + 1]) * inv;
+        odd |= !(fabsf(x) < INFINITY) || !(fabsf(y) < INFINITY);
+        w[e] = pack_half(x, y);
+      }
+      if (mine && c * 32 + k * 8 < a.dim)
+        *reinterpret_cast<uint4*>(out + c * 32 + k * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+  if (mine && a.lse != nullptr)
+    a.lse[token * a.heads_q + tile.head] = l == 0.f ? -INFINITY : (m - SHIFT + log2f(l)) * LN2;
+
+  // rows that may have met what their mask hides
+  unsigned rows = __ballot_sync(0xffffffffu, mine && odd && l - l == 0.f);
+  while (rows != 0) {
+    const int r = __ffs(rows) - 1;
+    rows &= rows - 1;
+    const int from = __shfl_sync(0xffffffffu, end, r), to = min(tile.blocks * BN, it.m);
+    bool bad = false;
+    for (int k = from; k < to && !bad; ++k) {
+      const float4 v = row4(a.v + (int64_t)(it.k0 + k) * a.v_token + it.g * a.v_head, lane, a.dim);
+      bad = __any_sync(0xffffffffu, !(fabsf(v.x) + fabsf(v.y) + fabsf(v.z) + fabsf(v.w) < INFINITY));
+    }
+    __syncwarp();  // the row's stores above come before these
+    if (bad) attend_row(a, (int64_t)it.q0 + tile.first + quad * 32 + r, tile.head, it.k0, (int64_t)it.k0 + from);
+  }
+}
+
+// ---- loads ---------------------------------------------------------------------------
+template <int DP>
+__device__ __forceinline__ void load_blocks(const Args& a, Ctl* ctl, const Item& it, int blocks, uint8_t* smem,
+                                            uint8_t* ring, const CUtensorMap& tm_q, const CUtensorMap& tm_k,
+                                            const CUtensorMap& tm_v) {
+  using S = Smem<DP>;
+  volatile int* abort = &ctl->abort;
+  const int lane = threadIdx.x & 31;
+  if (blocks == 0) return;
+  if (lane == 0) {
+    int tiles = 0;
+    for (int t = 0; t < 2; ++t) tiles += it.tile[t].blocks > 0;
+    uk_mbar_expect_tx(&ctl->q_full, tiles * S::TILE);
+    for (int t = 0; t < 2; ++t)
+      if (it.tile[t].blocks > 0)
+#pragma unroll
+        for (int c = 0; c < S::CHUNKS; ++c)
+          uk_tma_load_3d(smem + t * S::TILE + c * S::BOX, &tm_q, &ctl->q_full, c * 64, it.q0 + it.tile[t].first,
+                         it.tile[t].head);
+  }
+  __syncwarp();
+  uint32_t n = 0;  // blocks put into the ring: K and V alternate
+  bool ok = true;
+  for (; n < 2u * blocks; ++n) {
+    const int s = n % S::STAGES, j = n >> 1;
+    if (!(ok = __all_sync(0xffffffffu, uk_mbar_wait(&ctl->kv_empty[s], ((n / S::STAGES) & 1u) ^ 1u, abort, WAIT_NS)))) {
+      if (!*abort) raise_fault(ctl, UK_FAULT_PRODUCER);
+      break;
+    }
+    const bool fix = (n & 1u) && (j + 1) * BN > it.m;
+    uint8_t* dst = ring + (size_t)s * S::TILE;
+    uint64_t* bar = fix ? &ctl->v_landed : &ctl->kv_full[s];
+    if (lane == 0) {
+      uk_mbar_expect_tx(bar, S::TILE);
+#pragma unroll
+      for (int c = 0; c < S::CHUNKS; ++c)
+        uk_tma_load_3d(dst + c * S::BOX, n & 1u ? &tm_v : &tm_k, bar, c * 64, it.k0 + j * BN, it.g);
+    }
+    __syncwarp();
+    if (fix) {
+      // rows behind the sequence's last key hold whatever is there, and their weight is zero
+      if (!__all_sync(0xffffffffu, uk_mbar_wait(bar, 0, nullptr, WAIT_NS))) raise_fault(ctl, UK_FAULT_PRODUCER);
+      const int valid = it.m - j * BN;
+#pragma unroll
+      for (int c = 0; c < S::CHUNKS; ++c)
+        for (int x = valid * 8 + lane; x < BN * 8; x += 32)
+          reinterpret_cast<uint4*>(dst + c * S::BOX)[x] = make_uint4(0, 0, 0, 0);
+      uk_fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) uk_mbar_arrive(&ctl->kv_full[s]);
+    }
+  }
+  if (!ok || *abort) {  // the copies in flight land before this block's memory is given up
+    for (uint32_t x = n > S::STAGES ? n - S::STAGES : 0; x < n; ++x)
+      uk_mbar_wait(&ctl->kv_full[x % S::STAGES], (x / S::STAGES) & 1u, nullptr, WAIT_NS);
+    uk_mbar_wait(&ctl->q_full, 0, nullptr, WAIT_NS);
+  }
+}
+
+// ---- products, issued by one thread ------------------------------------------------------
+template <int DP>
+__device__ __forceinline__ void issue_products(Ctl* ctl, const Item& it, int blocks, uint8_t* smem, uint8_t* ring,
+                                               uint32_t tmem) {
+  using S = Smem<DP>;
+  volatile int* abort = &ctl->abort;
+  constexpr uint32_t IDESC_S = uk_idesc_f16_ab(BM, BN, 0, 0), IDESC_O = uk_idesc_f16_ab(BM, DP, 0, 1);
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (uk_mbar_wait(bar, parity, abort, WAIT_NS)) {
+      uk_tc_fence_after();
+      return true;
+    }
+    if (!*abort) raise_fault(ctl, UK_FAULT_MMA);
+    return false;
+  };
+  auto wait_block = [&](uint32_t n) { return wait(&ctl->kv_full[n % S::STAGES], (n / S::STAGES) & 1u); };
+  auto scores = [&](int t, uint32_t n) {  // S_t = Q_t K^T
+    const uint32_t sq = uk_smem_u32(smem + t * S::TILE), sk = uk_smem_u32(ring + (size_t)(n % S::STAGES) * S::TILE);
+#pragma unroll
+    for (int k = 0; k < DP / 16; ++k) {
+      const uint32_t at = (k / 4) * S::BOX + (k % 4) * 32;
+      uk_umma_f16(tmem + t * BN, uk_desc_sw128(sq + at, 16, 1024), uk_desc_sw128(sk + at, 16, 1024), IDESC_S, k > 0);
+    }
+    uk_umma_commit(&ctl->s_full[t]);
+  };
+  bool ok = blocks == 0 || (wait(&ctl->q_full, 0) && wait_block(0));
+  if (ok && blocks > 0) {
+    for (int t = 0; t < 2; ++t)
+      if (it.tile[t].blocks > 0) scores(t, 0);
+    uk_umma_commit(&ctl->kv_empty[0]);
+  }
+  for (int j = 0; j < blocks && ok; ++j) {
+    const uint32_t nv = 2 * j + 1, nk = nv + 1;
+    ok = wait_block(nv) && (j + 1 >= blocks || wait_block(nk));
+    const uint32_t sv = uk_smem_u32(ring + (size_t)(nv % S::STAGES) * S::TILE);
+    for (int t = 0; t < 2 && ok; ++t) {
+      if (j >= it.tile[t].blocks) continue;
+      if (!(ok = wait(&ctl->p_full[t], j & 1))) break;
+#pragma unroll
+      for (int k = 0; k < BN / 16; ++k)  // O_t += P_t V
+        uk_umma_f16_ts(tmem + 256 + t * 128, tmem + t * BN + k * 8, uk_desc_sw128(sv + k * 2048, S::BOX, 1024), IDESC_O,
+                       j > 0 || k > 0);
+      if (j + 1 < it.tile[t].blocks) scores(t, nk);
+      else uk_umma_commit(&ctl->o_full[t]);
+    }
+    if (ok) {
+      uk_umma_commit(&ctl->kv_empty[nv % S::STAGES]);
+      if (j + 1 < blocks) uk_umma_commit(&ctl->kv_empty[nk % S::STAGES]);
+    }
+  }
+  // every product issued completes before TMEM and shared memory are given up
+  uk_umma_commit(&ctl->teardown);
+  if (!uk_mbar_wait(&ctl->teardown, 0, nullptr, WAIT_NS)) atomicOr(&uk::g_attn_prompt_fault, UK_FAULT_TEARDOWN);
+}
+
+template <int DP>
+__global__ void __launch_bounds__(NUM_THREADS, 1)
+    k_attn_prompt(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                  const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ Args a) {
+  using S = Smem<DP>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* ring = smem + 2 * S::TILE;
+  Ctl* ctl = (Ctl*)(ring + (size_t)S::STAGES * S::TILE);
+  volatile int* abort = &ctl->abort;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (warp == LOAD_WARP) {
+    const bool any = find_item(a, blockIdx.x, &ctl->item);
+    if (lane == 0) {
+      ctl->any = any;
+      uk_mbar_init(&ctl->q_full, 1);
+      for (int s = 0; s < S::STAGES; ++s) {
+        uk_mbar_init(&ctl->kv_full[s], 1);
+        uk_mbar_init(&ctl->kv_empty[s], 1);
+      }
+      for (int t = 0; t < 2; ++t) {
+        uk_mbar_init(&ctl->s_full[t], 1);
+        uk_mbar_init(&ctl->p_full[t], 4);
+        uk_mbar_init(&ctl->o_full[t], 1);
+      }
+      uk_mbar_init(&ctl->v_landed, 1);
+      uk_mbar_init(&ctl->teardown, 1);
+      ctl->abort = 0;
+      uk_fence_mbar_init();
+      uk_tma_prefetch_desc(&tm_q);
+      uk_tma_prefetch_desc(&tm_k);
+      uk_tma_prefetch_desc(&tm_v);
+    }
+  }
+  if (warp == MMA_WARP) {
+    uk_tmem_alloc(&ctl->tmem, 512);
+    uk_tmem_relinquish();
+  }
+  uk_tc_fence_before();
+  __syncthreads();
+  uk_tc_fence_after();
+  const uint32_t tmem = ctl->tmem;
+  const Item& it = ctl->item;
+  const int blocks = ctl->any ? max(it.tile[0].blocks, it.tile[1].blocks) : 0;
+
+  if (!ctl->any) {
+    // past the list's end: the grid is an upper bound of its length
+  } else if (warp < 8) {
+    uk_regs_up<REGS_SOFTMAX>();
+    softmax_tile<DP>(a, ctl, it, warp >> 2, tmem);
+  } else {
+    uk_regs_down<REGS_OTHERS>();
+    if (warp == LOAD_WARP) load_blocks<DP>(a, ctl, it, blocks, smem, ring, tm_q, tm_k, tm_v);
+    else if (warp == MMA_WARP && lane == 0) issue_products<DP>(ctl, it, blocks, smem, ring, tmem);
+  }
+  __syncwarp();
+  uk_tc_fence_before();
+  __syncthreads();
+  if (warp == MMA_WARP) {
+    uk_tc_fence_after();
+    uk_tmem_dealloc(tmem, 512);
+  }
+}
+
+// No keys at all: every row of the sequences is zero.
+__global__ void __launch_bounds__(256) k_attn_prompt_no_keys(Args a) {
+  const int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int64_t t = w / a.heads_q;
+  const int h = (int)(w - t * a.heads_q);
+  if (t >= a.total_q || uk_find_seq(a.cu_q, a.n_seq, t) < 0) return;
+  attend_row(a, t, h, 0, 0);
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    cudaDriverEntryPointQueryResult q;
+    void* p = nullptr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = (PFN_cuTensorMapEncodeTiled_v12000)p;
+  });
+  return fn;
+}
+
+// packed rows [tokens][heads][dim] as a (dim, token, head) tensor; boxes of
+// 64 x 128 x 1, columns behind dim and rows behind the last filled with zeros
+int make_map(CUtensorMap* m, const char* name, const uint16_t* base, int dim, int64_t tokens, int heads,
+             int64_t token_stride, int64_t head_stride) {
+  auto fn = encode_fn();
+  if (!fn) return uk::fail(UK_ECUDA, "attn_prompt: cuTensorMapEncodeTiled is unavailable from the driver");
+  // a stride that nothing steps by still has to be one the map accepts
+  if (tokens == 1) token_stride = dim;
+  if (heads == 1) head_stride = dim;
+  cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)tokens, (cuuint64_t)heads};
+  cuuint64_t strides[2] = {(cuuint64_t)token_stride * 2, (cuuint64_t)head_stride * 2};
+  cuuint32_t box[3] = {64, 128, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<uint16_t*>(base), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return uk::fail(UK_ECUDA, "attn_prompt: no tensor map of %s (%d)", name, (int)r);
+  return UK_OK;
+}
+
+template <int DP>
+int launch(const Args& a, int64_t items, cudaStream_t st) {
+  CUtensorMap q, k, v;
+  if (int rc = make_map(&q, "Q", a.q, a.dim, a.total_q, a.heads_q, a.q_token, a.q_head)) return rc;
+  if (int rc = make_map(&k, "K", a.k, a.dim, a.total_k, a.heads_kv, a.k_token, a.k_head)) return rc;
+  if (int rc = make_map(&v, "V", a.v, a.dim, a.total_k, a.heads_kv, a.v_token, a.v_head)) return rc;
+  static bool attr_done[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !attr_done[dev]) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(k_attn_prompt<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Smem<DP>::BYTES);
+    if (e != cudaSuccess) return uk::fail(UK_ECUDA, "attn_prompt: smem attribute: %s", cudaGetErrorString(e));
+    if (dev >= 0 && dev < 64) attr_done[dev] = true;
+  }
+  k_attn_prompt<DP><<<(unsigned)items, NUM_THREADS, Smem<DP>::BYTES, st>>>(q, k, v, a);
+  return uk::check_launch("attn_prompt");
 }
 
 }  // namespace
@@ -108,8 +647,19 @@ extern "C" int uk_cuda_attn_prompt_f16(const uint16_t* Q, int64_t q_token_stride
   Args a{Q, K, V, O, q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride,
          o_token_stride, o_head_stride, LSE, cu_q, cu_k, n_seq, heads_q, heads_kv, heads_q / heads_kv, dim, causal,
          total_q, total_k, scale * LOG2E};
-  const int64_t blocks = (total_q * heads_q + WARPS - 1) / WARPS;
-  if (blocks > 0x7fffffff) return uk::fail(UK_EINVAL, "attn_prompt: total_q * heads_q exceeds the grid");
-  k_attn_prompt_rows<<<(unsigned)blocks, WARPS * 32, 0, (cudaStream_t)stream>>>(a);
-  return uk::check_launch("attn_prompt");
+  // a zero scale: any factor that no score can raise above rounding does the same
+  // and leaves hidden scores at -inf
+  if (a.scale2 == 0.f) a.scale2 = 1e-30f;
+  if (total_k == 0) {
+    const int64_t blocks = (total_q * heads_q + 7) / 8;
+    if (blocks > 0x7fffffff) return uk::fail(UK_EINVAL, "attn_prompt: total_q * heads_q exceeds the grid");
+    k_attn_prompt_no_keys<<<(unsigned)blocks, 256, 0, (cudaStream_t)stream>>>(a);
+    return uk::check_launch("attn_prompt");
+  }
+  // at most this many query blocks and pairs of tiles, whatever the lengths are
+  const int64_t seqs = n_seq < total_q ? n_seq : total_q;
+  const int64_t q_blocks = total_q / BM + seqs < total_q ? total_q / BM + seqs : total_q;
+  const int64_t items = (q_blocks * a.group + seqs) / 2 * heads_kv;
+  if (items > 0x7fffffff) return uk::fail(UK_EINVAL, "attn_prompt: %lld tiles exceed the grid", (long long)items);
+  return dim > 64 ? launch<128>(a, items, (cudaStream_t)stream) : launch<64>(a, items, (cudaStream_t)stream);
 }

@@ -151,6 +151,18 @@ __device__ __forceinline__ void uk_umma_f16(uint32_t d_tmem, uint64_t adesc, uin
       : "memory");
 }
 
+// The same with A in TMEM: lane = row, each 32-bit column two halves along K
+// (16 of K = 8 columns).
+__device__ __forceinline__ void uk_umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                               uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
 // mbarrier arrive (count one) once every tcgen05 op issued so far by this
 // thread has completed
 __device__ __forceinline__ void uk_umma_commit(uint64_t* bar) {
@@ -279,6 +291,18 @@ __device__ __forceinline__ void uk_pdl_launch_dependents() {
 // memory is visible (a no-op without a programmatic dependency)
 __device__ __forceinline__ void uk_pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// ---- register split between the warpgroups of a block -------------------------
+// every warp of a warpgroup executes it; the shares of all warpgroups together
+// stay within the registers the block was launched with
+template <int N>
+__device__ __forceinline__ void uk_regs_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void uk_regs_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 // ---- tf32 ----------------------------------------------------------------------
 // D[tmem] (+)= A * B, kind::tf32 (both operands tf32: fp32 bit patterns whose
 // low 13 mantissa bits the tensor core ignores), K = 8 per instruction.
@@ -304,6 +328,18 @@ __device__ __forceinline__ float uk_tf32_rna(float x) {
   uint32_t r;
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
   return __uint_as_float(r & 0xFFFFE000u);
+}
+
+// ---- TMA (tiled, 3-D, single-CTA destination) ------------------------------
+// c0 = innermost coordinate (elements; callers keep c0 * elem_size a multiple
+// of 16 bytes).
+__device__ __forceinline__ void uk_tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1,
+                                               int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+          uk_smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(uk_smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
 }
 
 // ---- TMA (tiled, 4-D, single-CTA destination) ------------------------------
