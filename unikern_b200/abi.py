@@ -130,10 +130,23 @@ def check(rc: int):
         raise UkError(rc, lib().uk_cuda_last_error().decode())
 
 
+_TORCH = None
+
+
+def _torch():
+    global _TORCH
+    if _TORCH is None:
+        import torch
+        _TORCH = torch
+    return _TORCH
+
+
 def _stream(stream=None):
-    import torch
-    s = stream if stream is not None else torch.cuda.current_stream()
-    return s.cuda_stream
+    if stream is not None:
+        return stream.cuda_stream
+    t = _torch()
+    # the handle behind torch.cuda.current_stream(), without the stream object (3 us a call)
+    return t._C._cuda_getCurrentRawStream(t.cuda.current_device())
 
 
 def _p(t):
@@ -379,56 +392,61 @@ class KvCache:
 
 
 def _index(t, n, name):
-    import torch
-    _need(t.dtype is torch.int32 and t.dim() == 1 and t.shape[0] == n and (n <= 1 or t.stride(0) == 1), name,
-          "must be a contiguous int32 tensor of", n)
+    shape = t.shape
+    if t.dtype is not _torch().int32 or len(shape) != 1 or shape[0] != n or (n > 1 and t.stride()[0] != 1):
+        _need(False, name, "must be a contiguous int32 tensor of", n)
+    return t.data_ptr()
 
 
 def _table(table):
-    import torch
-    _need(table.dtype is torch.int32 and table.dim() == 2 and (table.shape[1] <= 1 or table.stride(1) == 1),
-          "block_table must be an int32 [sequences, pages] tensor with contiguous rows")
-    return table.shape
+    """(sequences, pages, elements between rows, pointer)"""
+    shape, stride = table.shape, table.stride()
+    if table.dtype is not _torch().int32 or len(shape) != 2 or (shape[1] > 1 and stride[1] != 1):
+        _need(False, "block_table must be an int32 [sequences, pages] tensor with contiguous rows")
+    return shape[0], shape[1], stride[0], table.data_ptr()
 
 
-def _rows(t, name, heads, dim):
-    import torch
-    _need(t.dtype is torch.float16 and t.dim() == 3 and t.shape[1] == heads and t.shape[2] == dim
-          and t.stride(2) == 1, name, "must be a float16 [tokens, %d, %d] tensor with contiguous rows" % (heads, dim))
-    return t.shape[0]
+def _rows(t, name, heads, dim, n=None):
+    """(pointer, elements between tokens, between heads)"""
+    shape, stride = t.shape, t.stride()
+    if t.dtype is not _torch().float16 or len(shape) != 3 or shape[1] != heads or shape[2] != dim or stride[2] != 1:
+        _need(False, name, "must be a float16 [tokens, %d, %d] tensor with contiguous rows" % (heads, dim))
+    if n is not None and shape[0] != n:
+        _need(False, name, "must have", n, "rows")
+    return t.data_ptr(), stride[0], stride[1]
 
 
 def _lse(lse, n, heads):
-    import torch
-    _need(lse is None or (lse.dtype is torch.float32 and lse.shape == (n, heads) and lse.is_contiguous()),
-          "lse must be a contiguous float32 [%d, %d] tensor" % (n, heads))
+    if lse is None:
+        return None
+    if lse.dtype is not _torch().float32 or lse.shape != (n, heads) or not lse.is_contiguous():
+        _need(False, "lse must be a contiguous float32 [%d, %d] tensor" % (n, heads))
+    return lse.data_ptr()
 
 
 def kv_append(K, V, cache, block_table, cu_new, seq_lens, stream=None):
     """Append packed rows K, V [tokens, heads, dim] to a paged cache: rows
     cu_new[b] .. cu_new[b + 1] - 1 become the last of sequence b's seq_lens[b]
     positions (the lengths after the append)."""
-    n_seq, pages = _table(block_table)
-    total = _rows(K, "K", cache.heads, cache.dim)
-    _need(_rows(V, "V", cache.heads, cache.dim) == total, "K and V must have the same rows")
-    _index(cu_new, n_seq + 1, "cu_new")
-    _index(seq_lens, n_seq, "seq_lens")
-    check(lib().uk_cuda_kv_append_f16(_p(K), K.stride(0), K.stride(1), _p(V), V.stride(0), V.stride(1), total,
-                                      cache.ref, _p(block_table), block_table.stride(0), pages, _p(cu_new),
-                                      _p(seq_lens), n_seq, _stream(stream)))
+    n_seq, pages, row, table = _table(block_table)
+    k, k_token, k_head = _rows(K, "K", cache.heads, cache.dim)
+    total = K.shape[0]
+    v, v_token, v_head = _rows(V, "V", cache.heads, cache.dim, total)
+    cu, lens = _index(cu_new, n_seq + 1, "cu_new"), _index(seq_lens, n_seq, "seq_lens")
+    check(lib().uk_cuda_kv_append_f16(k, k_token, k_head, v, v_token, v_head, total, cache.ref, table, row, pages, cu,
+                                      lens, n_seq, _stream(stream)))
 
 
 def kv_gather(cache, block_table, cu_out, seq_lens, K, V, stream=None):
     """Read the last cu_out[b + 1] - cu_out[b] of each sequence's seq_lens[b]
     cached positions back into packed rows K, V [tokens, heads, dim]."""
-    n_seq, pages = _table(block_table)
-    total = _rows(K, "K", cache.heads, cache.dim)
-    _need(_rows(V, "V", cache.heads, cache.dim) == total, "K and V must have the same rows")
-    _index(cu_out, n_seq + 1, "cu_out")
-    _index(seq_lens, n_seq, "seq_lens")
-    check(lib().uk_cuda_kv_gather_f16(cache.ref, _p(block_table), block_table.stride(0), pages, _p(cu_out),
-                                      _p(seq_lens), n_seq, _p(K), K.stride(0), K.stride(1), _p(V), V.stride(0),
-                                      V.stride(1), total, _stream(stream)))
+    n_seq, pages, row, table = _table(block_table)
+    k, k_token, k_head = _rows(K, "K", cache.heads, cache.dim)
+    total = K.shape[0]
+    v, v_token, v_head = _rows(V, "V", cache.heads, cache.dim, total)
+    cu, lens = _index(cu_out, n_seq + 1, "cu_out"), _index(seq_lens, n_seq, "seq_lens")
+    check(lib().uk_cuda_kv_gather_f16(cache.ref, table, row, pages, cu, lens, n_seq, k, k_token, k_head, v, v_token,
+                                      v_head, total, _stream(stream)))
 
 
 def attn_decode_workspace(cache, heads_q, stream=None):
@@ -445,19 +463,17 @@ def attn_decode(Q, cache, block_table, seq_lens, O, scale=None, lse=None, worksp
     positions; Q, O [sequences, heads_q, dim], scale 1 / sqrt(dim) by default,
     lse [sequences, heads_q] gets the log of the softmax's sum.  Allocates its
     workspace through torch when none is passed."""
-    n_seq, pages = _table(block_table)
+    n_seq, pages, row, table = _table(block_table)
     heads_q = Q.shape[1] if Q.dim() == 3 else 0
-    _need(_rows(Q, "Q", heads_q, cache.dim) == n_seq, "Q must have one row per sequence")
-    _need(_rows(O, "O", heads_q, cache.dim) == n_seq, "O must have one row per sequence")
-    _index(seq_lens, n_seq, "seq_lens")
-    _lse(lse, n_seq, heads_q)
+    q, q_seq, q_head = _rows(Q, "Q", heads_q, cache.dim, n_seq)
+    o, o_seq, o_head = _rows(O, "O", heads_q, cache.dim, n_seq)
+    lens, lse = _index(seq_lens, n_seq, "seq_lens"), _lse(lse, n_seq, heads_q)
     # a workspace of the call's own stream: freed here, it can only be handed
     # out again to work behind this call
     ws = workspace if workspace is not None else attn_decode_workspace(cache, heads_q, stream)
-    check(lib().uk_cuda_attn_decode_f16(_p(Q), Q.stride(0), Q.stride(1), cache.ref, _p(block_table),
-                                        block_table.stride(0), pages, _p(seq_lens), n_seq, heads_q,
-                                        cache.dim ** -0.5 if scale is None else scale, _p(O), O.stride(0), O.stride(1),
-                                        _p(lse), _p(ws), ws.numel() * ws.element_size(), _stream(stream)))
+    check(lib().uk_cuda_attn_decode_f16(q, q_seq, q_head, cache.ref, table, row, pages, lens, n_seq, heads_q,
+                                        cache.dim ** -0.5 if scale is None else scale, o, o_seq, o_head, lse,
+                                        ws.data_ptr(), ws.numel() * ws.element_size(), _stream(stream)))
 
 
 def attn_prompt(Q, K, V, cu_q, cu_k, O, scale=None, causal=True, lse=None, stream=None):
@@ -466,19 +482,19 @@ def attn_prompt(Q, K, V, cu_q, cu_k, O, scale=None, causal=True, lse=None, strea
     cu_k[b + 1] - 1 of K, V [tokens, heads_kv, dim]; causal aligns the last
     query with the last key."""
     _need(Q.dim() == 3 and K.dim() == 3, "Q and K must be [tokens, heads, dim] tensors")
-    heads_q, dim, heads_kv = Q.shape[1], Q.shape[2], K.shape[1]
-    total_q, total_k = _rows(Q, "Q", heads_q, dim), _rows(K, "K", heads_kv, dim)
-    _need(_rows(V, "V", heads_kv, dim) == total_k, "K and V must have the same rows")
-    _need(_rows(O, "O", heads_q, dim) == total_q, "O must have Q's rows")
+    total_q, heads_q, dim = Q.shape
+    total_k, heads_kv, _ = K.shape
+    q, q_token, q_head = _rows(Q, "Q", heads_q, dim)
+    k, k_token, k_head = _rows(K, "K", heads_kv, dim)
+    v, v_token, v_head = _rows(V, "V", heads_kv, dim, total_k)
+    o, o_token, o_head = _rows(O, "O", heads_q, dim, total_q)
     n_seq = cu_q.shape[0] - 1
     _need(n_seq >= 0, "cu_q must have one value more than there are sequences")
-    _index(cu_q, n_seq + 1, "cu_q")
-    _index(cu_k, n_seq + 1, "cu_k")
-    _lse(lse, total_q, heads_q)
-    check(lib().uk_cuda_attn_prompt_f16(_p(Q), Q.stride(0), Q.stride(1), _p(K), K.stride(0), K.stride(1), _p(V),
-                                        V.stride(0), V.stride(1), _p(cu_q), _p(cu_k), n_seq, total_q, total_k, heads_q,
-                                        heads_kv, dim, dim ** -0.5 if scale is None else scale, int(causal), _p(O),
-                                        O.stride(0), O.stride(1), _p(lse), _stream(stream)))
+    cuq, cuk = _index(cu_q, n_seq + 1, "cu_q"), _index(cu_k, n_seq + 1, "cu_k")
+    check(lib().uk_cuda_attn_prompt_f16(q, q_token, q_head, k, k_token, k_head, v, v_token, v_head, cuq, cuk, n_seq,
+                                        total_q, total_k, heads_q, heads_kv, dim,
+                                        dim ** -0.5 if scale is None else scale, int(causal), o, o_token, o_head,
+                                        _lse(lse, total_q, heads_q), _stream(stream)))
 
 
 # ---- KML runner (host side) -----------------------------------------------------
