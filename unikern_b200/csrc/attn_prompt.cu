@@ -138,6 +138,8 @@ struct Item {
   Tile tile[2];
   int g;             // key head
   int q0, k0, n, m;  // the sequence: its first rows, query and key counts
+  int any;           // 0: there is no further item
+  __device__ __forceinline__ int blocks() const { return max(tile[0].blocks, tile[1].blocks); }
 };
 
 // Item i of the list: sequences in order; in each the pairs of tiles, the
@@ -199,21 +201,25 @@ struct Smem {
   static constexpr int BOX = 128 * 128;          // 128 rows of 128 bytes
   static constexpr int TILE = CHUNKS * BOX;      // a Q tile, a K or a V block
   static constexpr int STAGES = DP == 128 ? 5 : 10;
-  static constexpr size_t BYTES = 1024 + (size_t)(2 + STAGES) * TILE + 512;
+  static constexpr size_t BYTES = 1024 + (size_t)(2 + STAGES) * TILE + 768;
 };
 
 struct Ctl {
-  uint64_t q_full;
+  uint64_t q_full[2], q_empty[2];
   uint64_t kv_full[10], kv_empty[10];
-  uint64_t s_full[2], p_full[2], o_full[2];
-  uint64_t v_landed;  // a block whose rows behind the last key are zeroed before use
+  uint64_t s_full[2];           // S of a tile is written (and every product before it is done)
+  uint64_t p_half[2], p_full[2];  // the weights of its first 64 keys, of all 128
+  uint64_t o_full[2], o_empty[2];
+  uint64_t item_full[2], item_empty[2];
+  uint64_t next;      // the answer about the next block
+  uint64_t v_landed;  // a V block whose rows behind the last key are zeroed before use
   uint64_t teardown;
+  alignas(16) uint8_t answer[16];
   uint32_t tmem;
   int abort;
-  int any;
-  Item item;
+  Item item[2];
 };
-static_assert(sizeof(Ctl) <= 512, "control block");
+static_assert(sizeof(Ctl) <= 768, "control block");
 static_assert(Smem<128>::BYTES <= 232448 && Smem<64>::BYTES <= 232448, "shared memory per block on sm_100");
 
 __device__ __forceinline__ void raise_fault(Ctl* ctl, unsigned bit) {
@@ -221,41 +227,50 @@ __device__ __forceinline__ void raise_fault(Ctl* ctl, unsigned bit) {
   ctl->abort = 1;
 }
 
-// ---- the softmax of one tile ----------------------------------------------------------
+// a bounded wait by a whole warp: the same answer in every lane
+__device__ __forceinline__ bool wait_warp(Ctl* ctl, uint64_t* bar, uint32_t parity, unsigned bit) {
+  if (__all_sync(0xffffffffu, uk_mbar_wait(bar, parity, &ctl->abort, WAIT_NS))) return true;
+  if (!*(volatile int*)&ctl->abort) raise_fault(ctl, bit);
+  return false;
+}
+// ---- the softmax of a tile ------------------------------------------------------------
+// *turn: blocks of this tile's slot so far (over all items); *ends: items that had any.
 template <int DP>
-__device__ __forceinline__ void softmax_tile(const Args& a, Ctl* ctl, const Item& it, int t, uint32_t tmem) {
-  const Tile tile = it.tile[t];
-  if (tile.head < 0) return;
-  volatile int* abort = &ctl->abort;
+__device__ __forceinline__ bool softmax_tile(const Args& a, Ctl* ctl, const Item& it, int t, uint32_t tmem,
+                                             uint32_t* turn, uint32_t* ends) {
+  const Tile& tile = it.tile[t];
+  if (tile.head < 0) return true;
   const int lane = threadIdx.x & 31, quad = (threadIdx.x >> 5) & 3;
   const int i = quad * 32 + lane;  // row of the tile
   const uint32_t lanes = (uint32_t)(quad * 32) << 16;
   const uint32_t s_at = tmem + lanes + t * BN, o_at = tmem + lanes + 256 + t * 128;
-  // one past the last key this row sees, and the first row's of the tile
+  // one past the last key that the tile's first row and this row see
   const int64_t shift = a.causal ? (int64_t)it.m - it.n + tile.first + 1 : it.m;
   const int64_t end64 = a.causal ? shift + i : it.m;
   const int end = (int)(end64 < 0 ? 0 : end64 > it.m ? it.m : end64);
+  const int clear = (int)(shift < 0 ? 0 : shift > it.m ? it.m : shift);
   const bool neg = a.scale2 < 0.f;
   const float hidden = neg ? INFINITY : -INFINITY;
+  const uint64_t scale2 = uk_f2(a.scale2, a.scale2);
 
   float m = -INFINITY, l = 0.f;
-  for (int j = 0; j < tile.blocks; ++j) {
-    if (!__all_sync(0xffffffffu, uk_mbar_wait(&ctl->s_full[t], j & 1, abort, WAIT_NS))) {
-      if (!*abort) raise_fault(ctl, UK_FAULT_EPILOGUE);
-      return;
-    }
+  for (int j = 0; j < tile.blocks; ++j, ++*turn) {
+    if (!wait_warp(ctl, &ctl->s_full[t], *turn & 1u, UK_FAULT_EPILOGUE)) return false;
     uk_tc_fence_after();
     uint32_t s[4][32];
 #pragma unroll
     for (int c = 0; c < 4; ++c) uk_tmem_ld32(s_at + c * 32, s[c]);
     uk_tmem_ld_wait();
     const int base = j * BN;
-    if ((int64_t)base + BN > (shift < it.m ? shift : it.m)) {  // some row of the tile does not see the whole block
+    const bool edge = base + BN > clear;  // some row of the tile does not see the whole block
+    auto hide = [&](int c) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
+      for (int k = 0; k < 32; ++k)
+        if (base + c * 32 + k >= end) s[c][k] = __float_as_uint(hidden);
+    };
+    if (edge) {
 #pragma unroll
-        for (int k = 0; k < 32; ++k)
-          if (base + c * 32 + k >= end) s[c][k] = __float_as_uint(hidden);
+      for (int c = 0; c < 4; ++c) hide(c);
     }
     float top[4];
 #pragma unroll
@@ -264,14 +279,16 @@ __device__ __forceinline__ void softmax_tile(const Args& a, Ctl* ctl, const Item
 #pragma unroll
       for (int c = 0; c < 4; ++c)
 #pragma unroll
-        for (int k = 0; k < 32; ++k) top[c] = fmaxf(top[c], __uint_as_float(s[c][k]));
-      top[0] = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        for (int k = 0; k < 32; k += 2)
+          top[c] = uk_max3_nan(top[c], __uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1]));
+      top[0] = uk_max3_nan(uk_max3_nan(top[0], top[1], top[2]), top[3], top[3]);
     } else {
 #pragma unroll
       for (int c = 0; c < 4; ++c)
 #pragma unroll
-        for (int k = 0; k < 32; ++k) top[c] = fminf(top[c], __uint_as_float(s[c][k]));
-      top[0] = fminf(fminf(top[0], top[1]), fminf(top[2], top[3]));
+        for (int k = 0; k < 32; k += 2)
+          top[c] = uk_min3_nan(top[c], __uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1]));
+      top[0] = uk_min3_nan(uk_min3_nan(top[0], top[1], top[2]), top[3], top[3]);
     }
     const float mt = top[0] * a.scale2;
     if (__any_sync(0xffffffffu, mt > m + GROW)) {
@@ -281,36 +298,53 @@ __device__ __forceinline__ void softmax_tile(const Args& a, Ctl* ctl, const Item
       l *= f;
       if (j > 0) {
 #pragma unroll
-        for (int c = 0; c < DP / 32; ++c) {
-          uint32_t o[32];
-          uk_tmem_ld32(o_at + c * 32, o);
+        for (int c = 0; c < DP / 16; ++c) {
+          uint32_t o[16];
+          uk_tmem_ld16(o_at + c * 16, o);
           uk_tmem_ld_wait();
 #pragma unroll
-          for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-          uk_tmem_st32(o_at + c * 32, o);
+          for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+          uk_tmem_st16(o_at + c * 16, o);
         }
       }
     }
+    if (!(mt < INFINITY)) l = NAN;  // a score that is NaN or +inf: so is the softmax
     const float z = m == -INFINITY ? 0.f : SHIFT - m;
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    const uint64_t z2 = uk_f2(z, z);
+    uint64_t sum[2] = {uk_f2(0.f, 0.f), uk_f2(0.f, 0.f)};
+    // the second half of the row is read again from TMEM while the first half's
+    // weights are formed: kept in registers, it made them spill
+    uk_tmem_ld32(s_at + 64, s[2]);
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      uint32_t p[32];
+    for (int c = 0; c < 4; ++c) {
+      uint32_t p[16];
+      if (c == 2) {
+        uk_tmem_ld_wait();
+        uk_tmem_ld32(s_at + 96, s[3]);
+      }
+      if (c == 3) uk_tmem_ld_wait();
+      if (c >= 2 && edge) hide(c);
 #pragma unroll
-      for (int k = 0; k < 32; ++k) {
-        const float x = ex2(fmaf(__uint_as_float(s[2 * c + k / 16][2 * (k % 16)]), a.scale2, z));
-        const float y = ex2(fmaf(__uint_as_float(s[2 * c + k / 16][2 * (k % 16) + 1]), a.scale2, z));
-        sum[2 * (k & 1)] += x;
-        sum[2 * (k & 1) + 1] += y;
+      for (int k = 0; k < 16; ++k) {
+        const uint64_t x2 =
+            uk_f2_fma(uk_f2(__uint_as_float(s[c][2 * k]), __uint_as_float(s[c][2 * k + 1])), scale2, z2);
+        float x, y;
+        uk_f2_split(x2, &x, &y);
+        x = ex2(x), y = ex2(y);
+        sum[k & 1] = uk_f2_add(sum[k & 1], uk_f2(x, y));
         p[k] = pack_half(x, y);
       }
-      uk_tmem_st32(s_at + c * 32, p);
+      uk_tmem_st16(s_at + c * 16, p);
+      if (c & 1) {
+        uk_tmem_st_wait();
+        uk_tc_fence_before();
+        __syncwarp();
+        if (lane == 0) uk_mbar_arrive(c == 1 ? &ctl->p_half[t] : &ctl->p_full[t]);
+      }
     }
-    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-    uk_tmem_st_wait();
-    uk_tc_fence_before();
-    __syncwarp();
-    if (lane == 0) uk_mbar_arrive(&ctl->p_full[t]);
+    float l0, l1;
+    uk_f2_split(uk_f2_add(sum[0], sum[1]), &l0, &l1);
+    l += l0 + l1;
   }
 
   // ---- O / l, the log of the sum
@@ -319,10 +353,7 @@ __device__ __forceinline__ void softmax_tile(const Args& a, Ctl* ctl, const Item
   uint16_t* out = a.o + token * a.o_token + tile.head * a.o_head;
   bool odd = false;  // a finite sum, but not a finite row
   if (tile.blocks > 0) {
-    if (!__all_sync(0xffffffffu, uk_mbar_wait(&ctl->o_full[t], 0, abort, WAIT_NS))) {
-      if (!*abort) raise_fault(ctl, UK_FAULT_EPILOGUE);
-      return;
-    }
+    if (!wait_warp(ctl, &ctl->o_full[t], *ends & 1u, UK_FAULT_EPILOGUE)) return false;
     uk_tc_fence_after();
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -347,6 +378,12 @@ __device__ __forceinline__ void softmax_tile(const Args& a, Ctl* ctl, const Item
         *reinterpret_cast<uint4*>(out + c * 32 + k * 8) = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
+  if (tile.blocks > 0) {
+    uk_tc_fence_before();
+    __syncwarp();
+    if (lane == 0) uk_mbar_arrive(&ctl->o_empty[t]);
+    ++*ends;
+  }
   if (mine && a.lse != nullptr)
     a.lse[token * a.heads_q + tile.head] = l == 0.f ? -INFINITY : (m - SHIFT + log2f(l)) * LN2;
 
@@ -364,120 +401,200 @@ __device__ __forceinline__ void softmax_tile(const Args& a, Ctl* ctl, const Item
     __syncwarp();  // the row's stores above come before these
     if (bad) attend_row(a, (int64_t)it.q0 + tile.first + quad * 32 + r, tile.head, it.k0, (int64_t)it.k0 + from);
   }
+  return true;
 }
 
-// ---- loads ---------------------------------------------------------------------------
+// ---- items and loads, one warp ---------------------------------------------------------
 template <int DP>
-__device__ __forceinline__ void load_blocks(const Args& a, Ctl* ctl, const Item& it, int blocks, uint8_t* smem,
-                                            uint8_t* ring, const CUtensorMap& tm_q, const CUtensorMap& tm_k,
-                                            const CUtensorMap& tm_v) {
+__device__ __forceinline__ void load_items(const Args& a, Ctl* ctl, uint8_t* smem, uint8_t* ring, const CUtensorMap& tm_q,
+                                           const CUtensorMap& tm_k, const CUtensorMap& tm_v) {
   using S = Smem<DP>;
   volatile int* abort = &ctl->abort;
   const int lane = threadIdx.x & 31;
-  if (blocks == 0) return;
-  if (lane == 0) {
-    int tiles = 0;
-    for (int t = 0; t < 2; ++t) tiles += it.tile[t].blocks > 0;
-    uk_mbar_expect_tx(&ctl->q_full, tiles * S::TILE);
-    for (int t = 0; t < 2; ++t)
-      if (it.tile[t].blocks > 0)
-#pragma unroll
-        for (int c = 0; c < S::CHUNKS; ++c)
-          uk_tma_load_3d(smem + t * S::TILE + c * S::BOX, &tm_q, &ctl->q_full, c * 64, it.q0 + it.tile[t].first,
-                         it.tile[t].head);
-  }
-  __syncwarp();
-  uint32_t n = 0;  // blocks put into the ring: K and V alternate
-  bool ok = true;
-  for (; n < 2u * blocks; ++n) {
-    const int s = n % S::STAGES, j = n >> 1;
-    if (!(ok = __all_sync(0xffffffffu, uk_mbar_wait(&ctl->kv_empty[s], ((n / S::STAGES) & 1u) ^ 1u, abort, WAIT_NS)))) {
-      if (!*abort) raise_fault(ctl, UK_FAULT_PRODUCER);
-      break;
-    }
-    const bool fix = (n & 1u) && (j + 1) * BN > it.m;
-    uint8_t* dst = ring + (size_t)s * S::TILE;
-    uint64_t* bar = fix ? &ctl->v_landed : &ctl->kv_full[s];
+  int64_t block = blockIdx.x;
+  uint32_t n = 0, fixed = 0, q_turn[2] = {0, 0};  // blocks put into the ring, V blocks zeroed, Q tiles loaded
+  bool ok = true, asked = false;
+  uint32_t answers = 0;
+  for (uint32_t turn = 0; ok; ++turn) {
+    Item& it = ctl->item[turn & 1u];
+    if (!(ok = wait_warp(ctl, &ctl->item_empty[turn & 1u], ((turn >> 1) & 1u) ^ 1u, UK_FAULT_PRODUCER))) break;
+    bool any = false;
+    if (block >= 0) any = find_item(a, block, &it);
+    __syncwarp();
     if (lane == 0) {
-      uk_mbar_expect_tx(bar, S::TILE);
-#pragma unroll
-      for (int c = 0; c < S::CHUNKS; ++c)
-        uk_tma_load_3d(dst + c * S::BOX, n & 1u ? &tm_v : &tm_k, bar, c * 64, it.k0 + j * BN, it.g);
+      it.any = any;
+      uk_mbar_arrive(&ctl->item_full[turn & 1u]);  // releases the item to the waiting warps
+      if (any) {
+        uk_mbar_expect_tx(&ctl->next, 16);
+        uk_next_block_ask(ctl->answer, &ctl->next);
+      }
     }
     __syncwarp();
-    if (fix) {
-      // rows behind the sequence's last key hold whatever is there, and their weight is zero
-      if (!__all_sync(0xffffffffu, uk_mbar_wait(bar, 0, nullptr, WAIT_NS))) raise_fault(ctl, UK_FAULT_PRODUCER);
-      const int valid = it.m - j * BN;
+    if (!any) break;
+    asked = true;
+    const int blocks = it.blocks();
+    for (int j = 0; j < 2 * blocks && ok; ++j) {
+      if (j == 0) {
+        for (int t = 0; t < 2 && ok; ++t) {
+          if (it.tile[t].blocks == 0) continue;
+          if (!(ok = wait_warp(ctl, &ctl->q_empty[t], (q_turn[t] & 1u) ^ 1u, UK_FAULT_PRODUCER))) break;
+          ++q_turn[t];
+          if (lane == 0) {
+            uk_mbar_expect_tx(&ctl->q_full[t], S::TILE);
 #pragma unroll
-      for (int c = 0; c < S::CHUNKS; ++c)
-        for (int x = valid * 8 + lane; x < BN * 8; x += 32)
-          reinterpret_cast<uint4*>(dst + c * S::BOX)[x] = make_uint4(0, 0, 0, 0);
-      uk_fence_proxy_async_smem();
+            for (int c = 0; c < S::CHUNKS; ++c)
+              uk_tma_load_3d(smem + t * S::TILE + c * S::BOX, &tm_q, &ctl->q_full[t], c * 64, it.q0 + it.tile[t].first,
+                             it.tile[t].head);
+          }
+          __syncwarp();
+        }
+        if (!ok) break;
+      }
+      const int s = n % S::STAGES, at = (j >> 1) * BN;  // K and V blocks alternate
+      if (!(ok = wait_warp(ctl, &ctl->kv_empty[s], ((n / S::STAGES) & 1u) ^ 1u, UK_FAULT_PRODUCER))) break;
+      const bool fix = (j & 1) && at + BN > it.m;
+      uint8_t* dst = ring + (size_t)s * S::TILE;
+      uint64_t* bar = fix ? &ctl->v_landed : &ctl->kv_full[s];
+      if (lane == 0) {
+        uk_mbar_expect_tx(bar, S::TILE);
+#pragma unroll
+        for (int c = 0; c < S::CHUNKS; ++c)
+          uk_tma_load_3d(dst + c * S::BOX, j & 1 ? &tm_v : &tm_k, bar, c * 64, it.k0 + at, it.g);
+      }
       __syncwarp();
-      if (lane == 0) uk_mbar_arrive(&ctl->kv_full[s]);
+      ++n;
+      if (fix) {
+        // rows behind the sequence's last key hold whatever is there, and their weight is zero
+        if (!__all_sync(0xffffffffu, uk_mbar_wait(bar, fixed & 1u, nullptr, WAIT_NS))) raise_fault(ctl, UK_FAULT_PRODUCER);
+        ++fixed;
+        const int valid = it.m - at;
+#pragma unroll
+        for (int c = 0; c < S::CHUNKS; ++c)
+          for (int x = valid * 8 + lane; x < BN * 8; x += 32)
+            reinterpret_cast<uint4*>(dst + c * S::BOX)[x] = make_uint4(0, 0, 0, 0);
+        uk_fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) uk_mbar_arrive(&ctl->kv_full[s]);
+      }
     }
+    if (!ok) break;
+    if (!(ok = wait_warp(ctl, &ctl->next, answers & 1u, UK_FAULT_PRODUCER))) break;
+    ++answers;
+    asked = false;
+    block = uk_next_block(ctl->answer);
+    uk_fence_proxy_async_smem();  // read before the next answer is written
+    __syncwarp();
   }
-  if (!ok || *abort) {  // the copies in flight land before this block's memory is given up
+  if (!ok || *abort) {  // what is in flight lands before this block's memory is given up
+    if (asked) uk_mbar_wait(&ctl->next, answers & 1u, nullptr, WAIT_NS);
     for (uint32_t x = n > S::STAGES ? n - S::STAGES : 0; x < n; ++x)
       uk_mbar_wait(&ctl->kv_full[x % S::STAGES], (x / S::STAGES) & 1u, nullptr, WAIT_NS);
-    uk_mbar_wait(&ctl->q_full, 0, nullptr, WAIT_NS);
+    for (int t = 0; t < 2; ++t)
+      if (q_turn[t] > 0) uk_mbar_wait(&ctl->q_full[t], (q_turn[t] - 1) & 1u, nullptr, WAIT_NS);
   }
 }
 
-// ---- products, issued by one thread ------------------------------------------------------
+// ---- products ------------------------------------------------------------------------
+// The whole warp runs the loop and one elected lane issues: with control flow
+// and operands the same in every lane the descriptors stay in uniform registers.
+// Issued from a branch of a single lane, every product waited for its operands
+// to be moved there, longer than the 64 cycles it runs.
 template <int DP>
-__device__ __forceinline__ void issue_products(Ctl* ctl, const Item& it, int blocks, uint8_t* smem, uint8_t* ring,
-                                               uint32_t tmem) {
+__device__ __forceinline__ void issue_products(Ctl* ctl, uint8_t* smem, uint8_t* ring, uint32_t tmem) {
   using S = Smem<DP>;
-  volatile int* abort = &ctl->abort;
   constexpr uint32_t IDESC_S = uk_idesc_f16_ab(BM, BN, 0, 0), IDESC_O = uk_idesc_f16_ab(BM, DP, 0, 1);
+  const bool leader = uk_elect();
+  const uint64_t dq = uk_desc_sw128(uk_smem_u32(smem), 16, 1024);      // K-major: Q and K
+  const uint64_t dk = uk_desc_sw128(uk_smem_u32(ring), 16, 1024);
+  const uint64_t dv = uk_desc_sw128(uk_smem_u32(ring), S::BOX, 1024);  // MN-major: V
   auto wait = [&](uint64_t* bar, uint32_t parity) {
-    if (uk_mbar_wait(bar, parity, abort, WAIT_NS)) {
-      uk_tc_fence_after();
-      return true;
-    }
-    if (!*abort) raise_fault(ctl, UK_FAULT_MMA);
-    return false;
+    const bool ok = wait_warp(ctl, bar, parity & 1u, UK_FAULT_MMA);
+    uk_tc_fence_after();
+    return ok;
   };
-  auto wait_block = [&](uint32_t n) { return wait(&ctl->kv_full[n % S::STAGES], (n / S::STAGES) & 1u); };
-  auto scores = [&](int t, uint32_t n) {  // S_t = Q_t K^T
-    const uint32_t sq = uk_smem_u32(smem + t * S::TILE), sk = uk_smem_u32(ring + (size_t)(n % S::STAGES) * S::TILE);
-#pragma unroll
-    for (int k = 0; k < DP / 16; ++k) {
-      const uint32_t at = (k / 4) * S::BOX + (k % 4) * 32;
-      uk_umma_f16(tmem + t * BN, uk_desc_sw128(sq + at, 16, 1024), uk_desc_sw128(sk + at, 16, 1024), IDESC_S, k > 0);
-    }
-    uk_umma_commit(&ctl->s_full[t]);
+  auto commit = [&](uint64_t* bar) {
+    if (leader) uk_umma_commit(bar);
   };
-  bool ok = blocks == 0 || (wait(&ctl->q_full, 0) && wait_block(0));
-  if (ok && blocks > 0) {
-    for (int t = 0; t < 2; ++t)
-      if (it.tile[t].blocks > 0) scores(t, 0);
-    uk_umma_commit(&ctl->kv_empty[0]);
-  }
-  for (int j = 0; j < blocks && ok; ++j) {
-    const uint32_t nv = 2 * j + 1, nk = nv + 1;
-    ok = wait_block(nv) && (j + 1 >= blocks || wait_block(nk));
-    const uint32_t sv = uk_smem_u32(ring + (size_t)(nv % S::STAGES) * S::TILE);
-    for (int t = 0; t < 2 && ok; ++t) {
-      if (j >= it.tile[t].blocks) continue;
-      if (!(ok = wait(&ctl->p_full[t], j & 1))) break;
+  uint32_t slot = 0, phase = 0;  // the ring's next block
+  auto scores = [&](int t, uint32_t at) {  // S_t = Q_t K^T, K in the ring's slot `at`
+    const uint64_t q0 = dq + (uint32_t)t * (S::TILE >> 4), k0 = dk + at * (S::TILE >> 4);
+    if (leader) {
 #pragma unroll
-      for (int k = 0; k < BN / 16; ++k)  // O_t += P_t V
-        uk_umma_f16_ts(tmem + 256 + t * 128, tmem + t * BN + k * 8, uk_desc_sw128(sv + k * 2048, S::BOX, 1024), IDESC_O,
-                       j > 0 || k > 0);
-      if (j + 1 < it.tile[t].blocks) scores(t, nk);
-      else uk_umma_commit(&ctl->o_full[t]);
+      for (int k = 0; k < DP / 16; ++k) {
+        constexpr int BOX16 = S::BOX >> 4;
+        const int off = (k / 4) * BOX16 + (k % 4) * 2;
+        uk_umma_f16(tmem + t * BN, q0 + off, k0 + off, IDESC_S, k > 0);
+      }
+      uk_umma_commit(&ctl->s_full[t]);
     }
-    if (ok) {
-      uk_umma_commit(&ctl->kv_empty[nv % S::STAGES]);
-      if (j + 1 < blocks) uk_umma_commit(&ctl->kv_empty[nk % S::STAGES]);
+    __syncwarp();
+  };
+  uint32_t turn[2] = {0, 0}, ends[2] = {0, 0};  // blocks and items of each tile so far
+  bool ok = true;
+  for (uint32_t item = 0; ok; ++item) {
+    if (!(ok = wait(&ctl->item_full[item & 1u], item >> 1))) break;
+    const Item& it = ctl->item[item & 1u];
+    const int any = __shfl_sync(0xffffffffu, it.any, 0);
+    const int own[2] = {__shfl_sync(0xffffffffu, it.tile[0].blocks, 0), __shfl_sync(0xffffffffu, it.tile[1].blocks, 0)};
+    __syncwarp();
+    if (leader) uk_mbar_arrive(&ctl->item_empty[item & 1u]);
+    if (!any) break;
+    const int blocks = max(own[0], own[1]);
+    if (blocks == 0) continue;
+    // K of the first block
+    ok = wait(&ctl->kv_full[slot], phase);
+    for (int t = 0; t < 2 && ok; ++t)
+      if (own[t] > 0) {
+        if (!(ok = wait(&ctl->q_full[t], ends[t]))) break;
+        scores(t, slot);
+        if (own[t] == 1) commit(&ctl->q_empty[t]);
+      }
+    if (!ok) break;
+    commit(&ctl->kv_empty[slot]);
+    if (++slot == S::STAGES) slot = 0, phase ^= 1u;
+    for (int j = 0; j < blocks && ok; ++j) {
+      // V of this block, K of the next
+      const bool more = j + 1 < blocks;
+      const uint32_t sv = slot, pv = phase;
+      if (++slot == S::STAGES) slot = 0, phase ^= 1u;
+      const uint32_t sk = slot;
+      if (!(ok = wait(&ctl->kv_full[sv], pv) && (!more || wait(&ctl->kv_full[sk], phase)))) break;
+      const uint64_t v0 = dv + sv * (S::TILE >> 4);
+      for (int t = 0; t < 2 && ok; ++t) {
+        if (j >= own[t]) continue;
+        if (j == 0 && !(ok = wait(&ctl->o_empty[t], ends[t] ^ 1u))) break;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          if (!(ok = ok && wait(half == 0 ? &ctl->p_half[t] : &ctl->p_full[t], turn[t]))) break;
+          if (leader) {
+#pragma unroll
+            for (int k = half * 4; k < half * 4 + 4; ++k)  // O_t += P_t V
+              uk_umma_f16_ts(tmem + 256 + t * 128, tmem + t * BN + k * 8, v0 + k * (2048 >> 4), IDESC_O, j > 0 || k > 0);
+          }
+          __syncwarp();
+        }
+        if (!ok) break;
+        ++turn[t];
+        if (j + 1 < own[t]) {
+          scores(t, sk);
+          if (j + 2 == own[t]) commit(&ctl->q_empty[t]);
+        } else {
+          commit(&ctl->o_full[t]);
+          ++ends[t];
+        }
+      }
+      if (!ok) break;
+      commit(&ctl->kv_empty[sv]);
+      if (more) {
+        commit(&ctl->kv_empty[sk]);
+        if (++slot == S::STAGES) slot = 0, phase ^= 1u;
+      }
     }
   }
   // every product issued completes before TMEM and shared memory are given up
-  uk_umma_commit(&ctl->teardown);
-  if (!uk_mbar_wait(&ctl->teardown, 0, nullptr, WAIT_NS)) atomicOr(&uk::g_attn_prompt_fault, UK_FAULT_TEARDOWN);
+  commit(&ctl->teardown);
+  if (!__all_sync(0xffffffffu, uk_mbar_wait(&ctl->teardown, 0, nullptr, WAIT_NS)))
+    atomicOr(&uk::g_attn_prompt_fault, UK_FAULT_TEARDOWN);
 }
 
 template <int DP>
@@ -489,31 +606,32 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* ring = smem + 2 * S::TILE;
   Ctl* ctl = (Ctl*)(ring + (size_t)S::STAGES * S::TILE);
-  volatile int* abort = &ctl->abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  if (warp == LOAD_WARP) {
-    const bool any = find_item(a, blockIdx.x, &ctl->item);
-    if (lane == 0) {
-      ctl->any = any;
-      uk_mbar_init(&ctl->q_full, 1);
-      for (int s = 0; s < S::STAGES; ++s) {
-        uk_mbar_init(&ctl->kv_full[s], 1);
-        uk_mbar_init(&ctl->kv_empty[s], 1);
-      }
-      for (int t = 0; t < 2; ++t) {
-        uk_mbar_init(&ctl->s_full[t], 1);
-        uk_mbar_init(&ctl->p_full[t], 4);
-        uk_mbar_init(&ctl->o_full[t], 1);
-      }
-      uk_mbar_init(&ctl->v_landed, 1);
-      uk_mbar_init(&ctl->teardown, 1);
-      ctl->abort = 0;
-      uk_fence_mbar_init();
-      uk_tma_prefetch_desc(&tm_q);
-      uk_tma_prefetch_desc(&tm_k);
-      uk_tma_prefetch_desc(&tm_v);
+  if (warp == LOAD_WARP && lane == 0) {
+    for (int s = 0; s < S::STAGES; ++s) {
+      uk_mbar_init(&ctl->kv_full[s], 1);
+      uk_mbar_init(&ctl->kv_empty[s], 1);
     }
+    for (int t = 0; t < 2; ++t) {
+      uk_mbar_init(&ctl->q_full[t], 1);
+      uk_mbar_init(&ctl->q_empty[t], 1);
+      uk_mbar_init(&ctl->s_full[t], 1);
+      uk_mbar_init(&ctl->p_half[t], 4);
+      uk_mbar_init(&ctl->p_full[t], 4);
+      uk_mbar_init(&ctl->o_full[t], 1);
+      uk_mbar_init(&ctl->o_empty[t], 4);
+      uk_mbar_init(&ctl->item_full[t], 1);
+      uk_mbar_init(&ctl->item_empty[t], 9);  // 8 softmax warps and the MMA thread
+    }
+    uk_mbar_init(&ctl->next, 1);
+    uk_mbar_init(&ctl->v_landed, 1);
+    uk_mbar_init(&ctl->teardown, 1);
+    ctl->abort = 0;
+    uk_fence_mbar_init();
+    uk_tma_prefetch_desc(&tm_q);
+    uk_tma_prefetch_desc(&tm_k);
+    uk_tma_prefetch_desc(&tm_v);
   }
   if (warp == MMA_WARP) {
     uk_tmem_alloc(&ctl->tmem, 512);
@@ -523,18 +641,21 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   __syncthreads();
   uk_tc_fence_after();
   const uint32_t tmem = ctl->tmem;
-  const Item& it = ctl->item;
-  const int blocks = ctl->any ? max(it.tile[0].blocks, it.tile[1].blocks) : 0;
 
-  if (!ctl->any) {
-    // past the list's end: the grid is an upper bound of its length
-  } else if (warp < 8) {
+  if (warp < 8) {
     uk_regs_up<REGS_SOFTMAX>();
-    softmax_tile<DP>(a, ctl, it, warp >> 2, tmem);
+    uint32_t turn = 0, ends = 0;
+    for (uint32_t item = 0;; ++item) {
+      if (!wait_warp(ctl, &ctl->item_full[item & 1u], (item >> 1) & 1u, UK_FAULT_EPILOGUE)) break;
+      const Item& it = ctl->item[item & 1u];
+      if (!it.any || !softmax_tile<DP>(a, ctl, it, warp >> 2, tmem, &turn, &ends)) break;
+      __syncwarp();
+      if (lane == 0) uk_mbar_arrive(&ctl->item_empty[item & 1u]);
+    }
   } else {
     uk_regs_down<REGS_OTHERS>();
-    if (warp == LOAD_WARP) load_blocks<DP>(a, ctl, it, blocks, smem, ring, tm_q, tm_k, tm_v);
-    else if (warp == MMA_WARP && lane == 0) issue_products<DP>(ctl, it, blocks, smem, ring, tmem);
+    if (warp == LOAD_WARP) load_items<DP>(a, ctl, smem, ring, tm_q, tm_k, tm_v);
+    else if (warp == MMA_WARP) issue_products<DP>(ctl, smem, ring, tmem);
   }
   __syncwarp();
   uk_tc_fence_before();

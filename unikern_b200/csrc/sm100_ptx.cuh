@@ -29,6 +29,17 @@ __device__ __forceinline__ uint64_t uk_globaltimer() {
   return t;
 }
 
+// one lane of the (converged) warp
+__device__ __forceinline__ bool uk_elect() {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok));
+  return ok != 0;
+}
+
 // ---- mbarrier ----------------------------------------------------------------
 __device__ __forceinline__ void uk_mbar_init(uint64_t* bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(uk_smem_u32(bar)), "r"(count) : "memory");
@@ -201,6 +212,17 @@ __device__ __forceinline__ void uk_tmem_st32(uint32_t taddr, const uint32_t (&r)
       : "memory");
 }
 
+// 32 lanes x 16 columns
+__device__ __forceinline__ void uk_tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      :
+      : "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
 __device__ __forceinline__ void uk_tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Shared-memory matrix descriptor for a 128-byte-swizzled operand tile
@@ -290,6 +312,62 @@ __device__ __forceinline__ void uk_pdl_launch_dependents() {
 // block until the preceding kernel in the stream has completed and its
 // memory is visible (a no-op without a programmatic dependency)
 __device__ __forceinline__ void uk_pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// ---- fp32 pairs (two lanes of one 64-bit register pair) -------------------------
+__device__ __forceinline__ uint64_t uk_f2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void uk_f2_split(uint64_t v, float* lo, float* hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(*lo), "=f"(*hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t uk_f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t uk_f2_add(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// the largest of three; a NaN among them is the result
+__device__ __forceinline__ float uk_max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float uk_min3_nan(float a, float b, float c) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// ---- cluster launch control: the blocks of a grid taken over by running ones ---
+// ask for the next block that has not been launched; the answer (16 bytes) lands
+// in `answer` and counts on `bar`
+__device__ __forceinline__ void uk_next_block_ask(void* answer, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                   uk_smem_u32(answer)),
+               "r"(uk_smem_u32(bar))
+               : "memory");
+}
+// its index (x of the grid), or -1 when none is left
+__device__ __forceinline__ int uk_next_block(const void* answer) {
+  uint32_t ok, x;
+  asm volatile(
+      "{\n\t.reg .b128 a;\n\t.reg .pred p;\n\t"
+      "ld.shared.b128 a, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "mov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, a;\n\t}"
+      : "=r"(ok), "=r"(x)
+      : "r"(uk_smem_u32(answer))
+      : "memory");
+  return ok ? (int)x : -1;
+}
 
 // ---- register split between the warpgroups of a block -------------------------
 // every warp of a warpgroup executes it; the shares of all warpgroups together
