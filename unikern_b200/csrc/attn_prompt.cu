@@ -671,7 +671,7 @@ __global__ void __launch_bounds__(256) k_attn_prompt_no_keys(Args a) {
   const int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int64_t t = w / a.heads_q;
   const int h = (int)(w - t * a.heads_q);
-  if (t >= a.total_q || uk_find_seq(a.cu_q, a.n_seq, t) < 0) return;
+  if (t >= a.total_q || uk_find_seq<true>(a.cu_q, a.n_seq, t) < 0) return;
   attend_row(a, t, h, 0, 0);
 }
 

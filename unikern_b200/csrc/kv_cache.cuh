@@ -77,12 +77,14 @@ __device__ __forceinline__ int64_t uk_kv_exp(const UkKvView& c, int page, int of
 
 // the sequence of a packed row t: cu[b] <= t < cu[b + 1] for a non-decreasing
 // cu[0..n].  -1 when t lies before the first or behind the last sequence.
-__device__ __forceinline__ int uk_find_seq(const int32_t* __restrict__ cu, int n, int64_t t) {
-  if (t < __ldg(cu) || t >= __ldg(cu + n)) return -1;
+template <bool kGlobal>
+__device__ __forceinline__ int uk_find_seq(const int32_t* cu, int n, int64_t t) {
+  auto at = [&](int i) { return kGlobal ? __ldg(cu + i) : cu[i]; };
+  if (t < at(0) || t >= at(n)) return -1;
   int lo = 0, hi = n;  // cu[lo] <= t < cu[hi]
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (__ldg(cu + mid) <= t) lo = mid;
+    if (at(mid) <= t) lo = mid;
     else hi = mid;
   }
   return lo;
@@ -102,11 +104,21 @@ __device__ __forceinline__ void uk_e4m3x4_to_half2(uint32_t codes, uint32_t* lo,
       : "r"(codes));
 }
 
-// two floats as e4m3 codes, round to nearest even, lo in the low byte
-__device__ __forceinline__ uint32_t uk_float2_to_e4m3x2(float lo, float hi) {
+// two halves as e4m3 codes, round to nearest even, saturating; lo in the low byte
+__device__ __forceinline__ uint32_t uk_half2_to_e4m3x2(uint32_t x) {
   uint16_t r;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(x));
   return r;
+}
+__device__ __forceinline__ uint32_t uk_mul_half2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// two equal halves
+__device__ __forceinline__ uint32_t uk_half2_of(float x) {
+  const __half2 h = __float2half2_rn(x);
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 // 2^(e - 127) for an exponent byte (0 counts as 2^-127: not written by the append)
