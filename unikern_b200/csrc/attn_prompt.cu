@@ -116,30 +116,32 @@ __device__ __noinline__ void attend_row(const Args& a, int64_t t, int h, int64_t
 }
 
 // ---- what one CTA works on -----------------------------------------------------------
-constexpr int BM = 128, BN = 128;  // query rows and keys of a tile
+constexpr int BM = 128, BN = 128;  // query rows of a tile, keys of a block
+constexpr int UN = 64;             // keys of a softmax step (half a block)
 constexpr float GROW = 8.f;        // scores may pass the reference by 2^8 before it moves
 constexpr float SHIFT = 7.f;       // weights are held as 2^7 * 2^(s - m): up to 2^15, binary16 ends at 2^16
-// three warpgroups: two of softmax, one of the MMA and load warps (and two idle
-// ones).  They launch with 168 registers a thread; the softmax takes 216 (a row
+// three warpgroups: two of softmax, one of the MMA and load warps (and an idle
+// one).  They launch with 168 registers a thread; the softmax takes 216 (a row
 // of 128 scores stays in registers) and the others keep 72.
 constexpr int NUM_THREADS = 384;
 constexpr int REGS_LAUNCH = 168, REGS_SOFTMAX = 216, REGS_OTHERS = 72;
 static_assert(2 * REGS_SOFTMAX + REGS_OTHERS <= 3 * REGS_LAUNCH, "registers of the block");
-constexpr int MMA_WARP = 8, LOAD_WARP = 9;
+constexpr int MMA_WARP = 8, LOAD_WARP = 10;  // MMA_WARP + t: tile t
 constexpr uint64_t WAIT_NS = 4000000000ull;  // a row computed again may take long
 
 struct Tile {
   int head;    // query head; -1: no tile
   int first;   // its first row within the sequence
   int rows;    // rows it has
-  int blocks;  // blocks of keys some row of it sees
+  int units;   // runs of 64 keys that some row of it sees
+  __device__ __forceinline__ int blocks() const { return (units + 1) / 2; }
 };
 struct Item {
   Tile tile[2];
   int g;             // key head
   int q0, k0, n, m;  // the sequence: its first rows, query and key counts
   int any;           // 0: there is no further item
-  __device__ __forceinline__ int blocks() const { return max(tile[0].blocks, tile[1].blocks); }
+  __device__ __forceinline__ int blocks() const { return max(tile[0].blocks(), tile[1].blocks()); }
 };
 
 // Item i of the list: sequences in order; in each the pairs of tiles, the
@@ -182,14 +184,14 @@ __device__ bool find_item(const Args& a, int64_t item, Item* out) {
     for (int t = 0; t < 2; ++t) {
       const int64_t e = at / a.heads_kv * 2 + t;  // blocks * group fits 47 bits
       Tile& tile = out->tile[t];
-      tile.head = -1, tile.first = 0, tile.rows = 0, tile.blocks = 0;
+      tile.head = -1, tile.first = 0, tile.rows = 0, tile.units = 0;
       if (e >= (int64_t)blocks * a.group) continue;
       tile.head = out->g * a.group + (int)(e % a.group);
       tile.first = (blocks - 1 - (int)(e / a.group)) * BM;
       tile.rows = min(BM, out->n - tile.first);
       // one past the last key that its last row sees
       const int64_t end = a.causal ? (int64_t)out->m - out->n + tile.first + tile.rows : out->m;
-      tile.blocks = end <= 0 ? 0 : (int)((end + BN - 1) / BN);
+      tile.units = end <= 0 ? 0 : (int)((end + UN - 1) / UN);
     }
   }
   return __any_sync(0xffffffffu, found);
@@ -207,8 +209,8 @@ struct Smem {
 struct Ctl {
   uint64_t q_full[2], q_empty[2];
   uint64_t kv_full[10], kv_empty[10];
-  uint64_t s_full[2];           // S of a tile is written (and every product before it is done)
-  uint64_t p_half[2], p_full[2];  // the weights of its first 64 keys, of all 128
+  uint64_t s_full[2][2], p_full[2][2];  // of each tile, for the even and the odd runs of keys
+  uint64_t pv_done[2];                  // a run's product with V is in O
   uint64_t o_full[2], o_empty[2];
   uint64_t item_full[2], item_empty[2];
   uint64_t next;      // the answer about the next block
@@ -234,10 +236,11 @@ __device__ __forceinline__ bool wait_warp(Ctl* ctl, uint64_t* bar, uint32_t pari
   return false;
 }
 // ---- the softmax of a tile ------------------------------------------------------------
-// *turn: blocks of this tile's slot so far (over all items); *ends: items that had any.
+// *turn: runs of 64 keys of this tile's slot that came before, even and odd ones;
+// *ends: items that had any.
 template <int DP>
 __device__ __forceinline__ bool softmax_tile(const Args& a, Ctl* ctl, const Item& it, int t, uint32_t tmem,
-                                             uint32_t* turn, uint32_t* ends) {
+                                             uint32_t (&turn)[2], uint32_t* ends) {
   const Tile& tile = it.tile[t];
   if (tile.head < 0) return true;
   const int lane = threadIdx.x & 31, quad = (threadIdx.x >> 5) & 3;
@@ -249,54 +252,48 @@ __device__ __forceinline__ bool softmax_tile(const Args& a, Ctl* ctl, const Item
   const int64_t end64 = a.causal ? shift + i : it.m;
   const int end = (int)(end64 < 0 ? 0 : end64 > it.m ? it.m : end64);
   const int clear = (int)(shift < 0 ? 0 : shift > it.m ? it.m : shift);
-  const bool neg = a.scale2 < 0.f;
-  const float hidden = neg ? INFINITY : -INFINITY;
   const uint64_t scale2 = uk_f2(a.scale2, a.scale2);
+  const int units = tile.units;
 
   float m = -INFINITY, l = 0.f;
-  for (int j = 0; j < tile.blocks; ++j, ++*turn) {
-    if (!wait_warp(ctl, &ctl->s_full[t], *turn & 1u, UK_FAULT_EPILOGUE)) return false;
+  auto step = [&](int u, int h, uint32_t runs) {  // run u, of parity h; runs: of this tile's slot before it
+    if (!wait_warp(ctl, &ctl->s_full[t][h], turn[h] & 1u, UK_FAULT_EPILOGUE)) return false;
+    ++turn[h];
     uk_tc_fence_after();
-    uint32_t s[4][32];
-#pragma unroll
-    for (int c = 0; c < 4; ++c) uk_tmem_ld32(s_at + c * 32, s[c]);
+    const uint32_t at = s_at + h * UN;
+    uint32_t s[2][32];
+    uk_tmem_ld32(at, s[0]);
+    uk_tmem_ld32(at + 32, s[1]);
     uk_tmem_ld_wait();
-    const int base = j * BN;
-    const bool edge = base + BN > clear;  // some row of the tile does not see the whole block
-    auto hide = [&](int c) {
+    const int base = u * UN;
+    if (base + UN > clear) {  // some row of the tile does not see the whole run
 #pragma unroll
-      for (int k = 0; k < 32; ++k)
-        if (base + c * 32 + k >= end) s[c][k] = __float_as_uint(hidden);
-    };
-    if (edge) {
+      for (int c = 0; c < 2; ++c)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) hide(c);
+        for (int k = 0; k < 32; ++k)
+          if (base + c * 32 + k >= end) s[c][k] = 0xff800000u;  // -inf
     }
     float top[4];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) top[c] = hidden;
-    if (!neg) {
+    for (int c = 0; c < 4; ++c) {
+      top[c] = __uint_as_float(s[c / 2][16 * (c % 2)]);
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int k = 0; k < 32; k += 2)
-          top[c] = uk_max3_nan(top[c], __uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1]));
-      top[0] = uk_max3_nan(uk_max3_nan(top[0], top[1], top[2]), top[3], top[3]);
-    } else {
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int k = 0; k < 32; k += 2)
-          top[c] = uk_min3_nan(top[c], __uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1]));
-      top[0] = uk_min3_nan(uk_min3_nan(top[0], top[1], top[2]), top[3], top[3]);
+      for (int k = 1; k < 15; k += 2)
+        top[c] = uk_max3_nan(top[c], __uint_as_float(s[c / 2][16 * (c % 2) + k]),
+                             __uint_as_float(s[c / 2][16 * (c % 2) + k + 1]));
     }
-    const float mt = top[0] * a.scale2;
+    const float rest = uk_max3_nan(__uint_as_float(s[0][15]), __uint_as_float(s[0][31]),
+                                   uk_max3_nan(__uint_as_float(s[1][15]), __uint_as_float(s[1][31]), top[0]));
+    const float mt = uk_max3_nan(uk_max3_nan(top[1], top[2], top[3]), rest, rest) * a.scale2;
     if (__any_sync(0xffffffffu, mt > m + GROW)) {
       const float m2 = fmaxf(m, mt);
       const float f = m2 == -INFINITY ? 1.f : ex2(m - m2);
       m = m2;
       l *= f;
-      if (j > 0) {
+      if (u > 0) {
+        // the run before this one may still be on its way into O
+        if (!wait_warp(ctl, &ctl->pv_done[t], (runs - 1) & 1u, UK_FAULT_EPILOGUE)) return false;
+        uk_tc_fence_after();
 #pragma unroll
         for (int c = 0; c < DP / 16; ++c) {
           uint32_t o[16];
@@ -312,18 +309,9 @@ __device__ __forceinline__ bool softmax_tile(const Args& a, Ctl* ctl, const Item
     const float z = m == -INFINITY ? 0.f : SHIFT - m;
     const uint64_t z2 = uk_f2(z, z);
     uint64_t sum[2] = {uk_f2(0.f, 0.f), uk_f2(0.f, 0.f)};
-    // the second half of the row is read again from TMEM while the first half's
-    // weights are formed: kept in registers, it made them spill
-    uk_tmem_ld32(s_at + 64, s[2]);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
+    for (int c = 0; c < 2; ++c) {
       uint32_t p[16];
-      if (c == 2) {
-        uk_tmem_ld_wait();
-        uk_tmem_ld32(s_at + 96, s[3]);
-      }
-      if (c == 3) uk_tmem_ld_wait();
-      if (c >= 2 && edge) hide(c);
 #pragma unroll
       for (int k = 0; k < 16; ++k) {
         const uint64_t x2 =
@@ -334,25 +322,26 @@ __device__ __forceinline__ bool softmax_tile(const Args& a, Ctl* ctl, const Item
         sum[k & 1] = uk_f2_add(sum[k & 1], uk_f2(x, y));
         p[k] = pack_half(x, y);
       }
-      uk_tmem_st16(s_at + c * 16, p);
-      if (c & 1) {
-        uk_tmem_st_wait();
-        uk_tc_fence_before();
-        __syncwarp();
-        if (lane == 0) uk_mbar_arrive(c == 1 ? &ctl->p_half[t] : &ctl->p_full[t]);
-      }
+      uk_tmem_st16(at + c * 16, p);
     }
+    uk_tmem_st_wait();
+    uk_tc_fence_before();
+    __syncwarp();
+    if (lane == 0) uk_mbar_arrive(&ctl->p_full[t][h]);
     float l0, l1;
     uk_f2_split(uk_f2_add(sum[0], sum[1]), &l0, &l1);
     l += l0 + l1;
-  }
+    return true;
+  };
+  for (int u = 0; u < units; ++u)
+    if (!step(u, u & 1, turn[0] + turn[1])) return false;
 
   // ---- O / l, the log of the sum
   const bool mine = i < tile.rows;
   const int64_t token = (int64_t)it.q0 + tile.first + i;
   uint16_t* out = a.o + token * a.o_token + tile.head * a.o_head;
   bool odd = false;  // a finite sum, but not a finite row
-  if (tile.blocks > 0) {
+  if (units > 0) {
     if (!wait_warp(ctl, &ctl->o_full[t], *ends & 1u, UK_FAULT_EPILOGUE)) return false;
     uk_tc_fence_after();
   }
@@ -360,7 +349,7 @@ __device__ __forceinline__ bool softmax_tile(const Args& a, Ctl* ctl, const Item
 #pragma unroll
   for (int c = 0; c < DP / 32; ++c) {
     uint32_t o[32];
-    if (tile.blocks > 0) {
+    if (units > 0) {
       uk_tmem_ld32(o_at + c * 32, o);
       uk_tmem_ld_wait();
     }
@@ -370,7 +359,7 @@ __device__ __forceinline__ bool softmax_tile(const Args& a, Ctl* ctl, const Item
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         float x = 0.f, y = 0.f;
-        if (tile.blocks > 0) x = __uint_as_float(o[k * 8 + 2 * e]) * inv, y = __uint_as_float(o[k * 8 + 2 * e + 1]) * inv;
+        if (units > 0) x = __uint_as_float(o[k * 8 + 2 * e]) * inv, y = __uint_as_float(o[k * 8 + 2 * e + 1]) * inv;
         odd |= !(fabsf(x) < INFINITY) || !(fabsf(y) < INFINITY);
         w[e] = pack_half(x, y);
       }
@@ -378,7 +367,7 @@ __device__ __forceinline__ bool softmax_tile(const Args& a, Ctl* ctl, const Item
         *reinterpret_cast<uint4*>(out + c * 32 + k * 8) = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
-  if (tile.blocks > 0) {
+  if (units > 0) {
     uk_tc_fence_before();
     __syncwarp();
     if (lane == 0) uk_mbar_arrive(&ctl->o_empty[t]);
@@ -392,7 +381,7 @@ __device__ __forceinline__ bool softmax_tile(const Args& a, Ctl* ctl, const Item
   while (rows != 0) {
     const int r = __ffs(rows) - 1;
     rows &= rows - 1;
-    const int from = __shfl_sync(0xffffffffu, end, r), to = min(tile.blocks * BN, it.m);
+    const int from = __shfl_sync(0xffffffffu, end, r), to = min(units * UN, it.m);
     bool bad = false;
     for (int k = from; k < to && !bad; ++k) {
       const float4 v = row4(a.v + (int64_t)(it.k0 + k) * a.v_token + it.g * a.v_head, lane, a.dim);
@@ -436,7 +425,7 @@ __device__ __forceinline__ void load_items(const Args& a, Ctl* ctl, uint8_t* sme
     for (int j = 0; j < 2 * blocks && ok; ++j) {
       if (j == 0) {
         for (int t = 0; t < 2 && ok; ++t) {
-          if (it.tile[t].blocks == 0) continue;
+          if (it.tile[t].units == 0) continue;
           if (!(ok = wait_warp(ctl, &ctl->q_empty[t], (q_turn[t] & 1u) ^ 1u, UK_FAULT_PRODUCER))) break;
           ++q_turn[t];
           if (lane == 0) {
@@ -494,101 +483,100 @@ __device__ __forceinline__ void load_items(const Args& a, Ctl* ctl, uint8_t* sme
   }
 }
 
-// ---- products ------------------------------------------------------------------------
+// ---- products of tile t ----------------------------------------------------------------
 // The whole warp runs the loop and one elected lane issues: with control flow
-// and operands the same in every lane the descriptors stay in uniform registers.
-// Issued from a branch of a single lane, every product waited for its operands
-// to be moved there, longer than the 64 cycles it runs.
+// and operands the same in every lane the descriptors stay in uniform registers
+// (issued from a branch of a single lane, every product waited for its operands
+// to be moved there).  The tensor core takes few products ahead, so while this
+// warp waits for the softmax it would run dry; the other tile's warp feeds it
+// then (one warp for both tiles left it idle 40 % of the time).
 template <int DP>
-__device__ __forceinline__ void issue_products(Ctl* ctl, uint8_t* smem, uint8_t* ring, uint32_t tmem) {
+__device__ __forceinline__ void issue_products(Ctl* ctl, int t, uint8_t* smem, uint8_t* ring, uint32_t tmem) {
   using S = Smem<DP>;
-  constexpr uint32_t IDESC_S = uk_idesc_f16_ab(BM, BN, 0, 0), IDESC_O = uk_idesc_f16_ab(BM, DP, 0, 1);
-  const bool leader = uk_elect();
-  const uint64_t dq = uk_desc_sw128(uk_smem_u32(smem), 16, 1024);      // K-major: Q and K
+  constexpr uint32_t IDESC_S = uk_idesc_f16_ab(BM, UN, 0, 0), IDESC_O = uk_idesc_f16_ab(BM, DP, 0, 1);
+  const uint32_t leader = uk_elect();
+  const uint64_t dq = uk_desc_sw128(uk_smem_u32(smem + t * S::TILE), 16, 1024);  // K-major: Q and K
   const uint64_t dk = uk_desc_sw128(uk_smem_u32(ring), 16, 1024);
   const uint64_t dv = uk_desc_sw128(uk_smem_u32(ring), S::BOX, 1024);  // MN-major: V
+  const uint32_t s_at = tmem + t * BN, o_at = tmem + 256 + t * 128;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     const bool ok = wait_warp(ctl, bar, parity & 1u, UK_FAULT_MMA);
     uk_tc_fence_after();
     return ok;
   };
-  auto commit = [&](uint64_t* bar) {
-    if (leader) uk_umma_commit(bar);
+  auto commit = [&](uint64_t* bar) { uk_umma_commit_if(leader, bar); };
+  uint32_t slot = 0, phase = 0;              // the ring's next block
+  uint32_t turn[2] = {0, 0}, ends = 0;       // even and odd runs, items of this tile so far
+  auto next_slot = [&] {
+    if (++slot == S::STAGES) slot = 0, phase ^= 1u;
   };
-  uint32_t slot = 0, phase = 0;  // the ring's next block
-  auto scores = [&](int t, uint32_t at) {  // S_t = Q_t K^T, K in the ring's slot `at`
-    const uint64_t q0 = dq + (uint32_t)t * (S::TILE >> 4), k0 = dk + at * (S::TILE >> 4);
-    if (leader) {
+  // S for the even (h = 0) or odd run of the K block in the ring's slot `at`
+  auto scores = [&](int h, uint32_t at) {
+    const uint64_t k0 = dk + at * (S::TILE >> 4) + h * (UN * 128 >> 4);
 #pragma unroll
-      for (int k = 0; k < DP / 16; ++k) {
-        constexpr int BOX16 = S::BOX >> 4;
-        const int off = (k / 4) * BOX16 + (k % 4) * 2;
-        uk_umma_f16(tmem + t * BN, q0 + off, k0 + off, IDESC_S, k > 0);
-      }
-      uk_umma_commit(&ctl->s_full[t]);
+    for (int k = 0; k < DP / 16; ++k) {
+      constexpr int BOX16 = S::BOX >> 4;
+      const int off = (k / 4) * BOX16 + (k % 4) * 2;
+      uk_umma_f16_ss(leader, s_at + h * UN, dq + off, k0 + off, IDESC_S, k > 0);
     }
-    __syncwarp();
+    commit(&ctl->s_full[t][h]);
   };
-  uint32_t turn[2] = {0, 0}, ends[2] = {0, 0};  // blocks and items of each tile so far
   bool ok = true;
   for (uint32_t item = 0; ok; ++item) {
     if (!(ok = wait(&ctl->item_full[item & 1u], item >> 1))) break;
     const Item& it = ctl->item[item & 1u];
-    const int any = __shfl_sync(0xffffffffu, it.any, 0);
-    const int own[2] = {__shfl_sync(0xffffffffu, it.tile[0].blocks, 0), __shfl_sync(0xffffffffu, it.tile[1].blocks, 0)};
+    const int any = __reduce_max_sync(0xffffffffu, it.any);  // the same in every lane, for the compiler too
+    const int own = __reduce_max_sync(0xffffffffu, it.tile[t].units);
+    const int blocks = __reduce_max_sync(0xffffffffu, it.blocks());
     __syncwarp();
     if (leader) uk_mbar_arrive(&ctl->item_empty[item & 1u]);
     if (!any) break;
-    const int blocks = max(own[0], own[1]);
-    if (blocks == 0) continue;
-    // K of the first block
-    ok = wait(&ctl->kv_full[slot], phase);
-    for (int t = 0; t < 2 && ok; ++t)
-      if (own[t] > 0) {
-        if (!(ok = wait(&ctl->q_full[t], ends[t]))) break;
-        scores(t, slot);
-        if (own[t] == 1) commit(&ctl->q_empty[t]);
-      }
-    if (!ok) break;
-    commit(&ctl->kv_empty[slot]);
-    if (++slot == S::STAGES) slot = 0, phase ^= 1u;
+    // Each tile's warp gives every block back, used or not, and never before it
+    // is there: an early return would stand for the other warp's.
+    if (blocks > 0 && !(ok = wait(&ctl->kv_full[slot], phase))) break;
+    if (own > 0) {  // the scores of the first block
+      if (!(ok = wait(&ctl->q_full[t], ends))) break;
+      scores(0, slot);
+      if (own > 1) scores(1, slot);
+      if (own <= 2) commit(&ctl->q_empty[t]);
+    }
+    if (blocks > 0) {
+      commit(&ctl->kv_empty[slot]);
+      next_slot();
+    }
     for (int j = 0; j < blocks && ok; ++j) {
       // V of this block, K of the next
       const bool more = j + 1 < blocks;
       const uint32_t sv = slot, pv = phase;
-      if (++slot == S::STAGES) slot = 0, phase ^= 1u;
-      const uint32_t sk = slot;
-      if (!(ok = wait(&ctl->kv_full[sv], pv) && (!more || wait(&ctl->kv_full[sk], phase)))) break;
+      next_slot();
+      const uint32_t sk = slot, pk = phase;
+      if (more) next_slot();
       const uint64_t v0 = dv + sv * (S::TILE >> 4);
-      for (int t = 0; t < 2 && ok; ++t) {
-        if (j >= own[t]) continue;
-        if (j == 0 && !(ok = wait(&ctl->o_empty[t], ends[t] ^ 1u))) break;
+      if (!(ok = wait(&ctl->kv_full[sv], pv) && (!more || wait(&ctl->kv_full[sk], pk)))) break;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          if (!(ok = ok && wait(half == 0 ? &ctl->p_half[t] : &ctl->p_full[t], turn[t]))) break;
-          if (leader) {
+      for (int h = 0; h < 2; ++h) {
+        const int u = 2 * j + h;
+        if (!ok || u >= own) continue;
+        if (u == 0 && !(ok = wait(&ctl->o_empty[t], ends ^ 1u))) continue;
+        if (!(ok = wait(&ctl->p_full[t][h], turn[h]))) continue;
+        ++turn[h];
 #pragma unroll
-            for (int k = half * 4; k < half * 4 + 4; ++k)  // O_t += P_t V
-              uk_umma_f16_ts(tmem + 256 + t * 128, tmem + t * BN + k * 8, v0 + k * (2048 >> 4), IDESC_O, j > 0 || k > 0);
-          }
-          __syncwarp();
+        for (int k = 0; k < UN / 16; ++k)  // O += P V
+          uk_umma_f16_ts(leader, o_at, s_at + h * UN + k * 8, v0 + (h * (UN / 16) + k) * (2048 >> 4), IDESC_O,
+                         u > 0 || k > 0);
+        commit(&ctl->pv_done[t]);
+        if (u + 2 < own) {
+          scores(h, sk);
+          if (u + 3 == own) commit(&ctl->q_empty[t]);
         }
-        if (!ok) break;
-        ++turn[t];
-        if (j + 1 < own[t]) {
-          scores(t, sk);
-          if (j + 2 == own[t]) commit(&ctl->q_empty[t]);
-        } else {
+        if (u + 1 == own) {
           commit(&ctl->o_full[t]);
-          ++ends[t];
+          ++ends;
         }
       }
       if (!ok) break;
       commit(&ctl->kv_empty[sv]);
-      if (more) {
-        commit(&ctl->kv_empty[sk]);
-        if (++slot == S::STAGES) slot = 0, phase ^= 1u;
-      }
+      if (more) commit(&ctl->kv_empty[sk]);
     }
   }
   // every product issued completes before TMEM and shared memory are given up
@@ -606,27 +594,30 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* ring = smem + 2 * S::TILE;
   Ctl* ctl = (Ctl*)(ring + (size_t)S::STAGES * S::TILE);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // the same in every lane, for the compiler too: the branches by it are uniform
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   if (warp == LOAD_WARP && lane == 0) {
     for (int s = 0; s < S::STAGES; ++s) {
       uk_mbar_init(&ctl->kv_full[s], 1);
-      uk_mbar_init(&ctl->kv_empty[s], 1);
+      uk_mbar_init(&ctl->kv_empty[s], 2);  // both tiles' MMA warps
     }
     for (int t = 0; t < 2; ++t) {
       uk_mbar_init(&ctl->q_full[t], 1);
       uk_mbar_init(&ctl->q_empty[t], 1);
-      uk_mbar_init(&ctl->s_full[t], 1);
-      uk_mbar_init(&ctl->p_half[t], 4);
-      uk_mbar_init(&ctl->p_full[t], 4);
+      for (int h = 0; h < 2; ++h) {
+        uk_mbar_init(&ctl->s_full[t][h], 1);
+        uk_mbar_init(&ctl->p_full[t][h], 4);
+      }
+      uk_mbar_init(&ctl->pv_done[t], 1);
       uk_mbar_init(&ctl->o_full[t], 1);
       uk_mbar_init(&ctl->o_empty[t], 4);
       uk_mbar_init(&ctl->item_full[t], 1);
-      uk_mbar_init(&ctl->item_empty[t], 9);  // 8 softmax warps and the MMA thread
+      uk_mbar_init(&ctl->item_empty[t], 10);  // 8 softmax warps, 2 MMA warps
     }
     uk_mbar_init(&ctl->next, 1);
     uk_mbar_init(&ctl->v_landed, 1);
-    uk_mbar_init(&ctl->teardown, 1);
+    uk_mbar_init(&ctl->teardown, 2);
     ctl->abort = 0;
     uk_fence_mbar_init();
     uk_tma_prefetch_desc(&tm_q);
@@ -644,18 +635,18 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 
   if (warp < 8) {
     uk_regs_up<REGS_SOFTMAX>();
-    uint32_t turn = 0, ends = 0;
+    uint32_t turn[2] = {0, 0}, ends = 0;
     for (uint32_t item = 0;; ++item) {
       if (!wait_warp(ctl, &ctl->item_full[item & 1u], (item >> 1) & 1u, UK_FAULT_EPILOGUE)) break;
       const Item& it = ctl->item[item & 1u];
-      if (!it.any || !softmax_tile<DP>(a, ctl, it, warp >> 2, tmem, &turn, &ends)) break;
+      if (!it.any || !softmax_tile<DP>(a, ctl, it, warp >> 2, tmem, turn, &ends)) break;
       __syncwarp();
       if (lane == 0) uk_mbar_arrive(&ctl->item_empty[item & 1u]);
     }
   } else {
     uk_regs_down<REGS_OTHERS>();
     if (warp == LOAD_WARP) load_items<DP>(a, ctl, smem, ring, tm_q, tm_k, tm_v);
-    else if (warp == MMA_WARP) issue_products<DP>(ctl, smem, ring, tmem);
+    else if (warp < MMA_WARP + 2) issue_products<DP>(ctl, warp - MMA_WARP, smem, ring, tmem);
   }
   __syncwarp();
   uk_tc_fence_before();
@@ -666,13 +657,18 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   }
 }
 
-// No keys at all: every row of the sequences is zero.
-__global__ void __launch_bounds__(256) k_attn_prompt_no_keys(Args a) {
+// Row by row, a warp each: where there are no keys (every row is zero), and for a
+// negative scale, which no model has (the tiles' softmax takes the maximum before
+// it scales).
+__global__ void __launch_bounds__(256) k_attn_prompt_rows(const __grid_constant__ Args a) {
   const int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int64_t t = w / a.heads_q;
   const int h = (int)(w - t * a.heads_q);
-  if (t >= a.total_q || uk_find_seq<true>(a.cu_q, a.n_seq, t) < 0) return;
-  attend_row(a, t, h, 0, 0);
+  const int b = t < a.total_q ? uk_find_seq<true>(a.cu_q, a.n_seq, t) : -1;
+  if (b < 0) return;
+  const int64_t q1 = clamp64(__ldg(a.cu_q + b + 1), 0, a.total_q);
+  const int64_t k0 = clamp64(__ldg(a.cu_k + b), 0, a.total_k), k1 = clamp64(__ldg(a.cu_k + b + 1), k0, a.total_k);
+  attend_row(a, t, h, k0, a.causal ? k1 - (q1 - 1 - t) : k1);
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
@@ -771,10 +767,10 @@ extern "C" int uk_cuda_attn_prompt_f16(const uint16_t* Q, int64_t q_token_stride
   // a zero scale: any factor that no score can raise above rounding does the same
   // and leaves hidden scores at -inf
   if (a.scale2 == 0.f) a.scale2 = 1e-30f;
-  if (total_k == 0) {
+  if (total_k == 0 || a.scale2 < 0.f) {
     const int64_t blocks = (total_q * heads_q + 7) / 8;
     if (blocks > 0x7fffffff) return uk::fail(UK_EINVAL, "attn_prompt: total_q * heads_q exceeds the grid");
-    k_attn_prompt_no_keys<<<(unsigned)blocks, 256, 0, (cudaStream_t)stream>>>(a);
+    k_attn_prompt_rows<<<(unsigned)blocks, 256, 0, (cudaStream_t)stream>>>(a);
     return uk::check_launch("attn_prompt");
   }
   // at most this many query blocks and pairs of tiles, whatever the lengths are
