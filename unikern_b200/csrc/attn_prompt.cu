@@ -53,6 +53,7 @@ struct Args {
   int n_seq, heads_q, heads_kv, group, dim, causal;
   int64_t total_q, total_k;
   float scale2;
+  int levels;  // of the order of work
 };
 
 __device__ __forceinline__ float4 row4(const uint16_t* row, int lane, int dim) {
@@ -144,57 +145,82 @@ struct Item {
   __device__ __forceinline__ int blocks() const { return max(tile[0].blocks(), tile[1].blocks()); }
 };
 
-// Item i of the list: sequences in order; in each the pairs of tiles, the
-// tiles going from the last query block to the first (the longest first where
-// causal) and through the group's heads; a key head each.
-// One warp; lanes sum runs of sequences, the lane whose run holds the item goes on.
-__device__ bool find_item(const Args& a, int64_t item, Item* out) {
+// The list of items, by the work of a pair's first tile: first those of at least
+// 2^(levels - 1) runs of keys, then of half as many, and so on, at the end the
+// rest (blocks take items as they come free, so the last ones should be short).
+// Within a level: sequences in order; in each the pairs of its tiles, the tiles
+// going from the last query block to the first and through the group's heads,
+// for every key head.  A block's items come in rising order, so the search goes
+// on where the last one ended: 32 sequences at a time, a lane each.
+struct Cursor {
+  int level = 0, chunk = 0;
+  int64_t before = 0;  // items before this level's chunk
+};
+
+// One warp: item i, or false behind the list's end.
+__device__ bool find_item(const Args& a, int64_t item, Cursor& at, Item* out) {
   const int lane = threadIdx.x & 31;
-  const int per = (a.n_seq + 31) / 32;
-  const int first = min(lane * per, a.n_seq), last = min(first + per, a.n_seq);
-  auto bounds = [&](int b, int64_t* q0, int64_t* q1) {
-    *q0 = clamp64(__ldg(a.cu_q + b), 0, a.total_q);
-    *q1 = clamp64(__ldg(a.cu_q + b + 1), *q0, a.total_q);
-  };
-  auto items_of = [&](int b) -> int64_t {
-    int64_t q0, q1;
-    bounds(b, &q0, &q1);
-    return (((q1 - q0 + BM - 1) / BM * a.group + 1) / 2) * a.heads_kv;
-  };
-  int64_t mine = 0;
-  for (int b = first; b < last; ++b) mine += items_of(b);
-  int64_t incl = mine;
+  if (item < at.before) at = Cursor{};
+  for (; at.level <= a.levels; ++at.level, at.chunk = 0) {
+    for (; at.chunk * 32 < a.n_seq; ++at.chunk) {
+      const int b = at.chunk * 32 + lane;
+      int64_t q0 = 0, q1 = 0, k0 = 0, k1 = 0;
+      if (b < a.n_seq) {
+        q0 = clamp64(__ldg(a.cu_q + b), 0, a.total_q), q1 = clamp64(__ldg(a.cu_q + b + 1), q0, a.total_q);
+        k0 = clamp64(__ldg(a.cu_k + b), 0, a.total_k), k1 = clamp64(__ldg(a.cu_k + b + 1), k0, a.total_k);
+      }
+      const int n = (int)(q1 - q0), m = (int)(k1 - k0), blocks = (n + BM - 1) / BM;
+      // pairs whose first tile sees at least `units` runs of keys
+      auto pairs = [&](int units) -> int64_t {
+        int64_t tiles = blocks;
+        if (units > 0) {
+          const int64_t end = (int64_t)(units - 1) * UN;  // its last row sees more keys than that
+          if (a.causal) {
+            const int64_t x = end - m + n;
+            tiles = x >= n ? 0 : blocks - (x > 0 ? x / BM : 0);
+          } else if (m <= end) {
+            tiles = 0;
+          }
+        }
+        return (tiles * a.group + 1) / 2;
+      };
+      const int64_t above = at.level == 0 ? 0 : pairs(1 << (a.levels - at.level));
+      const int64_t here = pairs(at.level == a.levels ? 0 : 1 << (a.levels - 1 - at.level)) - above;
+      const int64_t mine = here * a.heads_kv;
+      int64_t incl = mine;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t t = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += t;
-  }
-  const bool found = item >= incl - mine && item < incl;
-  if (found) {
-    int64_t at = item - (incl - mine);
-    int b = first;
-    for (int64_t n; at >= (n = items_of(b)); ++b) at -= n;
-    int64_t q0, q1;
-    bounds(b, &q0, &q1);
-    const int64_t k0 = clamp64(__ldg(a.cu_k + b), 0, a.total_k), k1 = clamp64(__ldg(a.cu_k + b + 1), k0, a.total_k);
-    out->g = (int)(at % a.heads_kv);
-    out->q0 = (int)q0, out->k0 = (int)k0, out->n = (int)(q1 - q0), out->m = (int)(k1 - k0);
-    const int blocks = (out->n + BM - 1) / BM;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t t = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += t;
+      }
+      const int64_t all = __shfl_sync(0xffffffffu, incl, 31);
+      if (item >= at.before + all) {
+        at.before += all;
+        continue;
+      }
+      const int64_t x = item - at.before - (incl - mine);
+      if (x >= 0 && x < mine) {
+        const int64_t pair = above + x / a.heads_kv;
+        out->g = (int)(x % a.heads_kv);
+        out->q0 = (int)q0, out->k0 = (int)k0, out->n = n, out->m = m;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int64_t e = at / a.heads_kv * 2 + t;  // blocks * group fits 47 bits
-      Tile& tile = out->tile[t];
-      tile.head = -1, tile.first = 0, tile.rows = 0, tile.units = 0;
-      if (e >= (int64_t)blocks * a.group) continue;
-      tile.head = out->g * a.group + (int)(e % a.group);
-      tile.first = (blocks - 1 - (int)(e / a.group)) * BM;
-      tile.rows = min(BM, out->n - tile.first);
-      // one past the last key that its last row sees
-      const int64_t end = a.causal ? (int64_t)out->m - out->n + tile.first + tile.rows : out->m;
-      tile.units = end <= 0 ? 0 : (int)((end + UN - 1) / UN);
+        for (int t = 0; t < 2; ++t) {
+          const int64_t e = pair * 2 + t;
+          Tile& tile = out->tile[t];
+          tile.head = -1, tile.first = 0, tile.rows = 0, tile.units = 0;
+          if (e >= (int64_t)blocks * a.group) continue;
+          tile.head = out->g * a.group + (int)(e % a.group);
+          tile.first = (blocks - 1 - (int)(e / a.group)) * BM;
+          tile.rows = min(BM, n - tile.first);
+          // one past the last key that its last row sees
+          const int64_t end = a.causal ? (int64_t)m - n + tile.first + tile.rows : m;
+          tile.units = end <= 0 ? 0 : (int)((end + UN - 1) / UN);
+        }
+      }
+      return true;
     }
   }
-  return __any_sync(0xffffffffu, found);
+  return false;
 }
 
 template <int DP>
@@ -339,33 +365,54 @@ __device__ __forceinline__ bool softmax_tile(const Args& a, Ctl* ctl, const Item
   // ---- O / l, the log of the sum
   const bool mine = i < tile.rows;
   const int64_t token = (int64_t)it.q0 + tile.first + i;
-  uint16_t* out = a.o + token * a.o_token + tile.head * a.o_head;
-  bool odd = false;  // a finite sum, but not a finite row
   if (units > 0) {
     if (!wait_warp(ctl, &ctl->o_full[t], *ends & 1u, UK_FAULT_EPILOGUE)) return false;
     uk_tc_fence_after();
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
+  const uint64_t inv2 = uk_f2(inv, inv), zero2 = uk_f2(0.f, 0.f);
+  uint64_t odd2 = zero2;  // NaN once a value of the row is not finite
+  // Stores go by groups of four lanes: a 4 x 4 transpose of 16-byte pieces
+  // between their rows turns 32 lines touched by every store into 8 (the
+  // store path takes a line per cycle: 2000 cycles a tile pair at dim 64).
+  const int j4 = lane & 3;
+  uint16_t* out = a.o + ((int64_t)it.q0 + tile.first + (i - j4)) * a.o_token + tile.head * a.o_head + j4 * 8;
+  const int rows = tile.rows - (i - j4);  // of the group's four
 #pragma unroll
   for (int c = 0; c < DP / 32; ++c) {
-    uint32_t o[32];
+    uint32_t w[4][4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k][0] = w[k][1] = w[k][2] = w[k][3] = 0;
     if (units > 0) {
+      uint32_t o[32];
       uk_tmem_ld32(o_at + c * 32, o);
       uk_tmem_ld_wait();
-    }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      uint32_t w[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float x = 0.f, y = 0.f;
-        if (units > 0) x = __uint_as_float(o[k * 8 + 2 * e]) * inv, y = __uint_as_float(o[k * 8 + 2 * e + 1]) * inv;
-        odd |= !(fabsf(x) < INFINITY) || !(fabsf(y) < INFINITY);
-        w[e] = pack_half(x, y);
+      for (int k = 0; k < 16; ++k) {
+        const uint64_t v = uk_f2_fma(uk_f2(__uint_as_float(o[2 * k]), __uint_as_float(o[2 * k + 1])), inv2, zero2);
+        odd2 = uk_f2_fma(v, zero2, odd2);
+        float x, y;
+        uk_f2_split(v, &x, &y);
+        w[k / 4][k % 4] = pack_half(x, y);
       }
-      if (mine && c * 32 + k * 8 < a.dim)
-        *reinterpret_cast<uint4*>(out + c * 32 + k * 8) = make_uint4(w[0], w[1], w[2], w[3]);
     }
+#pragma unroll
+    for (int bit = 1; bit < 4; bit *= 2)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (k & bit) continue;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool up = lane & bit;
+          const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? w[k][e] : w[k + bit][e], bit);
+          if (up) w[k][e] = got;
+          else w[k + bit][e] = got;
+        }
+      }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (k < rows && c * 32 + j4 * 8 < a.dim)
+        *reinterpret_cast<uint4*>(out + k * a.o_token + c * 32) = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
   }
   if (units > 0) {
     uk_tc_fence_before();
@@ -376,11 +423,13 @@ __device__ __forceinline__ bool softmax_tile(const Args& a, Ctl* ctl, const Item
   if (mine && a.lse != nullptr)
     a.lse[token * a.heads_q + tile.head] = l == 0.f ? -INFINITY : (m - SHIFT + log2f(l)) * LN2;
 
-  // rows that may have met what their mask hides
-  unsigned rows = __ballot_sync(0xffffffffu, mine && odd && l - l == 0.f);
-  while (rows != 0) {
-    const int r = __ffs(rows) - 1;
-    rows &= rows - 1;
+  // rows that may have met what their mask hides: a finite sum, but not a finite row
+  float odd0, odd1;
+  uk_f2_split(odd2, &odd0, &odd1);
+  unsigned odd = __ballot_sync(0xffffffffu, mine && odd0 + odd1 != 0.f && l - l == 0.f);
+  while (odd != 0) {
+    const int r = __ffs(odd) - 1;
+    odd &= odd - 1;
     const int from = __shfl_sync(0xffffffffu, end, r), to = min(units * UN, it.m);
     bool bad = false;
     for (int k = from; k < to && !bad; ++k) {
@@ -396,7 +445,7 @@ __device__ __forceinline__ bool softmax_tile(const Args& a, Ctl* ctl, const Item
 // ---- items and loads, one warp ---------------------------------------------------------
 template <int DP>
 __device__ __forceinline__ void load_items(const Args& a, Ctl* ctl, uint8_t* smem, uint8_t* ring, const CUtensorMap& tm_q,
-                                           const CUtensorMap& tm_k, const CUtensorMap& tm_v) {
+                                           const CUtensorMap& tm_k, const CUtensorMap& tm_v, Cursor cursor, bool any) {
   using S = Smem<DP>;
   volatile int* abort = &ctl->abort;
   const int lane = threadIdx.x & 31;
@@ -407,8 +456,8 @@ __device__ __forceinline__ void load_items(const Args& a, Ctl* ctl, uint8_t* sme
   for (uint32_t turn = 0; ok; ++turn) {
     Item& it = ctl->item[turn & 1u];
     if (!(ok = wait_warp(ctl, &ctl->item_empty[turn & 1u], ((turn >> 1) & 1u) ^ 1u, UK_FAULT_PRODUCER))) break;
-    bool any = false;
-    if (block >= 0) any = find_item(a, block, &it);
+    // the first item was looked up before the barriers were up
+    if (turn > 0) any = block >= 0 && find_item(a, block, cursor, &it);
     __syncwarp();
     if (lane == 0) {
       it.any = any;
@@ -628,6 +677,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     uk_tmem_alloc(&ctl->tmem, 512);
     uk_tmem_relinquish();
   }
+  Cursor cursor;
+  bool any = false;
+  if (warp == LOAD_WARP) any = find_item(a, blockIdx.x, cursor, &ctl->item[0]);
   uk_tc_fence_before();
   __syncthreads();
   uk_tc_fence_after();
@@ -645,7 +697,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     }
   } else {
     uk_regs_down<REGS_OTHERS>();
-    if (warp == LOAD_WARP) load_items<DP>(a, ctl, smem, ring, tm_q, tm_k, tm_v);
+    if (warp == LOAD_WARP) load_items<DP>(a, ctl, smem, ring, tm_q, tm_k, tm_v, cursor, any);
     else if (warp < MMA_WARP + 2) issue_products<DP>(ctl, warp - MMA_WARP, smem, ring, tmem);
   }
   __syncwarp();
@@ -763,7 +815,7 @@ extern "C" int uk_cuda_attn_prompt_f16(const uint16_t* Q, int64_t q_token_stride
     if (int rc = uk::check_device_ptr(LSE, "LSE")) return rc;
   Args a{Q, K, V, O, q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride,
          o_token_stride, o_head_stride, LSE, cu_q, cu_k, n_seq, heads_q, heads_kv, heads_q / heads_kv, dim, causal,
-         total_q, total_k, scale * LOG2E};
+         total_q, total_k, scale * LOG2E, 0};
   // a zero scale: any factor that no score can raise above rounding does the same
   // and leaves hidden scores at -inf
   if (a.scale2 == 0.f) a.scale2 = 1e-30f;
@@ -774,6 +826,10 @@ extern "C" int uk_cuda_attn_prompt_f16(const uint16_t* Q, int64_t q_token_stride
     return uk::check_launch("attn_prompt");
   }
   // at most this many query blocks and pairs of tiles, whatever the lengths are
+  // the order of work: a level per power of two of the keys a tile can see; with
+  // many sequences every level is a long search, and the order matters less
+  if (n_seq <= 1024)
+    while ((total_k + UN - 1) / UN >> a.levels) ++a.levels;
   const int64_t seqs = n_seq < total_q ? n_seq : total_q;
   const int64_t q_blocks = total_q / BM + seqs < total_q ? total_q / BM + seqs : total_q;
   const int64_t items = (q_blocks * a.group + seqs) / 2 * heads_kv;
