@@ -14,7 +14,7 @@
 //   tail of long sequences, no empty CTAs.  A run that covers a pair whole
 //   writes O; a pair cut by a run's end leaves (m, l, o) in the workspace, at
 //   most two per CTA (the pair that entered its run, the pair that leaves it).
-// * k_attn_join: for each pair that left a run, the sum of its parts in the
+// * k_attn_join_few / _many: for each pair that left a run, the sum of its parts in the
 //   order of the CTAs (deterministic); launched programmatically behind the
 //   first.
 //
@@ -67,6 +67,7 @@ struct Args {
   // (by_pair), else one per CTA
   int4* recs;
   int by_pair;
+  int unit;  // bytes: a power of two that divides the cache's strides; rows are passed between lanes in units
 };
 
 template <int KIND, int DP>
@@ -205,20 +206,23 @@ __global__ void __launch_bounds__(THREADS, NH == 1 ? 3 : 2) k_attn_decode(Args a
   const int64_t room = (int64_t)c.max_pages * c.page_size;
   const int pairs = c.heads * a.chunks;
 
-  // sequences without positions have no tiles: their rows are written here
-  for (int b = blockIdx.x; b < a.n_seq; b += gridDim.x) {
-    const int len = __ldg(a.lens + b);
-    if (len > room && threadIdx.x == 0) atomicOr(&uk::g_attn_decode_fault, UK_FAULT_PAGE);
-    if (len > 0 && room > 0) continue;
-    for (int i = threadIdx.x; i < a.heads_q * (c.dim / 8); i += THREADS) {
-      const int h = i / (c.dim / 8), d = i % (c.dim / 8);
-      reinterpret_cast<uint4*>(a.o + b * a.o_seq + h * a.o_head)[d] = make_uint4(0, 0, 0, 0);
+  // sequences without positions have no tiles: their rows are written at the
+  // end, off the way to the first loads
+  auto write_empty = [&] {
+    for (int b = blockIdx.x; b < a.n_seq; b += gridDim.x) {
+      const int len = __ldg(a.lens + b);
+      if (len > room && threadIdx.x == 0) atomicOr(&uk::g_attn_decode_fault, UK_FAULT_PAGE);
+      if (len > 0 && room > 0) continue;
+      for (int i = threadIdx.x; i < a.heads_q * (c.dim / 8); i += THREADS) {
+        const int h = i / (c.dim / 8), d = i % (c.dim / 8);
+        reinterpret_cast<uint4*>(a.o + b * a.o_seq + h * a.o_head)[d] = make_uint4(0, 0, 0, 0);
+      }
+      if (a.lse != nullptr)
+        for (int h = threadIdx.x; h < a.heads_q; h += THREADS) a.lse[(int64_t)b * a.heads_q + h] = -INFINITY;
+      if (a.by_pair)
+        for (int i = threadIdx.x; i < pairs; i += THREADS) a.recs[b * pairs + i] = make_int4(-1, 0, 0, 0);
     }
-    if (a.lse != nullptr)
-      for (int h = threadIdx.x; h < a.heads_q; h += THREADS) a.lse[(int64_t)b * a.heads_q + h] = -INFINITY;
-    if (a.by_pair)
-      for (int i = threadIdx.x; i < pairs; i += THREADS) a.recs[b * pairs + i] = make_int4(-1, 0, 0, 0);
-  }
+  };
 
   int64_t x0, x1, before;
   int b;
@@ -226,6 +230,7 @@ __global__ void __launch_bounds__(THREADS, NH == 1 ? 3 : 2) k_attn_decode(Args a
   int4 rec = make_int4(-1, 0, 0, 0);
   if (x0 >= x1) {
     if (threadIdx.x == 0 && !a.by_pair) a.recs[blockIdx.x] = rec;
+    write_empty();
     return;
   }
 
@@ -243,12 +248,17 @@ __global__ void __launch_bounds__(THREADS, NH == 1 ? 3 : 2) k_attn_decode(Args a
     const int p1 = (int)min((int64_t)t1 * CT, (int64_t)len);  // one past the run's last
 
     // The rows of a warp tile at p.  kWhole: group n's page id and then the
-    // byte offset of its first row, the same in every lane; else lane i's own
-    // for position p + i.  -1: absent.  e: position p + lane's exponent bytes,
-    // the key's below the value's.
+    // byte offset of its first row, the same in every lane (-1: absent).  Else
+    // lane i's own for position p + i, the offset in units (ABSENT), with its
+    // exponent bytes (e4m3).  K and V load one tile ahead, page ids two (three
+    // without kWhole, and rows and exponents two): an instruction that needs a
+    // load stops the warp until it is there.
     constexpr int NR = kWhole ? NT : 1;
+    constexpr uint32_t ABSENT = 0xffffffffu;
     struct Where {
       int64_t row[NR];
+      uint32_t unit;
+      uint32_t ek, ev;
     };
     auto page_of = [&](int p, int (&page)[NR]) {
 #pragma unroll
@@ -257,9 +267,9 @@ __global__ void __launch_bounds__(THREADS, NH == 1 ? 3 : 2) k_attn_decode(Args a
         page[n] = pos < p1 && (kWhole || lane < WT) ? __ldg(table + c.div.div((uint32_t)pos)) : -1;
       }
     };
-    auto rows_of = [&](int p, const int (&page)[NR], uint32_t* e) {
+    auto rows_of = [&](int p, const int (&page)[NR]) {
       Where w;
-      *e = 127u | 127u << 8;
+      w.unit = ABSENT, w.ek = w.ev = 127;
 #pragma unroll
       for (int n = 0; n < NR; ++n) {
         const int pos = kWhole ? p + n * 16 : p + lane;
@@ -268,9 +278,11 @@ __global__ void __launch_bounds__(THREADS, NH == 1 ? 3 : 2) k_attn_decode(Args a
           if ((unsigned)page[n] < (uint64_t)c.pages) {
             const int off = pos - (int)c.div.div((uint32_t)pos) * c.page_size;
             w.row[n] = uk_kv_row(c, page[n], off, g);
+            if (!kWhole) w.unit = (uint32_t)((uint64_t)w.row[n] / (uint32_t)a.unit);
             if (!S::kF16) {
               const int64_t at = uk_kv_exp(c, page[n], off, g);
-              *e = __ldg(c.k_exp + at) | (uint32_t)__ldg(c.v_exp + at) << 8;
+              w.ek = __ldg(c.k_exp + at);
+              w.ev = __ldg(c.v_exp + at);
             }
           } else {
             atomicOr(&uk::g_attn_decode_fault, UK_FAULT_PAGE);
@@ -279,65 +291,109 @@ __global__ void __launch_bounds__(THREADS, NH == 1 ? 3 : 2) k_attn_decode(Args a
       }
       return w;
     };
-    // the row of position p + n * 16 + i, or -1
-    auto row_at = [&](const Where& w, int p, int n, int i) -> int64_t {
-      if (kWhole) return w.row[n] < 0 || p + n * 16 + i >= p1 ? -1 : w.row[n] + (int64_t)i * c.token_bytes;
-      return __shfl_sync(0xffffffffu, w.row[0], n * 16 + i);
-    };
 
     uint4 kr[NT][2][S::KC];
     uint32_t vr[NT][4][S::VC][S::VW];
     unsigned seen = 0;  // bit 2 n + i: position 16 n + 8 i + r of the tile counts
+    // a warp tile without absent positions, of rows as long as the operands:
+    // nothing to check per load
+    bool plain = false;
+    auto get_k = [&](const uint8_t* kp, bool on, uint4 (&to)[S::KC]) {
+#pragma unroll
+      for (int k = 0; k < S::KC; ++k) to[k] = ldg16(kp + k * 64, on && (k * 64 + q * 16) / (S::kF16 ? 2 : 1) < c.dim);
+    };
+    auto get_v = [&](const uint8_t* vp, bool on, uint32_t (&to)[S::VC][S::VW]) {
+#pragma unroll
+      for (int k = 0; k < S::VC; ++k) {
+        const bool y = on && (k * 128 + r * S::VB) / (S::kF16 ? 2 : 1) < c.dim;
+        if (S::VB == 16) {
+          const uint4 v = ldg16(vp + k * 128, y);
+          to[k][0] = v.x, to[k][1] = v.y, to[k][S::VW - 2] = v.z, to[k][S::VW - 1] = v.w;
+        } else {
+          const uint2 v = ldg8(vp + k * 128, y);
+          to[k][0] = v.x, to[k][1] = v.y;
+        }
+      }
+    };
     auto load_k = [&](const Where& w, int p) {
       seen = 0;
+      if constexpr (kWhole) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int64_t at = row_at(w, p, n, i * 8 + r);
-          if (at >= 0) seen |= 1u << (2 * n + i);
-          const uint8_t* kp = c.k + at + q * 16;
+          for (int i = 0; i < 2; ++i) {
+            const bool on = w.row[n] >= 0 && p + n * 16 + i * 8 + r < p1;
+            if (on) seen |= 1u << (2 * n + i);
+            get_k(c.k + w.row[n] + (int64_t)(i * 8 + r) * c.token_bytes + q * 16, on, kr[n][i]);
+          }
+      } else {
+        plain = c.dim == DP && __all_sync(0xffffffffu, lane >= WT || w.unit != ABSENT);
+        const uint8_t* kq = c.k + q * 16;
 #pragma unroll
-          for (int k = 0; k < S::KC; ++k)
-            kr[n][i][k] = ldg16(kp + k * 64, at >= 0 && (k * 64 + q * 16) / (S::kF16 ? 2 : 1) < c.dim);
-        }
-    };
-    auto load_v = [&](const Where& w, int p) {
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t u = __shfl_sync(0xffffffffu, w.unit, n * 16 + i * 8 + r);
+            const uint8_t* kp = kq + (uint64_t)u * (uint32_t)a.unit;
+            if (plain) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int64_t at = row_at(w, p, n, (i >> 1) * 8 + 2 * q + (i & 1));
-          const uint8_t* vp = c.v + at + r * S::VB;
-#pragma unroll
-          for (int k = 0; k < S::VC; ++k) {
-            const bool on = at >= 0 && (k * 128 + r * S::VB) / (S::kF16 ? 2 : 1) < c.dim;
-            if (S::VB == 16) {
-              const uint4 v = ldg16(vp + k * 128, on);
-              vr[n][i][k][0] = v.x;
-              vr[n][i][k][1] = v.y;
-              vr[n][i][k][S::VW - 2] = v.z;
-              vr[n][i][k][S::VW - 1] = v.w;
+              for (int k = 0; k < S::KC; ++k) kr[n][i][k] = ldg16(kp + k * 64, true);
             } else {
-              const uint2 v = ldg8(vp + k * 128, on);
-              vr[n][i][k][0] = v.x;
-              vr[n][i][k][1] = v.y;
+              if (u != ABSENT) seen |= 1u << (2 * n + i);
+              get_k(kp, u != ABSENT, kr[n][i]);
             }
           }
-        }
+        if (plain) seen = (1u << (2 * NT)) - 1;
+      }
+    };
+    auto load_v = [&](const Where& w, int p) {
+      if constexpr (kWhole) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int x = (i >> 1) * 8 + 2 * q + (i & 1);
+            get_v(c.v + w.row[n] + (int64_t)x * c.token_bytes + r * S::VB, w.row[n] >= 0 && p + n * 16 + x < p1,
+                  vr[n][i]);
+          }
+      } else {
+        const uint8_t* vq = c.v + r * S::VB;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t u = __shfl_sync(0xffffffffu, w.unit, n * 16 + (i >> 1) * 8 + 2 * q + (i & 1));
+            const uint8_t* vp = vq + (uint64_t)u * (uint32_t)a.unit;
+            if (plain) {
+#pragma unroll
+              for (int k = 0; k < S::VC; ++k) {
+                if (S::VB == 16) {
+                  const uint4 v = ldg16(vp + k * 128, true);
+                  vr[n][i][k][0] = v.x, vr[n][i][k][1] = v.y, vr[n][i][k][S::VW - 2] = v.z, vr[n][i][k][S::VW - 1] = v.w;
+                } else {
+                  const uint2 v = ldg8(vp + k * 128, true);
+                  vr[n][i][k][0] = v.x, vr[n][i][k][1] = v.y;
+                }
+              }
+            } else {
+              get_v(vp, u != ABSENT, vr[n][i]);
+            }
+          }
+      }
     };
 
     // the first tile's loads go out before Q is brought into shape
-    uint32_t e, e_next = 0;
-    int page_next[NR];
-    Where rows;
+    int page[NR];
+    Where rows, next;
     if (p0 < p1) {
-      int page[NR];
-      page_of(p0, page);
-      page_of(p0 + CT, page_next);
-      rows = rows_of(p0, page, &e);
+      int first[NR], second[NR];
+      page_of(p0, first);
+      page_of(p0 + CT, kWhole ? page : second);
+      if constexpr (!kWhole) page_of(p0 + 2 * CT, page);
+      rows = rows_of(p0, first);
       load_k(rows, p0);
       load_v(rows, p0);
+      if constexpr (!kWhole) next = rows_of(p0 + CT, second);
     }
 
     // Q in the operand's order of d; absent heads and d behind dim are zero
@@ -398,14 +454,27 @@ __global__ void __launch_bounds__(THREADS, NH == 1 ? 3 : 2) k_attn_decode(Args a
       }
       const unsigned now = seen;
       // ---- the next tile's rows and keys
-      rows = rows_of(p + CT, page_next, &e_next);
-      page_of(p + 2 * CT, page_next);
+      const Where now_at = rows;
+      if constexpr (kWhole) {
+        rows = rows_of(p + CT, page);
+        page_of(p + 2 * CT, page);
+      } else {
+        rows = next;
+        next = rows_of(p + 2 * CT, page);
+        page_of(p + 3 * CT, page);
+      }
       load_k(rows, p + CT);
 
       // ---- scores, reference and weights.  e4m3: the value row's scale 2^ev
       // goes into the weight's exponent, t = s + ev, and the codes enter the
       // product unscaled; l takes 2^(t - m) 2^-ev in fp32.
       float top[NH][2], inv_ev[NT][2];
+      float ek = 1.f, ev = 0.f, inv = 1.f;  // of this lane's position: scale * 2^ek, ev and 2^-ev
+      if (!S::kF16) {
+        ek = a.scale2 * uk_exp_scale(now_at.ek);
+        ev = __uint_as_float(0x4b000000u | now_at.ev) - 8388735.f;  // ev - 127, through 2^23
+        inv = uk_exp_scale(254u - now_at.ev);
+      }
 #pragma unroll
       for (int w = 0; w < NH; ++w) top[w][0] = top[w][1] = -INFINITY;
 #pragma unroll
@@ -414,10 +483,10 @@ __global__ void __launch_bounds__(THREADS, NH == 1 ? 3 : 2) k_attn_decode(Args a
         for (int i = 0; i < 2; ++i) {
           float f = 1.f, add = 0.f;
           if (!S::kF16) {
-            const uint32_t y = __shfl_sync(0xffffffffu, e, n * 16 + i * 8 + r);
-            f = a.scale2 * uk_exp_scale(y & 255u);
-            add = (float)((int)(y >> 8) - 127);
-            inv_ev[n][i] = uk_exp_scale(254u - (y >> 8));
+            const int from = n * 16 + i * 8 + r;
+            f = __shfl_sync(0xffffffffu, ek, from);
+            add = __shfl_sync(0xffffffffu, ev, from);
+            inv_ev[n][i] = __shfl_sync(0xffffffffu, inv, from);
           }
           const bool on = now >> (2 * n + i) & 1u;
 #pragma unroll
@@ -501,7 +570,6 @@ __global__ void __launch_bounds__(THREADS, NH == 1 ? 3 : 2) k_attn_decode(Args a
         }
       }
       load_v(rows, p + CT);
-      e = e_next;
     }
 
     // ---- the four warps' parts joined in shared memory
@@ -579,12 +647,73 @@ __global__ void __launch_bounds__(THREADS, NH == 1 ? 3 : 2) k_attn_decode(Args a
     }
   }
   if (threadIdx.x == 0 && !a.by_pair) a.recs[blockIdx.x] = rec;
+  write_empty();
+}
+
+// A warp per (cut pair, query head of its run), the parts one after the other
+// with a running reference, four loads of each kind in flight and nothing to
+// wait for between warps: for pairs of few parts.
+template <int DP, int NH>
+__global__ void __launch_bounds__(256) k_attn_join_few(Args a, int dim) {
+  uk_pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int4 rec = a.recs[blockIdx.x / NH];
+  const int b = rec.x, pair = rec.y, first = rec.z, n = rec.w - first + 1;
+  const int head = (blockIdx.x % NH) * 8 + warp;
+  if (b < 0) return;
+  const int g = pair / a.chunks, h = g * a.group + (pair % a.chunks) * 8 * NH + head;
+  if (h >= (g + 1) * a.group) return;
+  constexpr int LANES = DP / 4, PER = 32 / LANES, U = 4;  // lanes of a part's row; a warp takes PER parts at a time
+  const int d4 = lane % LANES;
+  float m = -INFINITY, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = lane / LANES; i0 < n; i0 += U * PER) {
+    float mi[U], li[U];
+    float4 v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * PER;
+      mi[u] = -INFINITY, li[u] = 0.f, v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i < n) {
+        const float* p = a.parts + ((int64_t)(first + i) * 2 + (i == 0 ? 1 : 0)) * part_floats(DP, NH);
+        mi[u] = p[head];
+        li[u] = p[8 * NH + head];
+        v[u] = reinterpret_cast<const float4*>(p + 16 * NH + head * DP)[d4];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float m2 = fmaxf(m, mi[u]);
+      const float f = m == m2 ? 1.f : ex2(m - m2), e = mi[u] == -INFINITY ? 1.f : ex2(mi[u] - m2);
+      m = m2;
+      l = l * f + li[u] * e;
+      o = make_float4(o.x * f + v[u].x * e, o.y * f + v[u].y * e, o.z * f + v[u].z * e, o.w * f + v[u].w * e);
+    }
+  }
+  if (PER == 2) {  // the two halves' sums
+    const float m1 = __shfl_xor_sync(0xffffffffu, m, 16), m2 = fmaxf(m, m1);
+    const float f = m == -INFINITY ? 1.f : ex2(m - m2), e = m1 == -INFINITY ? 1.f : ex2(m1 - m2);
+    m = m2;
+    l = l * f + __shfl_xor_sync(0xffffffffu, l, 16) * e;
+    o.x = o.x * f + __shfl_xor_sync(0xffffffffu, o.x, 16) * e;
+    o.y = o.y * f + __shfl_xor_sync(0xffffffffu, o.y, 16) * e;
+    o.z = o.z * f + __shfl_xor_sync(0xffffffffu, o.z, 16) * e;
+    o.w = o.w * f + __shfl_xor_sync(0xffffffffu, o.w, 16) * e;
+  }
+  if (lane >= LANES) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  if (d4 * 4 < dim)
+    reinterpret_cast<uint2*>(a.o + b * a.o_seq + (int64_t)h * a.o_head)[d4] =
+        make_uint2(pack_half(o.x * inv, o.y * inv), pack_half(o.z * inv, o.w * inv));
+  if (a.lse != nullptr && d4 == 0)
+    a.lse[(int64_t)b * a.heads_q + h] = l == 0.f ? -INFINITY : (m - SHIFT + log2f(l)) * LN2;
 }
 
 // One CTA per (cut pair, query head of its run): weights of the parts, then
-// their sum, the warps taking turns.
-template <int DP, int NH, int JT>
-__global__ void __launch_bounds__(JT) k_attn_join(Args a, int dim) {
+// their sum, the warps taking turns: for pairs of many parts.
+template <int DP, int NH>
+__global__ void __launch_bounds__(512) k_attn_join_many(Args a, int dim) {
+  constexpr int JT = 512;
   constexpr int JW = JT / 32;
   __shared__ float wt[MAX_CTAS];
   __shared__ float red[33];
@@ -656,19 +785,22 @@ size_t workspace_bytes_for(int ctas, int dp, int nh) {
 template <int DP, int NH>
 int launch_join(const Args& a, int dim, int ctas, cudaStream_t st) {
   const int64_t all = (int64_t)a.n_seq * (a.heads_q / a.group) * a.chunks;
-  // 16 warps where a pair can have more parts than four warps keep in flight
-  const bool wide = a.by_pair && ctas / all >= 16;
+  // 16 warps per head where a pair can have many parts (one sequence of 131071
+  // with two key heads, 148 parts a pair: 7.5 us against 17.4 by four warps);
+  // else a warp per head
+  const bool many = a.by_pair && ctas / all >= 16;
+  const int64_t recs = a.by_pair ? all : ctas;
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr{};
-  cfg.gridDim = dim3((unsigned)((a.by_pair ? all : ctas) * 8 * NH), 1, 1);
-  cfg.blockDim = dim3(wide ? 512 : THREADS, 1, 1);
+  cfg.gridDim = dim3((unsigned)(recs * (many ? 8 * NH : NH)), 1, 1);
+  cfg.blockDim = dim3(many ? 512 : 256, 1, 1);
   cfg.stream = st;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = wide ? cudaLaunchKernelEx(&cfg, k_attn_join<DP, NH, 512>, a, dim)
-                             : cudaLaunchKernelEx(&cfg, k_attn_join<DP, NH, THREADS>, a, dim);
+  const cudaError_t e = many ? cudaLaunchKernelEx(&cfg, k_attn_join_many<DP, NH>, a, dim)
+                             : cudaLaunchKernelEx(&cfg, k_attn_join_few<DP, NH>, a, dim);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return uk::fail(UK_ECUDA, "attn_decode: %s", cudaGetErrorString(e));
@@ -727,8 +859,18 @@ extern "C" int uk_cuda_attn_decode_f16(const uint16_t* Q, int64_t q_seq_stride, 
   if (workspace_bytes < need || !uk::aligned16(workspace))
     return uk::fail(UK_EINVAL, "attn_decode: workspace of %zu bytes, %zu wanted, 16-byte aligned", workspace_bytes, need);
   Args a{Q, q_seq_stride, q_head_stride, O, o_seq_stride, o_head_stride, LSE, seq_lens, n_seq, heads_q, group,
-         (group + 8 * nh - 1) / (8 * nh), scale * LOG2E, nullptr, (int4*)workspace, 0};
+         (group + 8 * nh - 1) / (8 * nh), scale * LOG2E, nullptr, (int4*)workspace, 0, 0};
   a.by_pair = (int64_t)n_seq * cache->heads * a.chunks <= ctas;
+  // rows cross lanes as 32-bit multiples of the strides' common power of two
+  int64_t strides = 4096;
+  if (c.pages > 1) strides |= c.page_bytes;
+  if (c.page_size > 1) strides |= c.token_bytes;
+  if (c.heads > 1) strides |= c.head_bytes;
+  a.unit = (int)(strides & -strides);
+  const int64_t far = (c.pages - 1) * c.page_bytes + (c.page_size - 1) * c.token_bytes + (c.heads - 1) * c.head_bytes;
+  if (c.pages > 0 && far / a.unit >= 0xffffffffll)
+    return uk::fail(UK_EINVAL, "attn_decode: a pool of %lld bytes with strides of multiples of %d bytes only",
+                    (long long)far, a.unit);
   a.parts = reinterpret_cast<float*>(a.recs + ctas);
   const cudaStream_t st = (cudaStream_t)stream;
   switch ((cache->kind == UK_KV_E4M3 ? 4 : 0) + (dp == 128 ? 2 : 0) + (nh - 1)) {
