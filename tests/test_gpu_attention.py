@@ -105,6 +105,28 @@ def test_decode_work_split(kind, lens):
     check_decode(pool, q, o, lse, 64 ** -0.5)
 
 
+@pytest.mark.parametrize("kind,page", [("f16", 16), ("f16", 5), ("e4m3", 32)])
+@pytest.mark.parametrize("heads,group,dim", [(8, 4, 128), (2, 12, 64), (1, 1, 32), (3, 20, 112)])
+def test_decode_short_tables(kind, page, heads, group, dim):
+    """Few pairs and short tables: every length around the shares of a cluster,
+    the same sequence beside others and alone, tables with room to spare."""
+    a = abi()
+    fault()
+    for lens in ([0], [1], [7], [63, 0], [64, 65], [511, 512, 0], [513], [0, 0, 1000]):
+        pool = Pool(kind, "hnd", heads, dim, page, lens, seed=4, table_pad=3)
+        q = randn(len(lens), heads * group, dim, seed=6)
+        o, lse = torch.full_like(q, math.nan), torch.full(q.shape[:2], math.nan, device="cuda")
+        a.attn_decode(q, pool.cache, pool.table, pool.lens_t, o, lse=lse)
+        check_decode(pool, q, o, lse, dim ** -0.5)
+        # the same table with far more room takes the other split of the work
+        wide = torch.full((len(lens), 70000 // page), -1, dtype=torch.int32, device="cuda")
+        wide[:, :pool.table.shape[1]] = pool.table
+        o2, lse2 = torch.full_like(q, math.nan), torch.full(q.shape[:2], math.nan, device="cuda")
+        a.attn_decode(q, pool.cache, wide, pool.lens_t, o2, lse=lse2)
+        check_decode(pool, q, o2, lse2, dim ** -0.5)
+    assert fault() == 0
+
+
 @pytest.mark.parametrize("kind", ["f16", "e4m3"])
 def test_decode_long(kind):
     """One long sequence, one key head: many parts joined; a strong first key

@@ -194,14 +194,22 @@ __device__ Line find_begin(const Args& a, int64_t room, int pairs, int64_t* x0, 
 // looked up by one lane and passed to the others (32 x 8192 f16 positions: 173
 // against 186 us).  e4m3 takes the second form always: its exponents are looked
 // up by position in any case (ragged 32 x 8192: 68 against 79 us with kWhole).
-template <int KIND, int DP, int NH, bool kWhole>
+//
+// kCluster: short caches of few pairs.  The eight CTAs of a cluster take a
+// pair's tiles in equal shares and add their sums up through distributed shared
+// memory: one launch, no workspace (use_clusters has the rule and both sides).
+constexpr int CLUSTER = 8;
+
+template <int KIND, int DP, int NH, bool kWhole, bool kCluster>
 __global__ void __launch_bounds__(THREADS, NH == 1 ? 3 : 2) k_attn_decode(Args a, UkKvView c) {
   using S = Shape<KIND, DP>;
   constexpr int CT = S::CT, WT = S::WT, NT = S::NT;
   __shared__ float sm_m[WARPS][8 * NH], sm_l[WARPS][8 * NH];
   __shared__ __align__(16) float sm_o[WARPS][8 * NH][DP + 2];
+  __shared__ float sum_m[kCluster ? 8 * NH : 1], sum_l[kCluster ? 8 * NH : 1];  // of this CTA's four warps
+  __shared__ __align__(16) float sum_o[kCluster ? 8 * NH : 1][kCluster ? DP : 4];
 
-  uk_pdl_launch_dependents();
+  if (!kCluster) uk_pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, q = lane & 3;
   const int64_t room = (int64_t)c.max_pages * c.page_size;
   const int pairs = c.heads * a.chunks;
@@ -224,21 +232,32 @@ __global__ void __launch_bounds__(THREADS, NH == 1 ? 3 : 2) k_attn_decode(Args a
     }
   };
 
-  int64_t x0, x1, before;
-  int b;
-  const Line line = find_begin<CT>(a, room, pairs, &x0, &x1, &b, &before);
+  int64_t x0 = 0, x1 = 0, before = 0;
+  int b, len, nt, pair;
+  Line line{0, 0};
   int4 rec = make_int4(-1, 0, 0, 0);
-  if (x0 >= x1) {
-    if (threadIdx.x == 0 && !a.by_pair) a.recs[blockIdx.x] = rec;
-    write_empty();
-    return;
+  if (kCluster) {
+    pair = (int)(blockIdx.x / CLUSTER);
+    b = pair / pairs;
+    pair -= b * pairs;
+    len = clamped_len(a, room, b), nt = (len + CT - 1) / CT;
+    const int rank = (int)(blockIdx.x % CLUSTER);
+    x0 = (int64_t)nt * rank / CLUSTER, x1 = (int64_t)nt * (rank + 1) / CLUSTER;
+    if (threadIdx.x == 0 && rank == 0 && __ldg(a.lens + b) > room) atomicOr(&uk::g_attn_decode_fault, UK_FAULT_PAGE);
+  } else {
+    line = find_begin<CT>(a, room, pairs, &x0, &x1, &b, &before);
+    if (x0 >= x1) {
+      if (threadIdx.x == 0 && !a.by_pair) a.recs[blockIdx.x] = rec;
+      write_empty();
+      return;
+    }
+    len = clamped_len(a, room, b), nt = (len + CT - 1) / CT;
+    pair = (int)((x0 - before * pairs) / nt);
   }
 
   int64_t x = x0;
-  int len = clamped_len(a, room, b), nt = (len + CT - 1) / CT;
-  int pair = (int)((x - before * pairs) / nt);
-  while (x < x1) {
-    const int64_t start = before * pairs + (int64_t)pair * nt;
+  for (bool more = true; more;) {
+    const int64_t start = kCluster ? 0 : before * pairs + (int64_t)pair * nt;
     const int t0 = (int)(x - start), t1 = (int)min((int64_t)nt, x1 - start);
     const int g = pair / a.chunks, h0 = g * a.group + (pair % a.chunks) * 8 * NH;
     const int heads = min(8 * NH, (g + 1) * a.group - h0);  // query heads of this run
@@ -611,7 +630,11 @@ __global__ void __launch_bounds__(THREADS, NH == 1 ? 3 : 2) k_attn_decode(Args a
 #pragma unroll
         for (int k = 0; k < 8; ++k) o[k] += sm_o[w][head][d + k] * f;
       }
-      if (entered || leaves) {
+      if (kCluster) {
+        if (d == 0) sum_m[head] = mm, sum_l[head] = ll;
+        *reinterpret_cast<float4*>(&sum_o[head][d]) = make_float4(o[0], o[1], o[2], o[3]);
+        *reinterpret_cast<float4*>(&sum_o[head][d + 4]) = make_float4(o[4], o[5], o[6], o[7]);
+      } else if (entered || leaves) {
         if (d == 0) {
           part[head] = mm;
           part[8 * NH + head] = ll;
@@ -629,6 +652,40 @@ __global__ void __launch_bounds__(THREADS, NH == 1 ? 3 : 2) k_attn_decode(Args a
           a.lse[(int64_t)b * a.heads_q + h0 + head] = ll == 0.f ? -INFINITY : (mm - SHIFT + log2f(ll)) * LN2;
       }
     }
+    if constexpr (kCluster) {
+      uk_cluster_sync();
+      // each CTA adds up an eighth of the pair's values, in the order of the ranks
+      const int i = (int)(blockIdx.x % CLUSTER) + CLUSTER * (int)threadIdx.x;
+      if (i < heads * LANES) {
+        const int head = i / LANES, d = (i % LANES) * 8;
+        float mi[CLUSTER], mm = -INFINITY, ll = 0.f, o[8];
+#pragma unroll
+        for (int k = 0; k < CLUSTER; ++k) {
+          mi[k] = uk_ld_dsmem_f32(uk_mapa(uk_smem_u32(&sum_m[head]), k));
+          mm = fmaxf(mm, mi[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) o[k] = 0.f;
+#pragma unroll
+        for (int k = 0; k < CLUSTER; ++k) {
+          const float f = mi[k] == -INFINITY ? 1.f : ex2(mi[k] - mm);
+          ll += uk_ld_dsmem_f32(uk_mapa(uk_smem_u32(&sum_l[head]), k)) * f;
+          const uint32_t at = uk_mapa(uk_smem_u32(&sum_o[head][d]), k);
+          const float4 u = uk_ld_dsmem_f32x4(at), v = uk_ld_dsmem_f32x4(at + 16);
+          o[0] += u.x * f, o[1] += u.y * f, o[2] += u.z * f, o[3] += u.w * f;
+          o[4] += v.x * f, o[5] += v.y * f, o[6] += v.z * f, o[7] += v.w * f;
+        }
+        const float inv = ll == 0.f ? 0.f : 1.f / ll;
+        if (d < c.dim)
+          *reinterpret_cast<uint4*>(a.o + b * a.o_seq + (int64_t)(h0 + head) * a.o_head + d) =
+              make_uint4(pack_half(o[0] * inv, o[1] * inv), pack_half(o[2] * inv, o[3] * inv),
+                         pack_half(o[4] * inv, o[5] * inv), pack_half(o[6] * inv, o[7] * inv));
+        if (a.lse != nullptr && d == 0)
+          a.lse[(int64_t)b * a.heads_q + h0 + head] = ll == 0.f ? -INFINITY : (mm - SHIFT + log2f(ll)) * LN2;
+      }
+      uk_cluster_sync();  // no CTA leaves while another reads its shared memory
+      return;
+    }
     if (!entered) {
       if (leaves) rec = make_int4(b, pair, blockIdx.x, (int)line.owner(start + nt - 1));
       if (a.by_pair && threadIdx.x == 0) a.recs[b * pairs + pair] = leaves ? rec : make_int4(-1, 0, 0, 0);
@@ -636,7 +693,8 @@ __global__ void __launch_bounds__(THREADS, NH == 1 ? 3 : 2) k_attn_decode(Args a
     __syncthreads();
 
     x = start + t1;
-    if (x < x1 && ++pair == pairs) {
+    more = x < x1;
+    if (more && ++pair == pairs) {
       pair = 0;
       before += nt;
       do {
@@ -782,6 +840,18 @@ size_t workspace_bytes_for(int ctas, int dp, int nh) {
   return (size_t)ctas * (sizeof(int4) + 2 * sizeof(float) * part_floats(dp, nh));
 }
 
+// Clusters of eight CTAs per pair, or the even split and its join?  The lengths are
+// not known here, the table's room is.  Clusters while they all run at once (two
+// CTAs per SM) and a CTA's share of the room, room / 8, is at most as many
+// positions as eight per CTA of the grid.  Measured on one B200 in a graph, 8 key
+// heads of 128, clusters against the split: 1 sequence of 500 4.5 / 7.7 us, 4000
+// 10.3 / 11.5, 8000 15.9 / 13.6; 4 sequences of 500 5.8 / 10.0, 16000 47.6 / 49.7;
+// 7 sequences (448 CTAs) of 2000 16.8 / 16.5, 13 of 500 15.1 / 12.7.
+bool use_clusters(int64_t pairs, int64_t room) {
+  const int64_t ctas = pairs * CLUSTER;
+  return ctas <= 2 * uk::sm_count() && room / CLUSTER <= 8 * ctas;
+}
+
 template <int DP, int NH>
 int launch_join(const Args& a, int dim, int ctas, cudaStream_t st) {
   const int64_t all = (int64_t)a.n_seq * (a.heads_q / a.group) * a.chunks;
@@ -808,14 +878,38 @@ int launch_join(const Args& a, int dim, int ctas, cudaStream_t st) {
   return UK_OK;
 }
 
-template <int KIND, int DP, int NH>
+template <int KIND, int DP, int NH, bool kWhole>
 int launch(const Args& a, const UkKvView& c, int ctas, cudaStream_t st) {
-  bool whole = false;
-  if constexpr (KIND == UK_KV_F16)
-    if ((whole = c.page_size % 16 == 0)) k_attn_decode<KIND, DP, NH, true><<<(unsigned)ctas, THREADS, 0, st>>>(a, c);
-  if (!whole) k_attn_decode<KIND, DP, NH, false><<<(unsigned)ctas, THREADS, 0, st>>>(a, c);
+  const int64_t all = (int64_t)a.n_seq * c.heads * a.chunks;
+  if (use_clusters(all, (int64_t)c.max_pages * c.page_size)) {
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr{};
+    cfg.gridDim = dim3((unsigned)(all * CLUSTER), 1, 1);
+    cfg.blockDim = dim3(THREADS, 1, 1);
+    cfg.stream = st;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = CLUSTER;
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, k_attn_decode<KIND, DP, NH, kWhole, true>, a, c);
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      return uk::fail(UK_ECUDA, "attn_decode: %s", cudaGetErrorString(e));
+    }
+    return UK_OK;
+  }
+  k_attn_decode<KIND, DP, NH, kWhole, false><<<(unsigned)ctas, THREADS, 0, st>>>(a, c);
   if (int rc = uk::check_launch("attn_decode")) return rc;
   return launch_join<DP, NH>(a, c.dim, ctas, st);
+}
+
+template <int KIND, int DP, int NH>
+int launch(const Args& a, const UkKvView& c, int ctas, cudaStream_t st) {
+  if constexpr (KIND == UK_KV_F16)
+    if (c.page_size % 16 == 0) return launch<KIND, DP, NH, true>(a, c, ctas, st);
+  return launch<KIND, DP, NH, false>(a, c, ctas, st);
 }
 
 }  // namespace
