@@ -397,8 +397,9 @@ int uk_cuda_attn_decode_f16(const uint16_t* Q, int64_t q_seq_stride, int64_t q_h
  * LSE [total_q][heads_q] as above, or NULL.  A query that sees no key gives
  * zeros and -inf.  Rows of O and LSE outside cu_q[0] .. cu_q[n_seq] - 1 are left
  * as they were.  cu_q and cu_k are device memory, non-decreasing within
- * [0, total_q] and [0, total_k]; values outside are clamped.  fp32 scores,
- * statistics and sums; the softmax weights enter the value product as binary16.
+ * [0, total_q] and [0, total_k]; values outside are clamped.  total_k up to
+ * 2^27.  fp32 scores, statistics and sums; the softmax weights enter the value
+ * product as binary16.  A negative scale runs row by row on CUDA cores.
  * Deterministic. */
 int uk_cuda_attn_prompt_f16(const uint16_t* Q, int64_t q_token_stride, int64_t q_head_stride, const uint16_t* K,
                             int64_t k_token_stride, int64_t k_head_stride, const uint16_t* V, int64_t v_token_stride,

@@ -60,7 +60,7 @@ def test_bad_caches(call, kw):
     lambda c: decode(None), lambda c: decode(c, heads_q=3), lambda c: decode(c, heads_q=0),
     lambda c: decode(c, n_seq=-1), lambda c: decode(c, scale=float("inf")), lambda c: decode(c, scale=float("nan")),
     lambda c: decode(c, max_pages=1), lambda c: decode(c),
-    lambda c: prompt(n_seq=-1), lambda c: prompt(tq=-1), lambda c: prompt(tk=1 << 33), lambda c: prompt(hq=3),
+    lambda c: prompt(n_seq=-1), lambda c: prompt(tq=-1), lambda c: prompt(tk=1 << 33), lambda c: prompt(tk=(1 << 27) + 1), lambda c: prompt(hq=3),
     lambda c: prompt(hk=0), lambda c: prompt(dim=12), lambda c: prompt(dim=256), lambda c: prompt(scale=float("nan")),
     lambda c: prompt(),
 ])

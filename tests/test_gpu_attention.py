@@ -1,11 +1,12 @@
 """Attention over a paged cache (one new token per sequence) and over packed
 prompts on the GPU, against the definition in 64 bits; bounds in attn_testutil."""
+import ctypes
 import math
 
 import pytest
 import torch
 
-from attn_testutil import Pool, assert_close, attention_f64, same_bits
+from attn_testutil import Pool, assert_close, attention_f64, quantise_f64, same_bits
 
 pytestmark = pytest.mark.gpu
 
@@ -220,23 +221,41 @@ def test_decode_absent_pages():
         check_decode(full, qq, o1, l1, 0.125)
 
 
-def test_decode_offsets_past_32_bits():
+@pytest.mark.parametrize("kind,page", [("f16", 16), ("f16", 7), ("e4m3", 16)])
+def test_decode_offsets_past_32_bits(kind, page):
     a = abi()
-    heads, dim, ps = 2, 64, 16
-    stride = (1 << 31) // 2 + 64
-    k, v = (torch.empty(4 * stride + ps * heads * dim, dtype=torch.float16, device="cuda")
-            .as_strided((5, ps, heads, dim), (stride, heads * dim, dim, 1)) for _ in "kv")
-    x = [randn(40, heads, dim, seed=i) for i in range(2)]
+    fault()
+    heads, dim = 2, 64
+    es, dt = (2, torch.float16) if kind == "f16" else (1, torch.float8_e4m3fn)
+    stride = (1 << 31) // es + 64  # elements: five pages span more than 8 GB
+    k, v = (torch.empty((4 * stride + page * heads * dim) * es, dtype=torch.uint8, device="cuda").view(dt)
+            .as_strided((5, page, heads, dim), (stride, heads * dim, dim, 1)) for _ in "kv")
+    e = [torch.empty(5, heads, page, dtype=torch.uint8, device="cuda") if kind == "e4m3" else None for _ in "kv"]
+    n = 3 * page - 2
+    x = [randn(n, heads, dim, seed=i) for i in range(2)]
     table = i32([[4, 0, 3]])
-    cache = a.KvCache(k, v)
-    a.kv_append(x[0], x[1], cache, table, i32([0, 40]), i32([40]))
+    cache = a.KvCache(k, v, *e)
+    a.kv_append(x[0], x[1], cache, table, i32([0, n]), i32([n]))
+    held = [t.double() if kind == "f16" else quantise_f64(t)[0] for t in x]
     q = randn(1, 6, dim, seed=7)
-    o = torch.empty_like(q)
-    a.attn_decode(q, cache, table, i32([40]), o)
-    seen = torch.ones(3, 40, dtype=torch.bool, device="cuda")
-    for g in range(heads):
-        ro, _, to, _ = attention_f64(q[0, 3 * g:3 * g + 3], x[0][:, g], x[1][:, g], dim ** -0.5, seen)
-        assert_close(o[0, 3 * g:3 * g + 3], ro, to, "o")
+    for room in (3, 9000):  # both splits of the work
+        wide = torch.full((1, room), -1, dtype=torch.int32, device="cuda")
+        wide[:, :3] = table
+        o = torch.empty_like(q)
+        a.attn_decode(q, cache, wide, i32([n]), o)
+        seen = torch.ones(3, n, dtype=torch.bool, device="cuda")
+        for g in range(heads):
+            ro, _, to, _ = attention_f64(q[0, 3 * g:3 * g + 3], held[0][:, g], held[1][:, g], dim ** -0.5, seen)
+            assert_close(o[0, 3 * g:3 * g + 3], ro, to, "o")
+    assert fault() == 0
+    # a pool whose rows 32 bits of its strides' common unit do not reach is refused
+    far = a.KvCacheStruct(*[getattr(cache.struct, f[0]) for f in a.KvCacheStruct._fields_])
+    far.pages, far.page_stride, far.token_stride = 1 << 30, 4096 + 8 * 16 // es, heads * dim
+    ws = a.attn_decode_workspace(cache, 6)
+    rc = a.lib().uk_cuda_attn_decode_f16(q.data_ptr(), q.stride(0), q.stride(1), ctypes.byref(far), table.data_ptr(), 3,
+                                         3, i32([n]).data_ptr(), 1, 6, 0.125, o.data_ptr(), o.stride(0), o.stride(1),
+                                         None, ws.data_ptr(), ws.numel(), None)
+    assert rc == 2
 
 
 # ---- packed prompts -------------------------------------------------------------------
@@ -446,6 +465,41 @@ def test_two_streams_with_a_workspace_each():
     torch.cuda.synchronize()
     for i, o in enumerate(got):
         assert same_bits(o, want[i % 2])
+
+
+def test_prompts_on_two_streams():
+    a = abi()
+    cu = i32([0, 700, 1500])
+    sets = [[randn(1500, h, d, seed=10 * i + s) for s, h in enumerate((8, 4, 4))] for i, d in enumerate((128, 64))]
+    want = [torch.empty_like(s[0]) for s in sets]
+    for s, o in zip(sets, want):
+        a.attn_prompt(*s, cu, cu, o)
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in sets], []
+    for rep in range(8):
+        for s, st in zip(sets, streams):
+            got.append(torch.empty_like(s[0]))
+            a.attn_prompt(*s, cu, cu, got[-1], stream=st)
+    torch.cuda.synchronize()
+    for i, o in enumerate(got):
+        assert same_bits(o, want[i % 2])
+    assert fault() == 0
+
+
+def test_prompt_more_keys_than_queries_ragged_groups():
+    """Odd groups, where a pair of tiles spans two query blocks with different
+    numbers of keys, and sequences whose tiles see no key at all between others."""
+    a = abi()
+    nq, nk = [300, 500, 129, 260, 1, 700], [100, 640, 0, 261, 300, 700]
+    for heads, group, dim in ((2, 3, 128), (1, 5, 64), (3, 1, 128)):
+        cu_q, cu_k = prefix(nq), prefix(nk)
+        q = randn(cu_q[-1], heads * group, dim, seed=1)
+        k, v = randn(cu_k[-1], heads, dim, seed=2), randn(cu_k[-1], heads, dim, seed=3)
+        for causal in (True, False):
+            o, lse = torch.full_like(q, math.nan), torch.full(q.shape[:2], math.nan, device="cuda")
+            a.attn_prompt(q, k, v, i32(cu_q), i32(cu_k), o, causal=causal, lse=lse)
+            check_prompt(q, k, v, cu_q, cu_k, o, lse, dim ** -0.5, causal)
+    assert fault() == 0
 
 
 def test_captured_and_replayed():

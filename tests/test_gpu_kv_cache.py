@@ -43,6 +43,11 @@ CASES = [  # kind, layout, heads, dim, page_size, lengths before, rows appended
     ("e4m3", "hnd", 8, 128, 16, [0, 100], [300, 77]),
     ("e4m3", "nhd", 7, 112, 64, [3], [129]),
     ("e4m3", "hnd", 4, 64, 128, [1000, 0], [5, 260]),
+    ("e4m3", "nhd", 1100, 16, 2, [1, 0], [2, 3]),  # more rows per token than a block stages exponents of
+    ("e4m3", "hnd", 2, 32, 16, [0] * 1500, [i % 3 for i in range(1500)]),  # more sequences than it holds bounds of
+    ("f16", "hnd", 1, 16, 16, [i % 5 for i in range(1023)], [i % 2 for i in range(1023)]),
+    ("f16", "nhd", 2, 64, 16, [0], [12000]),  # many tokens to a block
+    ("e4m3", "hnd", 2, 96, 48, [5, 0], [7001, 5000]),
 ]
 
 

@@ -794,7 +794,8 @@ extern "C" int uk_cuda_attn_prompt_f16(const uint16_t* Q, int64_t q_token_stride
                                        int64_t total_k, int heads_q, int heads_kv, int dim, float scale, int causal,
                                        uint16_t* O, int64_t o_token_stride, int64_t o_head_stride, float* LSE,
                                        void* stream) {
-  if (n_seq < 0 || total_q < 0 || total_k < 0 || total_q > 0x7fffffff || total_k > 0x7fffffff)
+  // 2^27 keys: a tile's pass over them stays well within the kernel's bounded waits
+  if (n_seq < 0 || total_q < 0 || total_k < 0 || total_q > 0x7fffffff || total_k > (1 << 27))
     return uk::fail(UK_EINVAL, "attn_prompt: n_seq %d, total_q %lld, total_k %lld", n_seq, (long long)total_q,
                     (long long)total_k);
   if (heads_kv < 1 || heads_q < 1 || heads_q > 65535 || heads_q % heads_kv != 0)
