@@ -502,6 +502,40 @@ def test_prompt_more_keys_than_queries_ragged_groups():
     assert fault() == 0
 
 
+@pytest.mark.parametrize("heads,group,dim", [(1, 1, 128), (1, 3, 64), (2, 4, 128), (2, 2, 40), (1, 7, 96)])
+def test_prompt_few_rows_behind_long_contexts(heads, group, dim):
+    """Few tiles over many keys: the keys are shared between blocks, evenly and
+    not, with shares that hold no key a row sees."""
+    a = abi()
+    for nq, nk in (([1], [5000]), ([130], [8192]), ([200], [4097]), ([3, 0, 40], [9000, 100, 1]),
+                   ([128], [2049]), ([5], [1024]), ([77, 33], [3000, 20000]), ([300], [300]), ([64], [40])):
+        cu_q, cu_k = [2 + c for c in prefix(nq)], [3 + c for c in prefix(nk)]
+        q = randn(cu_q[-1] + 4, heads * group, dim, seed=1)
+        k, v = randn(cu_k[-1] + 200, heads, dim, seed=2), randn(cu_k[-1] + 200, heads, dim, seed=3)
+        for x, cu in ((q, cu_q), (k, cu_k), (v, cu_k)):
+            x[:cu[0]], x[cu[-1]:] = math.nan, math.nan
+        for causal in (True, False):
+            o, lse = torch.full_like(q, 7.0), torch.full(q.shape[:2], 7.0, device="cuda")
+            a.attn_prompt(q, k, v, i32(cu_q), i32(cu_k), o, causal=causal, lse=lse)
+            check_prompt(q, k, v, cu_q, cu_k, o, lse, dim ** -0.5, causal)
+            for x in (o, lse):
+                assert (x[:cu_q[0]] == 7).all() and (x[cu_q[-1]:] == 7).all()
+    assert fault() == 0
+
+
+def test_prompt_few_rows_masked_nan():
+    """The same split with NaN at the keys that the last rows alone see."""
+    a = abi()
+    n, m, dim = 20, 6000, 64
+    q, k, v = randn(n, 2, dim, seed=1), randn(m, 2, dim, seed=2), randn(m, 2, dim, seed=3)
+    v[m - 5, 0, 7], v[m - 1] = math.nan, math.inf
+    o, lse = torch.empty_like(q), torch.empty(n, 2, device="cuda")
+    a.attn_prompt(q, k, v, i32([0, n]), i32([0, m]), o, lse=lse)
+    check_prompt(q[:15, :1], k[:m - 5, :1], v[:m - 5, :1], [0, 15], [0, m - 5], o[:15, :1], lse[:15, :1], 0.125, True)
+    check_prompt(q[:19, 1:], k[:m - 1, 1:], v[:m - 1, 1:], [0, 19], [0, m - 1], o[:19, 1:], lse[:19, 1:], 0.125, True)
+    assert torch.isnan(o[15:, 0, 7]).all() and not torch.isfinite(o[19]).any()
+
+
 def test_captured_and_replayed():
     """Decode and prompt in one graph, replayed with other lengths and inputs;
     the workspace serves an eager call between replays."""

@@ -54,6 +54,8 @@ struct Args {
   int64_t total_q, total_k;
   float scale2;
   int levels;  // of the order of work
+  int tiles;   // of an item: 2, or 1 where pairs would leave SMs without work
+  int split;   // CTAs (a cluster) that share a tile's keys
 };
 
 __device__ __forceinline__ float4 row4(const uint16_t* row, int lane, int dim) {
@@ -142,6 +144,8 @@ struct Item {
   int g;             // key head
   int q0, k0, n, m;  // the sequence: its first rows, query and key counts
   int any;           // 0: there is no further item
+  int first_block;   // the first block of keys that this CTA works on
+  int all_units;     // tile 0's runs of keys, of which tile[0].units are this CTA's
   __device__ __forceinline__ int blocks() const { return max(tile[0].blocks(), tile[1].blocks()); }
 };
 
@@ -182,7 +186,7 @@ __device__ bool find_item(const Args& a, int64_t item, Cursor& at, Item* out) {
             tiles = 0;
           }
         }
-        return (tiles * a.group + 1) / 2;
+        return (tiles * a.group + a.tiles - 1) / a.tiles;
       };
       const int64_t above = at.level == 0 ? 0 : pairs(1 << (a.levels - at.level));
       const int64_t here = pairs(at.level == a.levels ? 0 : 1 << (a.levels - 1 - at.level)) - above;
@@ -203,12 +207,13 @@ __device__ bool find_item(const Args& a, int64_t item, Cursor& at, Item* out) {
         const int64_t pair = above + x / a.heads_kv;
         out->g = (int)(x % a.heads_kv);
         out->q0 = (int)q0, out->k0 = (int)k0, out->n = n, out->m = m;
+        out->first_block = 0;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const int64_t e = pair * 2 + t;
+          const int64_t e = pair * a.tiles + t;
           Tile& tile = out->tile[t];
           tile.head = -1, tile.first = 0, tile.rows = 0, tile.units = 0;
-          if (e >= (int64_t)blocks * a.group) continue;
+          if (t >= a.tiles || e >= (int64_t)blocks * a.group) continue;
           tile.head = out->g * a.group + (int)(e % a.group);
           tile.first = (blocks - 1 - (int)(e / a.group)) * BM;
           tile.rows = min(BM, n - tile.first);
@@ -245,6 +250,7 @@ struct Ctl {
   alignas(16) uint8_t answer[16];
   uint32_t tmem;
   int abort;
+  unsigned odd[4];  // rows of a shared tile to look at again
   Item item[2];
 };
 static_assert(sizeof(Ctl) <= 768, "control block");
@@ -264,20 +270,48 @@ __device__ __forceinline__ bool wait_warp(Ctl* ctl, uint64_t* bar, uint32_t pari
 // ---- the softmax of a tile ------------------------------------------------------------
 // *turn: runs of 64 keys of this tile's slot that came before, even and odd ones;
 // *ends: items that had any.
+// One past the last key that row i of a tile sees.
+__device__ __forceinline__ int end_of_row(const Args& a, const Item& it, const Tile& tile, int i) {
+  const int64_t end = a.causal ? (int64_t)it.m - it.n + tile.first + 1 + i : it.m;
+  return (int)(end < 0 ? 0 : end > it.m ? it.m : end);
+}
+
+// A row with a finite sum that is not finite itself (one warp): it is computed
+// again where one of the keys between its mask and the end of its blocks is not.
+__device__ __noinline__ void look_again(const Args& a, const Item& it, const Tile& tile, int row, int units) {
+  const int lane = threadIdx.x & 31, from = end_of_row(a, it, tile, row), to = min(units * UN, it.m);
+  bool bad = false;
+  for (int k = from; k < to && !bad; ++k) {
+    const float4 v = row4(a.v + (int64_t)(it.k0 + k) * a.v_token + it.g * a.v_head, lane, a.dim);
+    bad = __any_sync(0xffffffffu, !(fabsf(v.x) + fabsf(v.y) + fabsf(v.z) + fabsf(v.w) < INFINITY));
+  }
+  __syncwarp();  // the row's stores before come before these
+  if (bad) attend_row(a, (int64_t)it.q0 + tile.first + row, tile.head, it.k0, (int64_t)it.k0 + from);
+}
+
+// A shared tile's sums in shared memory: 128 rows of DP floats (16-byte pieces
+// exchanged by the row's low bits: a thread per row writes without conflicts),
+// then the rows' references and sums.
 template <int DP>
+struct Shared {
+  float* o;
+  float* m;
+  float* l;
+  __device__ __forceinline__ explicit Shared(uint8_t* ring)
+      : o((float*)ring), m((float*)(ring + 2 * Smem<DP>::TILE)), l(m + BM) {}
+  __device__ __forceinline__ float* piece(int row, int c) const { return o + row * DP + (c ^ (row & 7)) * 4; }
+};
+
+template <int DP, bool kSplit>
 __device__ __forceinline__ bool softmax_tile(const Args& a, Ctl* ctl, const Item& it, int t, uint32_t tmem,
-                                             uint32_t (&turn)[2], uint32_t* ends) {
+                                             uint8_t* ring, uint32_t (&turn)[2], uint32_t* ends) {
   const Tile& tile = it.tile[t];
   if (tile.head < 0) return true;
   const int lane = threadIdx.x & 31, quad = (threadIdx.x >> 5) & 3;
   const int i = quad * 32 + lane;  // row of the tile
   const uint32_t lanes = (uint32_t)(quad * 32) << 16;
   const uint32_t s_at = tmem + lanes + t * BN, o_at = tmem + lanes + 256 + t * 128;
-  // one past the last key that the tile's first row and this row see
-  const int64_t shift = a.causal ? (int64_t)it.m - it.n + tile.first + 1 : it.m;
-  const int64_t end64 = a.causal ? shift + i : it.m;
-  const int end = (int)(end64 < 0 ? 0 : end64 > it.m ? it.m : end64);
-  const int clear = (int)(shift < 0 ? 0 : shift > it.m ? it.m : shift);
+  const int end = end_of_row(a, it, tile, i), clear = end_of_row(a, it, tile, 0);
   const uint64_t scale2 = uk_f2(a.scale2, a.scale2);
   const int units = tile.units;
 
@@ -291,7 +325,7 @@ __device__ __forceinline__ bool softmax_tile(const Args& a, Ctl* ctl, const Item
     uk_tmem_ld32(at, s[0]);
     uk_tmem_ld32(at + 32, s[1]);
     uk_tmem_ld_wait();
-    const int base = u * UN;
+    const int base = (u + (kSplit ? 2 * it.first_block : 0)) * UN;
     if (base + UN > clear) {  // some row of the tile does not see the whole run
 #pragma unroll
       for (int c = 0; c < 2; ++c)
@@ -369,6 +403,24 @@ __device__ __forceinline__ bool softmax_tile(const Args& a, Ctl* ctl, const Item
     if (!wait_warp(ctl, &ctl->o_full[t], *ends & 1u, UK_FAULT_EPILOGUE)) return false;
     uk_tc_fence_after();
   }
+  if constexpr (kSplit) {
+    const Shared<DP> sh(ring);  // every product has read its blocks: the ring is free
+    sh.m[i] = m, sh.l[i] = l;
+#pragma unroll
+    for (int c = 0; c < DP / 32; ++c) {
+      uint32_t o[32];
+#pragma unroll
+      for (int k = 0; k < 32; ++k) o[k] = 0;
+      if (units > 0) {
+        uk_tmem_ld32(o_at + c * 32, o);
+        uk_tmem_ld_wait();
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        *reinterpret_cast<uint4*>(sh.piece(i, c * 8 + k)) = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+    }
+    return true;
+  }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const uint64_t inv2 = uk_f2(inv, inv), zero2 = uk_f2(0.f, 0.f);
   uint64_t odd2 = zero2;  // NaN once a value of the row is not finite
@@ -430,20 +482,55 @@ __device__ __forceinline__ bool softmax_tile(const Args& a, Ctl* ctl, const Item
   while (odd != 0) {
     const int r = __ffs(odd) - 1;
     odd &= odd - 1;
-    const int from = __shfl_sync(0xffffffffu, end, r), to = min(units * UN, it.m);
-    bool bad = false;
-    for (int k = from; k < to && !bad; ++k) {
-      const float4 v = row4(a.v + (int64_t)(it.k0 + k) * a.v_token + it.g * a.v_head, lane, a.dim);
-      bad = __any_sync(0xffffffffu, !(fabsf(v.x) + fabsf(v.y) + fabsf(v.z) + fabsf(v.w) < INFINITY));
-    }
-    __syncwarp();  // the row's stores above come before these
-    if (bad) attend_row(a, (int64_t)it.q0 + tile.first + quad * 32 + r, tile.head, it.k0, (int64_t)it.k0 + from);
+    look_again(a, it, tile, quad * 32 + r, units);
   }
   return true;
 }
 
-// ---- items and loads, one warp ---------------------------------------------------------
+// ---- a shared tile: the CTAs of a cluster add up their sums, a share of the rows each -----
+// The eight softmax warps: the others have given their registers away.
 template <int DP>
+__device__ __forceinline__ void join_shares(const Args& a, Ctl* ctl, uint8_t* ring) {
+  const Shared<DP> sh(ring);
+  const Item& it = ctl->item[0];
+  const Tile& tile = it.tile[0];
+  const int rank = (int)(blockIdx.x % a.split), rows = BM / a.split;
+  for (int x = threadIdx.x; x < rows * (DP / 8); x += 256) {
+    const int row = rank * rows + x / (DP / 8), d = x % (DP / 8) * 8;
+    if (row >= tile.rows || d >= a.dim) continue;
+    float mm = -INFINITY, l = 0.f, o[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) o[k] = 0.f;
+    for (int c = 0; c < a.split; ++c) mm = fmaxf(mm, uk_ld_dsmem_f32(uk_mapa(uk_smem_u32(sh.m + row), c)));
+    for (int c = 0; c < a.split; ++c) {  // in the order of the ranks
+      const float m = uk_ld_dsmem_f32(uk_mapa(uk_smem_u32(sh.m + row), c)), f = m == -INFINITY ? 1.f : ex2(m - mm);
+      const float4 u = uk_ld_dsmem_f32x4(uk_mapa(uk_smem_u32(sh.piece(row, d / 4)), c));
+      const float4 v = uk_ld_dsmem_f32x4(uk_mapa(uk_smem_u32(sh.piece(row, d / 4 + 1)), c));
+      l += uk_ld_dsmem_f32(uk_mapa(uk_smem_u32(sh.l + row), c)) * f;
+      o[0] += u.x * f, o[1] += u.y * f, o[2] += u.z * f, o[3] += u.w * f;
+      o[4] += v.x * f, o[5] += v.y * f, o[6] += v.z * f, o[7] += v.w * f;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    bool odd = false;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      o[k] *= inv;
+      odd |= !(fabsf(o[k]) < INFINITY);
+    }
+    const int64_t token = (int64_t)it.q0 + tile.first + row;
+    *reinterpret_cast<uint4*>(a.o + token * a.o_token + tile.head * a.o_head + d) = make_uint4(
+        pack_half(o[0], o[1]), pack_half(o[2], o[3]), pack_half(o[4], o[5]), pack_half(o[6], o[7]));
+    if (a.lse != nullptr && d == 0)
+      a.lse[token * a.heads_q + tile.head] = l == 0.f ? -INFINITY : (mm - SHIFT + log2f(l)) * LN2;
+    if (odd && l - l == 0.f) atomicOr(&ctl->odd[row / 32], 1u << (row % 32));
+  }
+  asm volatile("bar.sync 1, 256;" ::: "memory");
+  for (int row = rank * rows + (int)(threadIdx.x >> 5); row < (rank + 1) * rows; row += 8)
+    if (ctl->odd[row / 32] >> (row % 32) & 1u) look_again(a, it, tile, row, it.all_units);
+}
+
+// ---- items and loads, one warp ---------------------------------------------------------
+template <int DP, bool kSplit>
 __device__ __forceinline__ void load_items(const Args& a, Ctl* ctl, uint8_t* smem, uint8_t* ring, const CUtensorMap& tm_q,
                                            const CUtensorMap& tm_k, const CUtensorMap& tm_v, Cursor cursor, bool any) {
   using S = Smem<DP>;
@@ -462,14 +549,14 @@ __device__ __forceinline__ void load_items(const Args& a, Ctl* ctl, uint8_t* sme
     if (lane == 0) {
       it.any = any;
       uk_mbar_arrive(&ctl->item_full[turn & 1u]);  // releases the item to the waiting warps
-      if (any) {
+      if (any && !kSplit) {
         uk_mbar_expect_tx(&ctl->next, 16);
         uk_next_block_ask(ctl->answer, &ctl->next);
       }
     }
     __syncwarp();
     if (!any) break;
-    asked = true;
+    asked = !kSplit;
     const int blocks = it.blocks();
     for (int j = 0; j < 2 * blocks && ok; ++j) {
       if (j == 0) {
@@ -488,7 +575,7 @@ __device__ __forceinline__ void load_items(const Args& a, Ctl* ctl, uint8_t* sme
         }
         if (!ok) break;
       }
-      const int s = n % S::STAGES, at = (j >> 1) * BN;  // K and V blocks alternate
+      const int s = n % S::STAGES, at = (it.first_block + (j >> 1)) * BN;  // K and V blocks alternate
       if (!(ok = wait_warp(ctl, &ctl->kv_empty[s], ((n / S::STAGES) & 1u) ^ 1u, UK_FAULT_PRODUCER))) break;
       const bool fix = (j & 1) && at + BN > it.m;
       uint8_t* dst = ring + (size_t)s * S::TILE;
@@ -515,7 +602,7 @@ __device__ __forceinline__ void load_items(const Args& a, Ctl* ctl, uint8_t* sme
         if (lane == 0) uk_mbar_arrive(&ctl->kv_full[s]);
       }
     }
-    if (!ok) break;
+    if (!ok || kSplit) break;
     if (!(ok = wait_warp(ctl, &ctl->next, answers & 1u, UK_FAULT_PRODUCER))) break;
     ++answers;
     asked = false;
@@ -539,7 +626,7 @@ __device__ __forceinline__ void load_items(const Args& a, Ctl* ctl, uint8_t* sme
 // to be moved there).  The tensor core takes few products ahead, so while this
 // warp waits for the softmax it would run dry; the other tile's warp feeds it
 // then (one warp for both tiles left it idle 40 % of the time).
-template <int DP>
+template <int DP, bool kSplit>
 __device__ __forceinline__ void issue_products(Ctl* ctl, int t, uint8_t* smem, uint8_t* ring, uint32_t tmem) {
   using S = Smem<DP>;
   constexpr uint32_t IDESC_S = uk_idesc_f16_ab(BM, UN, 0, 0), IDESC_O = uk_idesc_f16_ab(BM, DP, 0, 1);
@@ -627,6 +714,7 @@ __device__ __forceinline__ void issue_products(Ctl* ctl, int t, uint8_t* smem, u
       commit(&ctl->kv_empty[sv]);
       if (more) commit(&ctl->kv_empty[sk]);
     }
+    if (kSplit) break;
   }
   // every product issued completes before TMEM and shared memory are given up
   commit(&ctl->teardown);
@@ -634,7 +722,9 @@ __device__ __forceinline__ void issue_products(Ctl* ctl, int t, uint8_t* smem, u
     atomicOr(&uk::g_attn_prompt_fault, UK_FAULT_TEARDOWN);
 }
 
-template <int DP>
+// kSplit: a cluster of a.split CTAs per tile, each with a share of its keys, and
+// one tile per block (no next item).
+template <int DP, bool kSplit>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
     k_attn_prompt(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                   const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ Args a) {
@@ -668,6 +758,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     uk_mbar_init(&ctl->v_landed, 1);
     uk_mbar_init(&ctl->teardown, 2);
     ctl->abort = 0;
+    for (int i = 0; i < 4; ++i) ctl->odd[i] = 0;
     uk_fence_mbar_init();
     uk_tma_prefetch_desc(&tm_q);
     uk_tma_prefetch_desc(&tm_k);
@@ -679,7 +770,21 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   }
   Cursor cursor;
   bool any = false;
-  if (warp == LOAD_WARP) any = find_item(a, blockIdx.x, cursor, &ctl->item[0]);
+  if (warp == LOAD_WARP) {
+    any = find_item(a, kSplit ? blockIdx.x / a.split : blockIdx.x, cursor, &ctl->item[0]);
+    __syncwarp();
+    if (kSplit && lane == 0) {
+      Item& it = ctl->item[0];
+      it.any = any;  // read by every warp at the end, too
+      if (any) {
+        const int rank = (int)(blockIdx.x % a.split), blocks = it.tile[0].blocks();
+        const int from = (int)((int64_t)blocks * rank / a.split), to = (int)((int64_t)blocks * (rank + 1) / a.split);
+        it.first_block = from;
+        it.all_units = it.tile[0].units;
+        it.tile[0].units = to > from ? min(it.all_units, 2 * to) - 2 * from : 0;
+      }
+    }
+  }
   uk_tc_fence_before();
   __syncthreads();
   uk_tc_fence_after();
@@ -691,14 +796,14 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     for (uint32_t item = 0;; ++item) {
       if (!wait_warp(ctl, &ctl->item_full[item & 1u], (item >> 1) & 1u, UK_FAULT_EPILOGUE)) break;
       const Item& it = ctl->item[item & 1u];
-      if (!it.any || !softmax_tile<DP>(a, ctl, it, warp >> 2, tmem, turn, &ends)) break;
+      if (!it.any || !softmax_tile<DP, kSplit>(a, ctl, it, warp >> 2, tmem, ring, turn, &ends) || kSplit) break;
       __syncwarp();
       if (lane == 0) uk_mbar_arrive(&ctl->item_empty[item & 1u]);
     }
   } else {
     uk_regs_down<REGS_OTHERS>();
-    if (warp == LOAD_WARP) load_items<DP>(a, ctl, smem, ring, tm_q, tm_k, tm_v, cursor, any);
-    else if (warp < MMA_WARP + 2) issue_products<DP>(ctl, warp - MMA_WARP, smem, ring, tmem);
+    if (warp == LOAD_WARP) load_items<DP, kSplit>(a, ctl, smem, ring, tm_q, tm_k, tm_v, cursor, any);
+    else if (warp < MMA_WARP + 2) issue_products<DP, kSplit>(ctl, warp - MMA_WARP, smem, ring, tmem);
   }
   __syncwarp();
   uk_tc_fence_before();
@@ -706,6 +811,12 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   if (warp == MMA_WARP) {
     uk_tc_fence_after();
     uk_tmem_dealloc(tmem, 512);
+  }
+  if constexpr (kSplit) {
+    uk_cluster_sync();  // every CTA's sums are there
+    if (warp < 8 && ctl->item[0].any && !ctl->abort) join_shares<DP>(a, ctl, ring);
+    __syncwarp();
+    uk_cluster_sync();  // no CTA leaves while another reads its shared memory
   }
 }
 
@@ -766,13 +877,35 @@ int launch(const Args& a, int64_t items, cudaStream_t st) {
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !attr_done[dev]) {
-    const cudaError_t e =
-        cudaFuncSetAttribute(k_attn_prompt<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Smem<DP>::BYTES);
+    const int bytes = (int)Smem<DP>::BYTES;
+    cudaError_t e = cudaFuncSetAttribute(k_attn_prompt<DP, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(k_attn_prompt<DP, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return uk::fail(UK_ECUDA, "attn_prompt: smem attribute: %s", cudaGetErrorString(e));
     if (dev >= 0 && dev < 64) attr_done[dev] = true;
   }
-  k_attn_prompt<DP><<<(unsigned)items, NUM_THREADS, Smem<DP>::BYTES, st>>>(q, k, v, a);
-  return uk::check_launch("attn_prompt");
+  if (a.split == 1) {
+    k_attn_prompt<DP, false><<<(unsigned)items, NUM_THREADS, Smem<DP>::BYTES, st>>>(q, k, v, a);
+    return uk::check_launch("attn_prompt");
+  }
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr{};
+  cfg.gridDim = dim3((unsigned)(items * a.split), 1, 1);
+  cfg.blockDim = dim3(NUM_THREADS, 1, 1);
+  cfg.dynamicSmemBytes = Smem<DP>::BYTES;
+  cfg.stream = st;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = (unsigned)a.split;
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, k_attn_prompt<DP, true>, q, k, v, a);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return uk::fail(UK_ECUDA, "attn_prompt: %s", cudaGetErrorString(e));
+  }
+  return UK_OK;
 }
 
 }  // namespace
@@ -816,7 +949,7 @@ extern "C" int uk_cuda_attn_prompt_f16(const uint16_t* Q, int64_t q_token_stride
     if (int rc = uk::check_device_ptr(LSE, "LSE")) return rc;
   Args a{Q, K, V, O, q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride,
          o_token_stride, o_head_stride, LSE, cu_q, cu_k, n_seq, heads_q, heads_kv, heads_q / heads_kv, dim, causal,
-         total_q, total_k, scale * LOG2E, 0};
+         total_q, total_k, scale * LOG2E, 0, 2, 1};
   // a zero scale: any factor that no score can raise above rounding does the same
   // and leaves hidden scores at -inf
   if (a.scale2 == 0.f) a.scale2 = 1e-30f;
@@ -832,8 +965,20 @@ extern "C" int uk_cuda_attn_prompt_f16(const uint16_t* Q, int64_t q_token_stride
   if (n_seq <= 1024)
     while ((total_k + UN - 1) / UN >> a.levels) ++a.levels;
   const int64_t seqs = n_seq < total_q ? n_seq : total_q;
-  const int64_t q_blocks = total_q / BM + seqs < total_q ? total_q / BM + seqs : total_q;
-  const int64_t items = (q_blocks * a.group + seqs) / 2 * heads_kv;
+  const int64_t most = (total_q + (BM - 1) * seqs) / BM, q_blocks = most < total_q ? most : total_q;
+  int64_t items = (q_blocks * a.group + seqs) / 2 * heads_kv;
+  // Few tiles: where all of them can run at once, a tile per block instead of a
+  // pair (one alone takes two thirds of a pair's time), and its keys shared by a
+  // cluster of 2, 4 or 8 blocks while the SMs last and every one keeps four blocks
+  // of keys on average.  One B200, 32 heads over 8 of 128: 512 rows 17.9 us in
+  // pairs, 14.6 in single tiles (1024 rows, 256 tiles: 25.2 against 26.8); 200 rows
+  // behind 8000 keys 124 us in pairs, 92 in single tiles, 60 shared by two.
+  const int64_t tiles = q_blocks * a.group * heads_kv;
+  if (tiles <= uk::sm_count()) {
+    a.tiles = 1, items = tiles;
+    const int64_t blocks = total_k / n_seq / BN;
+    while (a.split < 8 && tiles * a.split * 2 <= uk::sm_count() && blocks >= 8 * a.split) a.split *= 2;
+  }
   if (items > 0x7fffffff) return uk::fail(UK_EINVAL, "attn_prompt: %lld tiles exceed the grid", (long long)items);
   return dim > 64 ? launch<128>(a, items, (cudaStream_t)stream) : launch<64>(a, items, (cudaStream_t)stream);
 }
