@@ -288,6 +288,11 @@ PROMPT = [  # heads_kv, group, dim, query lengths, key lengths (None: the same)
     (2, 3, 24, [40, 0, 17, 140], [0, 30, 400, 139]),
     (1, 8, 96, [513], [700]),
     (1, 1, 128, [1] * 40, [i * 7 for i in range(40)]),
+    (2, 20, 64, [14, 3, 200], [400, 3, 260]),
+    (1, 128, 32, [1, 2, 65], [300, 2, 65]),
+    (1, 130, 16, [3, 70], [3, 200]),  # more query heads of a key head than a tile has rows
+    (1, 65, 40, [2, 130], None),
+    (2, 33, 72, [1, 129, 64], [700, 129, 64]),
 ]
 
 

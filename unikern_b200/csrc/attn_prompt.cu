@@ -8,19 +8,22 @@
 // The work is bound by the tensor cores (4 dim flops per visible pair and head)
 // and, nearly as much, by the exponentials (one per pair and head; the MUFU
 // makes 16 per cycle and SM, a 128 x 128 tile's take as long as its two
-// products at dim 128).  One CTA per SM works on two tiles of 128
-// query rows of one key head at a time, so that one tile's products run while
-// the other's softmax does:
-//   warp 9     loads (TMA): both Q tiles, then K and V blocks of 128 keys through
-//              a ring in shared memory;
-//   warp 8     issues tcgen05.mma: S = Q K^T into 128 TMEM columns, O += P V with
-//              P in TMEM;
-//   warps 0-3  softmax of tile 0, a thread per row: reads its S row from TMEM,
-//              writes P (binary16) over it, rescales O when m moves, and at the
-//              end divides by l and stores; warps 4-7 the same for tile 1.
-// TMEM: S/P of tile 0 and 1 at columns 0 and 128, O at 256 and 384.  A tile's next
-// S is issued behind the product that reads its P, and the tensor core runs one
-// thread's products in order, so S arriving also says that O is up to date.
+// products at dim 128); long prompts run into the power limit first (8192 rows,
+// 32 heads over 8 of 128: 1370 MHz).  A tile has 128 rows: the heads of a key
+// head's group, side by side for each of as many tokens as fit (32 for groups of
+// 4), so short sequences fill it too.  A CTA (one per SM) works on two tiles of
+// one key head at a time, so that one tile's products run while the other's
+// softmax does:
+//   warp 10      loads (TMA): both Q tiles, then K and V blocks of 128 keys through
+//                a ring in shared memory; finds the next pair of tiles meanwhile;
+//   warps 8, 9   issue tcgen05.mma, a tile each: S = Q K^T for runs of 64 keys,
+//                O += P V with P in TMEM;
+//   warps 0-3    softmax of tile 0, a thread per row: reads a run of its S row from
+//                TMEM, writes P (binary16) over it, rescales O when m moves, and at
+//                the end divides by l and stores; warps 4-7 the same for tile 1.
+// TMEM: S/P of tile 0 and 1 at columns 0 and 128 (even and odd runs, 64 each), O
+// at 256 and 384.  A run's S is issued behind the product that reads the P in its
+// place, and the tensor core runs one thread's products in order.
 //
 // What lies behind a row's mask: scores are replaced before the maximum, V rows
 // behind the sequence's last key are zeroed in shared memory (a zero weight
@@ -33,6 +36,7 @@
 #include <cudaTypedefs.h>
 
 #include <mutex>
+#include <utility>
 
 #include "kv_cache.cuh"
 
@@ -56,6 +60,9 @@ struct Args {
   int levels;  // of the order of work
   int tiles;   // of an item: 2, or 1 where pairs would leave SMs without work
   int split;   // CTAs (a cluster) that share a tile's keys
+  // a tile is `tokens` query tokens by `heads` query heads of one key head, the
+  // heads of a token side by side; `chunks` tiles make the key head's group
+  int tokens, heads, chunks;
 };
 
 __device__ __forceinline__ float4 row4(const uint16_t* row, int lane, int dim) {
@@ -119,7 +126,7 @@ __device__ __noinline__ void attend_row(const Args& a, int64_t t, int h, int64_t
 }
 
 // ---- what one CTA works on -----------------------------------------------------------
-constexpr int BM = 128, BN = 128;  // query rows of a tile, keys of a block
+constexpr int BM = 128, BN = 128;  // rows of a tile, keys of a block
 constexpr int UN = 64;             // keys of a softmax step (half a block)
 constexpr float GROW = 8.f;        // scores may pass the reference by 2^8 before it moves
 constexpr float SHIFT = 7.f;       // weights are held as 2^7 * 2^(s - m): up to 2^15, binary16 ends at 2^16
@@ -133,11 +140,23 @@ constexpr int MMA_WARP = 8, LOAD_WARP = 10;  // MMA_WARP + t: tile t
 constexpr uint64_t WAIT_NS = 4000000000ull;  // a row computed again may take long
 
 struct Tile {
-  int head;    // query head; -1: no tile
-  int first;   // its first row within the sequence
-  int rows;    // rows it has
+  int head;    // its first query head; -1: no tile
+  int heads;   // query heads it has
+  int first;   // its first token within the sequence
+  int tokens;  // tokens it has
   int units;   // runs of 64 keys that some row of it sees
   __device__ __forceinline__ int blocks() const { return (units + 1) / 2; }
+};
+// row i of a tile: token i / a.heads of it, head i % a.heads
+struct Row {
+  int token, head;
+  bool on;
+  __device__ __forceinline__ Row(const Args& a, const Tile& t, int i) {
+    token = i / a.heads;
+    head = i - token * a.heads;
+    on = token < t.tokens && head < t.heads;
+    token += t.first, head += t.head;
+  }
 };
 struct Item {
   Tile tile[2];
@@ -153,8 +172,8 @@ struct Item {
 // 2^(levels - 1) runs of keys, then of half as many, and so on, at the end the
 // rest (blocks take items as they come free, so the last ones should be short).
 // Within a level: sequences in order; in each the pairs of its tiles, the tiles
-// going from the last query block to the first and through the group's heads,
-// for every key head.  A block's items come in rising order, so the search goes
+// going from the last tokens to the first and through the group's heads, for
+// every key head.  A block's items come in rising order, so the search goes
 // on where the last one ended: 32 sequences at a time, a lane each.
 struct Cursor {
   int level = 0, chunk = 0;
@@ -173,7 +192,7 @@ __device__ bool find_item(const Args& a, int64_t item, Cursor& at, Item* out) {
         q0 = clamp64(__ldg(a.cu_q + b), 0, a.total_q), q1 = clamp64(__ldg(a.cu_q + b + 1), q0, a.total_q);
         k0 = clamp64(__ldg(a.cu_k + b), 0, a.total_k), k1 = clamp64(__ldg(a.cu_k + b + 1), k0, a.total_k);
       }
-      const int n = (int)(q1 - q0), m = (int)(k1 - k0), blocks = (n + BM - 1) / BM;
+      const int n = (int)(q1 - q0), m = (int)(k1 - k0), blocks = (n + a.tokens - 1) / a.tokens;
       // pairs whose first tile sees at least `units` runs of keys
       auto pairs = [&](int units) -> int64_t {
         int64_t tiles = blocks;
@@ -181,12 +200,12 @@ __device__ bool find_item(const Args& a, int64_t item, Cursor& at, Item* out) {
           const int64_t end = (int64_t)(units - 1) * UN;  // its last row sees more keys than that
           if (a.causal) {
             const int64_t x = end - m + n;
-            tiles = x >= n ? 0 : blocks - (x > 0 ? x / BM : 0);
+            tiles = x >= n ? 0 : blocks - (x > 0 ? x / a.tokens : 0);
           } else if (m <= end) {
             tiles = 0;
           }
         }
-        return (tiles * a.group + a.tiles - 1) / a.tiles;
+        return (tiles * a.chunks + a.tiles - 1) / a.tiles;
       };
       const int64_t above = at.level == 0 ? 0 : pairs(1 << (a.levels - at.level));
       const int64_t here = pairs(at.level == a.levels ? 0 : 1 << (a.levels - 1 - at.level)) - above;
@@ -212,13 +231,15 @@ __device__ bool find_item(const Args& a, int64_t item, Cursor& at, Item* out) {
         for (int t = 0; t < 2; ++t) {
           const int64_t e = pair * a.tiles + t;
           Tile& tile = out->tile[t];
-          tile.head = -1, tile.first = 0, tile.rows = 0, tile.units = 0;
-          if (t >= a.tiles || e >= (int64_t)blocks * a.group) continue;
-          tile.head = out->g * a.group + (int)(e % a.group);
-          tile.first = (blocks - 1 - (int)(e / a.group)) * BM;
-          tile.rows = min(BM, n - tile.first);
-          // one past the last key that its last row sees
-          const int64_t end = a.causal ? (int64_t)m - n + tile.first + tile.rows : m;
+          tile.head = -1, tile.heads = 0, tile.first = 0, tile.tokens = 0, tile.units = 0;
+          if (t >= a.tiles || e >= (int64_t)blocks * a.chunks) continue;
+          const int chunk = (int)(e % a.chunks);
+          tile.head = out->g * a.group + chunk * a.heads;
+          tile.heads = min(a.heads, a.group - chunk * a.heads);
+          tile.first = (blocks - 1 - (int)(e / a.chunks)) * a.tokens;
+          tile.tokens = min(a.tokens, n - tile.first);
+          // one past the last key that its last token sees
+          const int64_t end = a.causal ? (int64_t)m - n + tile.first + tile.tokens : m;
           tile.units = end <= 0 ? 0 : (int)((end + UN - 1) / UN);
         }
       }
@@ -270,23 +291,24 @@ __device__ __forceinline__ bool wait_warp(Ctl* ctl, uint64_t* bar, uint32_t pari
 // ---- the softmax of a tile ------------------------------------------------------------
 // *turn: runs of 64 keys of this tile's slot that came before, even and odd ones;
 // *ends: items that had any.
-// One past the last key that row i of a tile sees.
-__device__ __forceinline__ int end_of_row(const Args& a, const Item& it, const Tile& tile, int i) {
-  const int64_t end = a.causal ? (int64_t)it.m - it.n + tile.first + 1 + i : it.m;
+// One past the last key that a token of the sequence sees.
+__device__ __forceinline__ int end_of(const Args& a, const Item& it, int token) {
+  const int64_t end = a.causal ? (int64_t)it.m - it.n + 1 + token : it.m;
   return (int)(end < 0 ? 0 : end > it.m ? it.m : end);
 }
 
 // A row with a finite sum that is not finite itself (one warp): it is computed
 // again where one of the keys between its mask and the end of its blocks is not.
 __device__ __noinline__ void look_again(const Args& a, const Item& it, const Tile& tile, int row, int units) {
-  const int lane = threadIdx.x & 31, from = end_of_row(a, it, tile, row), to = min(units * UN, it.m);
+  const Row r(a, tile, row);
+  const int lane = threadIdx.x & 31, from = end_of(a, it, r.token), to = min(units * UN, it.m);
   bool bad = false;
   for (int k = from; k < to && !bad; ++k) {
     const float4 v = row4(a.v + (int64_t)(it.k0 + k) * a.v_token + it.g * a.v_head, lane, a.dim);
     bad = __any_sync(0xffffffffu, !(fabsf(v.x) + fabsf(v.y) + fabsf(v.z) + fabsf(v.w) < INFINITY));
   }
   __syncwarp();  // the row's stores before come before these
-  if (bad) attend_row(a, (int64_t)it.q0 + tile.first + row, tile.head, it.k0, (int64_t)it.k0 + from);
+  if (bad) attend_row(a, (int64_t)it.q0 + r.token, r.head, it.k0, (int64_t)it.k0 + from);
 }
 
 // A shared tile's sums in shared memory: 128 rows of DP floats (16-byte pieces
@@ -311,7 +333,9 @@ __device__ __forceinline__ bool softmax_tile(const Args& a, Ctl* ctl, const Item
   const int i = quad * 32 + lane;  // row of the tile
   const uint32_t lanes = (uint32_t)(quad * 32) << 16;
   const uint32_t s_at = tmem + lanes + t * BN, o_at = tmem + lanes + 256 + t * 128;
-  const int end = end_of_row(a, it, tile, i), clear = end_of_row(a, it, tile, 0);
+  const Row row(a, tile, i);
+  // one past the last key that this row and that the tile's first token see
+  const int end = end_of(a, it, row.token), clear = end_of(a, it, tile.first);
   const uint64_t scale2 = uk_f2(a.scale2, a.scale2);
   const int units = tile.units;
 
@@ -345,7 +369,9 @@ __device__ __forceinline__ bool softmax_tile(const Args& a, Ctl* ctl, const Item
     const float rest = uk_max3_nan(__uint_as_float(s[0][15]), __uint_as_float(s[0][31]),
                                    uk_max3_nan(__uint_as_float(s[1][15]), __uint_as_float(s[1][31]), top[0]));
     const float mt = uk_max3_nan(uk_max3_nan(top[1], top[2], top[3]), rest, rest) * a.scale2;
-    if (__any_sync(0xffffffffu, mt > m + GROW)) {
+    // the rows of the warp move together; ones that stand for nothing have no say
+    // (what they hold is whatever shared memory held)
+    if (__any_sync(0xffffffffu, row.on && mt > m + GROW)) {
       const float m2 = fmaxf(m, mt);
       const float f = m2 == -INFINITY ? 1.f : ex2(m - m2);
       m = m2;
@@ -397,8 +423,8 @@ __device__ __forceinline__ bool softmax_tile(const Args& a, Ctl* ctl, const Item
     if (!step(u, u & 1, turn[0] + turn[1])) return false;
 
   // ---- O / l, the log of the sum
-  const bool mine = i < tile.rows;
-  const int64_t token = (int64_t)it.q0 + tile.first + i;
+  const bool mine = row.on;
+  const int64_t token = (int64_t)it.q0 + row.token;
   if (units > 0) {
     if (!wait_warp(ctl, &ctl->o_full[t], *ends & 1u, UK_FAULT_EPILOGUE)) return false;
     uk_tc_fence_after();
@@ -428,8 +454,10 @@ __device__ __forceinline__ bool softmax_tile(const Args& a, Ctl* ctl, const Item
   // between their rows turns 32 lines touched by every store into 8 (the
   // store path takes a line per cycle: 2000 cycles a tile pair at dim 64).
   const int j4 = lane & 3;
-  uint16_t* out = a.o + ((int64_t)it.q0 + tile.first + (i - j4)) * a.o_token + tile.head * a.o_head + j4 * 8;
-  const int rows = tile.rows - (i - j4);  // of the group's four
+  const uint64_t own = mine ? (uint64_t)(a.o + token * a.o_token + row.head * a.o_head) : 0;
+  uint16_t* out[4];  // of the group's four rows
+#pragma unroll
+  for (int k = 0; k < 4; ++k) out[k] = (uint16_t*)__shfl_sync(0xffffffffu, own, (lane & ~3) + k);
 #pragma unroll
   for (int c = 0; c < DP / 32; ++c) {
     uint32_t w[4][4];
@@ -463,8 +491,8 @@ __device__ __forceinline__ bool softmax_tile(const Args& a, Ctl* ctl, const Item
       }
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      if (k < rows && c * 32 + j4 * 8 < a.dim)
-        *reinterpret_cast<uint4*>(out + k * a.o_token + c * 32) = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
+      if (out[k] != nullptr && c * 32 + j4 * 8 < a.dim)
+        *reinterpret_cast<uint4*>(out[k] + c * 32 + j4 * 8) = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
   }
   if (units > 0) {
     uk_tc_fence_before();
@@ -473,7 +501,7 @@ __device__ __forceinline__ bool softmax_tile(const Args& a, Ctl* ctl, const Item
     ++*ends;
   }
   if (mine && a.lse != nullptr)
-    a.lse[token * a.heads_q + tile.head] = l == 0.f ? -INFINITY : (m - SHIFT + log2f(l)) * LN2;
+    a.lse[token * a.heads_q + row.head] = l == 0.f ? -INFINITY : (m - SHIFT + log2f(l)) * LN2;
 
   // rows that may have met what their mask hides: a finite sum, but not a finite row
   float odd0, odd1;
@@ -497,7 +525,8 @@ __device__ __forceinline__ void join_shares(const Args& a, Ctl* ctl, uint8_t* ri
   const int rank = (int)(blockIdx.x % a.split), rows = BM / a.split;
   for (int x = threadIdx.x; x < rows * (DP / 8); x += 256) {
     const int row = rank * rows + x / (DP / 8), d = x % (DP / 8) * 8;
-    if (row >= tile.rows || d >= a.dim) continue;
+    const Row r(a, tile, row);
+    if (!r.on || d >= a.dim) continue;
     float mm = -INFINITY, l = 0.f, o[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) o[k] = 0.f;
@@ -517,11 +546,11 @@ __device__ __forceinline__ void join_shares(const Args& a, Ctl* ctl, uint8_t* ri
       o[k] *= inv;
       odd |= !(fabsf(o[k]) < INFINITY);
     }
-    const int64_t token = (int64_t)it.q0 + tile.first + row;
-    *reinterpret_cast<uint4*>(a.o + token * a.o_token + tile.head * a.o_head + d) = make_uint4(
+    const int64_t token = (int64_t)it.q0 + r.token;
+    *reinterpret_cast<uint4*>(a.o + token * a.o_token + r.head * a.o_head + d) = make_uint4(
         pack_half(o[0], o[1]), pack_half(o[2], o[3]), pack_half(o[4], o[5]), pack_half(o[6], o[7]));
     if (a.lse != nullptr && d == 0)
-      a.lse[token * a.heads_q + tile.head] = l == 0.f ? -INFINITY : (mm - SHIFT + log2f(l)) * LN2;
+      a.lse[token * a.heads_q + r.head] = l == 0.f ? -INFINITY : (mm - SHIFT + log2f(l)) * LN2;
     if (odd && l - l == 0.f) atomicOr(&ctl->odd[row / 32], 1u << (row % 32));
   }
   asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -565,11 +594,12 @@ __device__ __forceinline__ void load_items(const Args& a, Ctl* ctl, uint8_t* sme
           if (!(ok = wait_warp(ctl, &ctl->q_empty[t], (q_turn[t] & 1u) ^ 1u, UK_FAULT_PRODUCER))) break;
           ++q_turn[t];
           if (lane == 0) {
-            uk_mbar_expect_tx(&ctl->q_full[t], S::TILE);
+            // rows behind the last token's and head's stay as they are in shared memory: nobody reads their sums
+            uk_mbar_expect_tx(&ctl->q_full[t], S::CHUNKS * 128 * a.heads * a.tokens);
 #pragma unroll
             for (int c = 0; c < S::CHUNKS; ++c)
-              uk_tma_load_3d(smem + t * S::TILE + c * S::BOX, &tm_q, &ctl->q_full[t], c * 64, it.q0 + it.tile[t].first,
-                             it.tile[t].head);
+              uk_tma_load_3d(smem + t * S::TILE + c * S::BOX, &tm_q, &ctl->q_full[t], c * 64, it.tile[t].head,
+                             it.q0 + it.tile[t].first);
           }
           __syncwarp();
         }
@@ -847,18 +877,25 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
-// packed rows [tokens][heads][dim] as a (dim, token, head) tensor; boxes of
-// 64 x 128 x 1, columns behind dim and rows behind the last filled with zeros
+// packed rows [tokens][heads][dim] as a (dim, token, head) tensor, boxes of 64 x
+// `tokens` x 1 (K, V), or as (dim, head, token), boxes of 64 x `heads` x `tokens`
+// (Q); columns behind dim and rows behind the last are filled with zeros
 int make_map(CUtensorMap* m, const char* name, const uint16_t* base, int dim, int64_t tokens, int heads,
-             int64_t token_stride, int64_t head_stride) {
+             int64_t token_stride, int64_t head_stride, int box_tokens, int box_heads) {
   auto fn = encode_fn();
   if (!fn) return uk::fail(UK_ECUDA, "attn_prompt: cuTensorMapEncodeTiled is unavailable from the driver");
   // a stride that nothing steps by still has to be one the map accepts
   if (tokens == 1) token_stride = dim;
   if (heads == 1) head_stride = dim;
+  const bool by_head = box_heads > 0;
   cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)tokens, (cuuint64_t)heads};
   cuuint64_t strides[2] = {(cuuint64_t)token_stride * 2, (cuuint64_t)head_stride * 2};
-  cuuint32_t box[3] = {64, 128, 1};
+  cuuint32_t box[3] = {64, (cuuint32_t)box_tokens, 1};
+  if (by_head) {
+    std::swap(dims[1], dims[2]);
+    std::swap(strides[0], strides[1]);
+    box[1] = (cuuint32_t)box_heads, box[2] = (cuuint32_t)box_tokens;
+  }
   cuuint32_t estr[3] = {1, 1, 1};
   const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<uint16_t*>(base), dims, strides, box, estr,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -870,9 +907,9 @@ int make_map(CUtensorMap* m, const char* name, const uint16_t* base, int dim, in
 template <int DP>
 int launch(const Args& a, int64_t items, cudaStream_t st) {
   CUtensorMap q, k, v;
-  if (int rc = make_map(&q, "Q", a.q, a.dim, a.total_q, a.heads_q, a.q_token, a.q_head)) return rc;
-  if (int rc = make_map(&k, "K", a.k, a.dim, a.total_k, a.heads_kv, a.k_token, a.k_head)) return rc;
-  if (int rc = make_map(&v, "V", a.v, a.dim, a.total_k, a.heads_kv, a.v_token, a.v_head)) return rc;
+  if (int rc = make_map(&q, "Q", a.q, a.dim, a.total_q, a.heads_q, a.q_token, a.q_head, a.tokens, a.heads)) return rc;
+  if (int rc = make_map(&k, "K", a.k, a.dim, a.total_k, a.heads_kv, a.k_token, a.k_head, BN, 0)) return rc;
+  if (int rc = make_map(&v, "V", a.v, a.dim, a.total_k, a.heads_kv, a.v_token, a.v_head, BN, 0)) return rc;
   static bool attr_done[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -949,7 +986,7 @@ extern "C" int uk_cuda_attn_prompt_f16(const uint16_t* Q, int64_t q_token_stride
     if (int rc = uk::check_device_ptr(LSE, "LSE")) return rc;
   Args a{Q, K, V, O, q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride,
          o_token_stride, o_head_stride, LSE, cu_q, cu_k, n_seq, heads_q, heads_kv, heads_q / heads_kv, dim, causal,
-         total_q, total_k, scale * LOG2E, 0, 2, 1};
+         total_q, total_k, scale * LOG2E, 0, 2, 1, 0, 0, 0};
   // a zero scale: any factor that no score can raise above rounding does the same
   // and leaves hidden scores at -inf
   if (a.scale2 == 0.f) a.scale2 = 1e-30f;
@@ -965,15 +1002,19 @@ extern "C" int uk_cuda_attn_prompt_f16(const uint16_t* Q, int64_t q_token_stride
   if (n_seq <= 1024)
     while ((total_k + UN - 1) / UN >> a.levels) ++a.levels;
   const int64_t seqs = n_seq < total_q ? n_seq : total_q;
-  const int64_t most = (total_q + (BM - 1) * seqs) / BM, q_blocks = most < total_q ? most : total_q;
-  int64_t items = (q_blocks * a.group + seqs) / 2 * heads_kv;
+  // the heads of a group in as few tiles as hold them, a tile's rows filled up with tokens
+  a.chunks = (a.group + BM - 1) / BM;
+  a.heads = (a.group + a.chunks - 1) / a.chunks;
+  a.tokens = BM / a.heads;
+  const int64_t most = (total_q + (a.tokens - 1) * seqs) / a.tokens, q_blocks = most < total_q ? most : total_q;
+  int64_t items = (q_blocks * a.chunks + seqs) / 2 * heads_kv;
   // Few tiles: where all of them can run at once, a tile per block instead of a
   // pair (one alone takes two thirds of a pair's time), and its keys shared by a
   // cluster of 2, 4 or 8 blocks while the SMs last and every one keeps four blocks
   // of keys on average.  One B200, 32 heads over 8 of 128: 512 rows 17.9 us in
   // pairs, 14.6 in single tiles (1024 rows, 256 tiles: 25.2 against 26.8); 200 rows
   // behind 8000 keys 124 us in pairs, 92 in single tiles, 60 shared by two.
-  const int64_t tiles = q_blocks * a.group * heads_kv;
+  const int64_t tiles = q_blocks * a.chunks * heads_kv;
   if (tiles <= uk::sm_count()) {
     a.tiles = 1, items = tiles;
     const int64_t blocks = total_k / n_seq / BN;
