@@ -99,6 +99,30 @@ def test_append_then_gather(kind, layout, heads, dim, page, past, new):
     assert fault() == 0
 
 
+@pytest.mark.parametrize("kind", ["f16", "e4m3"])
+@pytest.mark.parametrize("dim", [64, 72])
+@pytest.mark.parametrize("shift,pad", [(0, 0), (8, 0), (0, 8), (16, 16), (8, 8)])
+def test_gather_into_any_alignment(kind, dim, shift, pad):
+    """Rows that begin on 32- and on 16-byte boundaries, and what lies between
+    them left as it was."""
+    a = abi()
+    if kind == "e4m3" and dim % 16:
+        dim = 48
+    heads, n = 3, 37
+    pool = Pool(kind, "hnd", heads, dim, 16, [n])
+    outs, flat = [], []
+    for _ in "kv":
+        f = torch.full((shift + n * heads * (dim + pad),), 7.0, dtype=torch.float16, device="cuda")
+        flat.append(f)
+        outs.append(f[shift:].view(n, heads, dim + pad)[:, :, :dim])
+    a.kv_gather(pool.cache, pool.table, i32([0, n]), i32([n]), *outs)
+    assert fault() == 0
+    for i in range(2):
+        assert torch.equal(outs[i].double(), pool.get(i, 0, 0, n))
+        assert (flat[i][:shift] == 7).all()
+        assert (flat[i][shift:].view(n, heads, dim + pad)[:, :, dim:] == 7).all()
+
+
 def test_quantiser_at_its_borders():
     """Maxima at and next to 448 * 2^e, zeros, subnormals, the largest values,
     infinities and NaN, one row each."""

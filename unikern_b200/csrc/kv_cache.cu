@@ -215,7 +215,15 @@ __global__ void __launch_bounds__(THREADS) k_kv_append(Rows in, UkKvView c, cons
   }
 }
 
-template <int GL, bool kQuantise>
+// kWide: rows of whole lanes on 32-byte boundaries, stored by one instruction a
+// lane (4 x 16384 positions out of e4m3: 67.9 us, by two 71.7).
+__device__ __forceinline__ void st32(void* p, const Half16& x) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(x.lo.x), "r"(x.lo.y), "r"(x.lo.z),
+               "r"(x.lo.w), "r"(x.hi.x), "r"(x.hi.y), "r"(x.hi.z), "r"(x.hi.w)
+               : "memory");
+}
+
+template <int GL, bool kQuantise, bool kWide>
 __global__ void __launch_bounds__(THREADS) k_kv_gather(Rows out, UkKvView c, const int32_t* __restrict__ cu,
                                                        const int32_t* __restrict__ lens, int n_seq, int tok,
                                                        UkFastDiv per_token) {
@@ -264,8 +272,12 @@ __global__ void __launch_bounds__(THREADS) k_kv_gather(Rows out, UkKvView c, con
       const int64_t t = t0 + r[u].tok;
       uint16_t* p = (r[u].is_v ? out.v + t * out.v_token + r[u].head * out.v_head
                                : out.k + t * out.k_token + r[u].head * out.k_head) + l * 16;
-      if (mine[u] && lo_on) *reinterpret_cast<uint4*>(p) = x[u].lo;
-      if (mine[u] && hi_on) *reinterpret_cast<uint4*>(p + 8) = x[u].hi;
+      if (kWide) {
+        if (mine[u] && lo_on) st32(p, x[u]);
+      } else {
+        if (mine[u] && lo_on) *reinterpret_cast<uint4*>(p) = x[u].lo;
+        if (mine[u] && hi_on) *reinterpret_cast<uint4*>(p + 8) = x[u].hi;
+      }
     }
   }
 }
@@ -368,15 +380,24 @@ void launch_append(const Rows& rows, const UkKvView& v, const int32_t* cu, const
   }
 }
 
-template <bool kQuantise>
+template <bool kQuantise, bool kWide>
 void launch_gather(const Rows& rows, const UkKvView& v, const int32_t* cu, const int32_t* lens, int n_seq, int tok,
                    unsigned blocks, cudaStream_t st) {
   const UkFastDiv d = UkFastDiv::make(2u * v.heads);
   switch (lanes_for(v.dim)) {
-    case 2: k_kv_gather<2, kQuantise><<<blocks, THREADS, 0, st>>>(rows, v, cu, lens, n_seq, tok, d); break;
-    case 4: k_kv_gather<4, kQuantise><<<blocks, THREADS, 0, st>>>(rows, v, cu, lens, n_seq, tok, d); break;
-    default: k_kv_gather<8, kQuantise><<<blocks, THREADS, 0, st>>>(rows, v, cu, lens, n_seq, tok, d); break;
+    case 2: k_kv_gather<2, kQuantise, kWide><<<blocks, THREADS, 0, st>>>(rows, v, cu, lens, n_seq, tok, d); break;
+    case 4: k_kv_gather<4, kQuantise, kWide><<<blocks, THREADS, 0, st>>>(rows, v, cu, lens, n_seq, tok, d); break;
+    default: k_kv_gather<8, kQuantise, kWide><<<blocks, THREADS, 0, st>>>(rows, v, cu, lens, n_seq, tok, d); break;
   }
+}
+
+// whole lanes of 16 values on 32-byte boundaries
+bool wide_rows(const Rows& r, const UkKvView& v) {
+  auto bad = [&](const uint16_t* p, int64_t token, int64_t head) {
+    return reinterpret_cast<uintptr_t>(p) % 32 != 0 || (r.total > 1 && token % 16 != 0) ||
+           (v.heads > 1 && head % 16 != 0);
+  };
+  return v.dim % 16 == 0 && !bad(r.k, r.k_token, r.k_head) && !bad(r.v, r.v_token, r.v_head);
 }
 
 }  // namespace
@@ -413,9 +434,9 @@ extern "C" int uk_cuda_kv_gather_f16(const uk_kv_cache* cache, const int32_t* bl
                        cache != nullptr ? cache->dim : 0, &view, GATHER_TOK, &tok, &blocks))
     return rc;
   if (blocks == 0) return UK_OK;
-  if (cache->kind == UK_KV_E4M3)
-    launch_gather<true>(rows, view, cu_out, seq_lens, n_seq, tok, (unsigned)blocks, (cudaStream_t)stream);
-  else
-    launch_gather<false>(rows, view, cu_out, seq_lens, n_seq, tok, (unsigned)blocks, (cudaStream_t)stream);
+  const bool wide = wide_rows(rows, view);
+  auto launch = cache->kind == UK_KV_E4M3 ? (wide ? launch_gather<true, true> : launch_gather<true, false>)
+                                          : (wide ? launch_gather<false, true> : launch_gather<false, false>);
+  launch(rows, view, cu_out, seq_lens, n_seq, tok, (unsigned)blocks, (cudaStream_t)stream);
   return uk::check_launch("kv_gather");
 }
