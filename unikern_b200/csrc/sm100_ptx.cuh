@@ -359,11 +359,6 @@ __device__ __forceinline__ float uk_max3_nan(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-__device__ __forceinline__ float uk_min3_nan(float a, float b, float c) {
-  float r;
-  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
 
 // ---- cluster launch control: the blocks of a grid taken over by running ones ---
 // ask for the next block that has not been launched; the answer (16 bytes) lands

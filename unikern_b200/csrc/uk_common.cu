@@ -69,7 +69,7 @@ extern "C" {
 
 const char* uk_cuda_last_error(void) { return uk::g_last_error.c_str(); }
 
-int uk_cuda_abi_version(void) { return 10000; }
+int uk_cuda_abi_version(void) { return 10100; }
 
 int uk_cuda_device_supported(void) {
   int dev = 0, major = 0, minor = 0;
