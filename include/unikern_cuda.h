@@ -320,7 +320,7 @@ int uk_cuda_decode_rmsnorm_gemm_f16(const float* X, const float* gamma, float ep
  *               is within [-24, 15].
  * Any page_size >= 1; dim a multiple of 8 (e4m3: of 16) from 8 to 128; pools
  * 16-byte aligned, strides multiples of 16 bytes; max_pages * page_size below
- * 2^31 - 4096.
+ * 2^31 - 4096; up to 2^24 sequences in a call.
  * Page ids and lengths are device memory and are not trusted: a page id outside
  * the pool or a position beyond max_pages pages is treated as absent (nothing is
  * written there; it reads as zeros; attention does not see it) and sets bit 64
@@ -372,7 +372,8 @@ int uk_cuda_kv_gather_f16(const uk_kv_cache* cache, const int32_t* block_table, 
  *   p < seq_lens[b], g = h / (heads_q / cache->heads);
  * LSE[b][h] = log sum_p exp(scale * Q[b][h] . K[p][g]) (fp32; NULL to leave it
  * out).  A sequence of length zero gives zeros and -inf.  Q, O binary16
- * [n_seq][heads_q][dim], strides in elements (multiples of 8, 16-byte aligned).
+ * [n_seq][heads_q][dim], strides in elements (multiples of 8, 16-byte aligned);
+ * heads_q up to 65535.  O overlaps neither Q nor the cache.
  * Scores, softmax statistics and sums are fp32; the softmax weights enter the
  * value product as binary16, one rounding into O.  A NaN or an infinity among
  * the values seen makes that column's outputs NaN or infinite.
@@ -397,8 +398,9 @@ int uk_cuda_attn_decode_f16(const uint16_t* Q, int64_t q_seq_stride, int64_t q_h
  * LSE [total_q][heads_q] as above, or NULL.  A query that sees no key gives
  * zeros and -inf.  Rows of O and LSE outside cu_q[0] .. cu_q[n_seq] - 1 are left
  * as they were.  cu_q and cu_k are device memory, non-decreasing within
- * [0, total_q] and [0, total_k]; values outside are clamped.  total_k up to
- * 2^27.  fp32 scores, statistics and sums; the softmax weights enter the value
+ * [0, total_q] and [0, total_k]; values outside are clamped.  Up to
+ * 2^24 sequences, 2^31 - 256 query and 2^25 key rows, 65535 query heads.  O does
+ * not overlap Q, K or V.  fp32 scores, statistics and sums; the softmax weights enter the value
  * product as binary16.  A negative scale runs row by row on CUDA cores.
  * Deterministic. */
 int uk_cuda_attn_prompt_f16(const uint16_t* Q, int64_t q_token_stride, int64_t q_head_stride, const uint16_t* K,
@@ -476,7 +478,8 @@ int uk_cuda_peer_barrier(unsigned* const* flag_list, int n, int rank, unsigned e
  * kernel of this library expired since the last call, otherwise a bit mask
  * (1 producer, 2 MMA issuer, 4 epilogue, 8 teardown, 16 self-test, 32 peer
  * wait; and 64, not a wait: a page id or a position outside the pool or the
- * block table was skipped by a cache or attention call).  Synchronises with the device and clears the word.  A kernel whose
+ * block table was skipped by a cache or attention call).  Synchronises with
+ * the device and clears the word.  A kernel whose
  * wait expires unwinds and leaves its outputs undefined instead of hanging.
  * No reference counterpart (the reference has no device-side waits). */
 unsigned uk_cuda_pipeline_fault(void);

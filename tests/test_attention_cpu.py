@@ -60,13 +60,28 @@ def test_bad_caches(call, kw):
     lambda c: decode(None), lambda c: decode(c, heads_q=3), lambda c: decode(c, heads_q=0),
     lambda c: decode(c, n_seq=-1), lambda c: decode(c, scale=float("inf")), lambda c: decode(c, scale=float("nan")),
     lambda c: decode(c, max_pages=1), lambda c: decode(c),
-    lambda c: prompt(n_seq=-1), lambda c: prompt(tq=-1), lambda c: prompt(tk=1 << 33), lambda c: prompt(tk=(1 << 27) + 1), lambda c: prompt(hq=3),
+    lambda c: prompt(n_seq=-1), lambda c: prompt(tq=-1), lambda c: prompt(tk=1 << 33),
+    lambda c: prompt(tk=(1 << 27) + 1), lambda c: prompt(hq=3),
     lambda c: prompt(hk=0), lambda c: prompt(dim=12), lambda c: prompt(dim=256), lambda c: prompt(scale=float("nan")),
     lambda c: prompt(),
 ])
 def test_bad_arguments(f):
     assert f(cache(token_stride=128, head_stride=64)) == 2
     assert abi.lib().uk_cuda_last_error()
+
+
+@pytest.mark.parametrize("f,said", [
+    # limits of the kernels' 32-bit numbers and bounded waits
+    (lambda c: append(c, n_seq=(1 << 24) + 1), "n_seq"), (lambda c: gather(c, n_seq=(1 << 24) + 1), "n_seq"),
+    (lambda c: decode(c, n_seq=(1 << 24) + 1), "n_seq"), (lambda c: prompt(n_seq=(1 << 24) + 1), "n_seq"),
+    (lambda c: decode(c, heads_q=65536), "heads_q"), (lambda c: prompt(hq=65536), "heads"),
+    (lambda c: prompt(tq=(1 << 31) - 255), "total_q"), (lambda c: prompt(tk=(1 << 25) + 1), "total_k"),
+    # finite, but not times log2 e
+    (lambda c: decode(c, scale=3e38), "scale"), (lambda c: prompt(scale=-3e38), "scale"),
+])
+def test_limits(f, said):
+    assert f(cache(token_stride=128, head_stride=64)) == 2
+    assert said in abi.lib().uk_cuda_last_error().decode()
 
 
 def test_nothing_to_do():

@@ -18,7 +18,6 @@ _PATH = Path(os.environ.get("UNIKERN_CUDA_LIB") or Path(__file__).resolve().pare
 vp, i64, i32, f32, sz = C.c_void_p, C.c_int64, C.c_int, C.c_float, C.c_size_t
 
 
-
 class KvCacheStruct(C.Structure):
     """uk_kv_cache."""
     _fields_ = [("k", vp), ("v", vp), ("k_exp", vp), ("v_exp", vp), ("page_stride", i64), ("token_stride", i64),

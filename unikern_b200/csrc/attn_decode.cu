@@ -14,9 +14,9 @@
 //   tail of long sequences, no empty CTAs.  A run that covers a pair whole
 //   writes O; a pair cut by a run's end leaves (m, l, o) in the workspace, at
 //   most two per CTA (the pair that entered its run, the pair that leaves it).
-// * k_attn_join_few / _many: for each pair that left a run, the sum of its parts in the
-//   order of the CTAs (deterministic); launched programmatically behind the
-//   first.
+// * k_attn_join_few / _many: for each pair that left a run, the sum of its parts
+//   in the order of the CTAs (deterministic); launched programmatically behind
+//   the first.
 //
 // Within a CTA each of 4 warps takes its own 16 or 32 positions of a tile and
 // never waits for another: rows go from global memory straight into the
@@ -403,7 +403,8 @@ __global__ void __launch_bounds__(THREADS, NH == 1 ? 3 : 2) k_attn_decode(Args a
               for (int k = 0; k < S::VC; ++k) {
                 if (S::VB == 16) {
                   const uint4 v = ldg16(vp + k * 128, true);
-                  vr[n][i][k][0] = v.x, vr[n][i][k][1] = v.y, vr[n][i][k][S::VW - 2] = v.z, vr[n][i][k][S::VW - 1] = v.w;
+                  vr[n][i][k][0] = v.x, vr[n][i][k][1] = v.y;
+                  vr[n][i][k][S::VW - 2] = v.z, vr[n][i][k][S::VW - 1] = v.w;
                 } else {
                   const uint2 v = ldg8(vp + k * 128, true);
                   vr[n][i][k][0] = v.x, vr[n][i][k][1] = v.y;
@@ -559,7 +560,8 @@ __global__ void __launch_bounds__(THREADS, NH == 1 ? 3 : 2) k_attn_decode(Args a
       uint32_t pf[NT][NH][2];
 #pragma unroll
       for (int w = 0; w < NH; ++w) {
-        const float z0 = m[w][0] == -INFINITY ? 0.f : m[w][0] - SHIFT, z1 = m[w][1] == -INFINITY ? 0.f : m[w][1] - SHIFT;
+        const float z0 = m[w][0] == -INFINITY ? 0.f : m[w][0] - SHIFT;
+        const float z1 = m[w][1] == -INFINITY ? 0.f : m[w][1] - SHIFT;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -950,15 +952,18 @@ extern "C" int uk_cuda_attn_decode_f16(const uint16_t* Q, int64_t q_seq_stride, 
                                        int max_pages, const int32_t* seq_lens, int n_seq, int heads_q, float scale,
                                        uint16_t* O, int64_t o_seq_stride, int64_t o_head_stride, float* LSE,
                                        void* workspace, size_t workspace_bytes, void* stream) {
-  if (n_seq < 0 || heads_q < 1) return uk::fail(UK_EINVAL, "attn_decode: n_seq %d, heads_q %d", n_seq, heads_q);
-  if (!(scale - scale == 0.f)) return uk::fail(UK_EINVAL, "attn_decode: the scale is not finite");
+  if (n_seq < 0 || n_seq > uk::MAX_SEQS || heads_q < 1 || heads_q > 65535)
+    return uk::fail(UK_EINVAL, "attn_decode: n_seq %d (at most 2^24), heads_q %d (at most 65535)", n_seq, heads_q);
+  const float scale2 = scale * LOG2E;
+  if (!(scale2 - scale2 == 0.f)) return uk::fail(UK_EINVAL, "attn_decode: the scale is not finite");
   UkKvView c;
   if (int rc = uk::kv_view(cache, block_table, table_stride, n_seq, max_pages, "attn_decode", &c)) return rc;
   if (heads_q % cache->heads != 0)
     return uk::fail(UK_EINVAL, "attn_decode: %d query heads do not divide over %d key heads", heads_q, cache->heads);
   if (n_seq == 0) return UK_OK;
   if (int rc = uk::check_rows("attn_decode", "Q", Q, n_seq, heads_q, q_seq_stride, q_head_stride, 0)) return rc;
-  if (int rc = uk::check_rows("attn_decode", "O", O, n_seq, heads_q, o_seq_stride, o_head_stride, cache->dim)) return rc;
+  if (int rc = uk::check_rows("attn_decode", "O", O, n_seq, heads_q, o_seq_stride, o_head_stride, cache->dim))
+    return rc;
   if (int rc = uk::check_device_ptr(seq_lens, "seq_lens")) return rc;
   if (LSE != nullptr)
     if (int rc = uk::check_device_ptr(LSE, "LSE")) return rc;
@@ -966,9 +971,10 @@ extern "C" int uk_cuda_attn_decode_f16(const uint16_t* Q, int64_t q_seq_stride, 
   const int group = heads_q / cache->heads, nh = heads_nh(group), ctas = grid_ctas(nh), dp = padded_dim(cache->dim);
   const size_t need = workspace_bytes_for(ctas, dp, nh);
   if (workspace_bytes < need || !uk::aligned16(workspace))
-    return uk::fail(UK_EINVAL, "attn_decode: workspace of %zu bytes, %zu wanted, 16-byte aligned", workspace_bytes, need);
+    return uk::fail(UK_EINVAL, "attn_decode: workspace of %zu bytes, %zu wanted, 16-byte aligned", workspace_bytes,
+                    need);
   Args a{Q, q_seq_stride, q_head_stride, O, o_seq_stride, o_head_stride, LSE, seq_lens, n_seq, heads_q, group,
-         (group + 8 * nh - 1) / (8 * nh), scale * LOG2E, nullptr, (int4*)workspace, 0, 0};
+         (group + 8 * nh - 1) / (8 * nh), scale2, nullptr, (int4*)workspace, 0, 0};
   a.by_pair = (int64_t)n_seq * cache->heads * a.chunks <= ctas;
   // rows cross lanes as 32-bit multiples of the strides' common power of two
   int64_t strides = 4096;

@@ -68,7 +68,8 @@ struct Args {
 __device__ __forceinline__ float4 row4(const uint16_t* row, int lane, int dim) {
   if (lane * 4 >= dim) return make_float4(0.f, 0.f, 0.f, 0.f);
   const uint2 w = __ldg(reinterpret_cast<const uint2*>(row) + lane);
-  const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w.x)), y = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
+  const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w.x));
+  const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
   return make_float4(x.x, x.y, y.x, y.y);
 }
 
@@ -137,7 +138,7 @@ constexpr int NUM_THREADS = 384;
 constexpr int REGS_LAUNCH = 168, REGS_SOFTMAX = 216, REGS_OTHERS = 72;
 static_assert(2 * REGS_SOFTMAX + REGS_OTHERS <= 3 * REGS_LAUNCH, "registers of the block");
 constexpr int MMA_WARP = 8, LOAD_WARP = 10;  // MMA_WARP + t: tile t
-constexpr uint64_t WAIT_NS = 4000000000ull;  // a row computed again may take long
+constexpr uint64_t WAIT_NS = 30000000000ull;  // 30 s: rows computed again may take long
 
 struct Tile {
   int head;    // its first query head; -1: no tile
@@ -443,7 +444,8 @@ __device__ __forceinline__ bool softmax_tile(const Args& a, Ctl* ctl, const Item
       }
 #pragma unroll
       for (int k = 0; k < 8; ++k)
-        *reinterpret_cast<uint4*>(sh.piece(i, c * 8 + k)) = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+        *reinterpret_cast<uint4*>(sh.piece(i, c * 8 + k)) =
+            make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
     }
     return true;
   }
@@ -560,8 +562,9 @@ __device__ __forceinline__ void join_shares(const Args& a, Ctl* ctl, uint8_t* ri
 
 // ---- items and loads, one warp ---------------------------------------------------------
 template <int DP, bool kSplit>
-__device__ __forceinline__ void load_items(const Args& a, Ctl* ctl, uint8_t* smem, uint8_t* ring, const CUtensorMap& tm_q,
-                                           const CUtensorMap& tm_k, const CUtensorMap& tm_v, Cursor cursor, bool any) {
+__device__ __forceinline__ void load_items(const Args& a, Ctl* ctl, uint8_t* smem, uint8_t* ring,
+                                           const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v,
+                                           Cursor cursor, bool any) {
   using S = Smem<DP>;
   volatile int* abort = &ctl->abort;
   const int lane = threadIdx.x & 31;
@@ -620,7 +623,8 @@ __device__ __forceinline__ void load_items(const Args& a, Ctl* ctl, uint8_t* sme
       ++n;
       if (fix) {
         // rows behind the sequence's last key hold whatever is there, and their weight is zero
-        if (!__all_sync(0xffffffffu, uk_mbar_wait(bar, fixed & 1u, nullptr, WAIT_NS))) raise_fault(ctl, UK_FAULT_PRODUCER);
+        if (!__all_sync(0xffffffffu, uk_mbar_wait(bar, fixed & 1u, nullptr, WAIT_NS)))
+          raise_fault(ctl, UK_FAULT_PRODUCER);
         ++fixed;
         const int valid = it.m - at;
 #pragma unroll
@@ -964,21 +968,26 @@ extern "C" int uk_cuda_attn_prompt_f16(const uint16_t* Q, int64_t q_token_stride
                                        int64_t total_k, int heads_q, int heads_kv, int dim, float scale, int causal,
                                        uint16_t* O, int64_t o_token_stride, int64_t o_head_stride, float* LSE,
                                        void* stream) {
-  // 2^27 keys: a tile's pass over them stays well within the kernel's bounded waits
-  if (n_seq < 0 || total_q < 0 || total_k < 0 || total_q > 0x7fffffff || total_k > (1 << 27))
-    return uk::fail(UK_EINVAL, "attn_prompt: n_seq %d, total_q %lld, total_k %lld", n_seq, (long long)total_q,
-                    (long long)total_k);
+  // 2^25 keys: a tile's pass over them (0.4 s), and a warp's over each of its 32 rows
+  // when all have to be computed again (5 s), stay well within the kernel's bounded
+  // waits; queries: a tile's row numbers stay within 31 bits
+  if (n_seq < 0 || n_seq > uk::MAX_SEQS || total_q < 0 || total_k < 0 || total_q > 0x7fffff00 || total_k > (1 << 25))
+    return uk::fail(UK_EINVAL, "attn_prompt: n_seq %d (at most 2^24), total_q %lld (2^31 - 256), total_k %lld (2^25)",
+                    n_seq, (long long)total_q, (long long)total_k);
   if (heads_kv < 1 || heads_q < 1 || heads_q > 65535 || heads_q % heads_kv != 0)
     return uk::fail(UK_EINVAL, "attn_prompt: %d query heads do not divide over %d key heads", heads_q, heads_kv);
   if (dim < 8 || dim > 128 || dim % 8 != 0)
     return uk::fail(UK_EINVAL, "attn_prompt: dim %d must be a multiple of 8 from 8 to 128", dim);
-  if (!(scale - scale == 0.f)) return uk::fail(UK_EINVAL, "attn_prompt: the scale is not finite");
+  const float scale2 = scale * LOG2E;
+  if (!(scale2 - scale2 == 0.f)) return uk::fail(UK_EINVAL, "attn_prompt: the scale is not finite");
   if (total_q == 0 || n_seq == 0) return UK_OK;
   if (int rc = uk::check_rows("attn_prompt", "Q", Q, total_q, heads_q, q_token_stride, q_head_stride, dim)) return rc;
   if (int rc = uk::check_rows("attn_prompt", "O", O, total_q, heads_q, o_token_stride, o_head_stride, dim)) return rc;
   if (total_k > 0) {
-    if (int rc = uk::check_rows("attn_prompt", "K", K, total_k, heads_kv, k_token_stride, k_head_stride, dim)) return rc;
-    if (int rc = uk::check_rows("attn_prompt", "V", V, total_k, heads_kv, v_token_stride, v_head_stride, dim)) return rc;
+    if (int rc = uk::check_rows("attn_prompt", "K", K, total_k, heads_kv, k_token_stride, k_head_stride, dim))
+      return rc;
+    if (int rc = uk::check_rows("attn_prompt", "V", V, total_k, heads_kv, v_token_stride, v_head_stride, dim))
+      return rc;
   }
   if (int rc = uk::check_device_ptr(cu_q, "cu_q")) return rc;
   if (int rc = uk::check_device_ptr(cu_k, "cu_k")) return rc;
@@ -986,7 +995,7 @@ extern "C" int uk_cuda_attn_prompt_f16(const uint16_t* Q, int64_t q_token_stride
     if (int rc = uk::check_device_ptr(LSE, "LSE")) return rc;
   Args a{Q, K, V, O, q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride,
          o_token_stride, o_head_stride, LSE, cu_q, cu_k, n_seq, heads_q, heads_kv, heads_q / heads_kv, dim, causal,
-         total_q, total_k, scale * LOG2E, 0, 2, 1, 0, 0, 0};
+         total_q, total_k, scale2, 0, 2, 1, 0, 0, 0};
   // a zero scale: any factor that no score can raise above rounding does the same
   // and leaves hidden scores at -inf
   if (a.scale2 == 0.f) a.scale2 = 1e-30f;
@@ -996,7 +1005,6 @@ extern "C" int uk_cuda_attn_prompt_f16(const uint16_t* Q, int64_t q_token_stride
     k_attn_prompt_rows<<<(unsigned)blocks, 256, 0, (cudaStream_t)stream>>>(a);
     return uk::check_launch("attn_prompt");
   }
-  // at most this many query blocks and pairs of tiles, whatever the lengths are
   // the order of work: a level per power of two of the keys a tile can see; with
   // many sequences every level is a long search, and the order matters less
   if (n_seq <= 1024)
@@ -1006,6 +1014,7 @@ extern "C" int uk_cuda_attn_prompt_f16(const uint16_t* Q, int64_t q_token_stride
   a.chunks = (a.group + BM - 1) / BM;
   a.heads = (a.group + a.chunks - 1) / a.chunks;
   a.tokens = BM / a.heads;
+  // at most this many query blocks and pairs of tiles, whatever the lengths are
   const int64_t most = (total_q + (a.tokens - 1) * seqs) / a.tokens, q_blocks = most < total_q ? most : total_q;
   int64_t items = (q_blocks * a.chunks + seqs) / 2 * heads_kv;
   // Few tiles: where all of them can run at once, a tile per block instead of a

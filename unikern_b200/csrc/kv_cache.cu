@@ -218,8 +218,8 @@ __global__ void __launch_bounds__(THREADS) k_kv_append(Rows in, UkKvView c, cons
 // kWide: rows of whole lanes on 32-byte boundaries, stored by one instruction a
 // lane (4 x 16384 positions out of e4m3: 67.9 us, by two 71.7).
 __device__ __forceinline__ void st32(void* p, const Half16& x) {
-  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(x.lo.x), "r"(x.lo.y), "r"(x.lo.z),
-               "r"(x.lo.w), "r"(x.hi.x), "r"(x.hi.y), "r"(x.hi.z), "r"(x.hi.w)
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(x.lo.x), "r"(x.lo.y),
+               "r"(x.lo.z), "r"(x.lo.w), "r"(x.hi.x), "r"(x.hi.y), "r"(x.hi.z), "r"(x.hi.w)
                : "memory");
 }
 
@@ -355,11 +355,14 @@ int prepare(const char* what, Rows* rows, const uk_kv_cache* cache, const int32_
             int most, int* tok, int64_t* blocks) {
   *blocks = 0;
   if (rows->total < 0 || n_seq < 0) return uk::fail(UK_EINVAL, "%s: negative total or n_seq", what);
-  if (rows->total > 0x7fffffff) return uk::fail(UK_EINVAL, "%s: total %lld exceeds 31 bits", what, (long long)rows->total);
+  if (rows->total > 0x7fffffff || n_seq > uk::MAX_SEQS)
+    return uk::fail(UK_EINVAL, "%s: total %lld (at most 2^31 - 1) or n_seq %d (at most 2^24)", what,
+                    (long long)rows->total, n_seq);
   if (int rc = uk::kv_view(cache, table, table_stride, n_seq, max_pages, what, view)) return rc;
   if (rows->total == 0 || n_seq == 0) return UK_OK;
-  if (int rc = uk::check_rows(what, "K", rows->k, rows->total, cache->heads, rows->k_token, rows->k_head, least)) return rc;
-  if (int rc = uk::check_rows(what, "V", rows->v, rows->total, cache->heads, rows->v_token, rows->v_head, least)) return rc;
+  const int heads = cache->heads;
+  if (int rc = uk::check_rows(what, "K", rows->k, rows->total, heads, rows->k_token, rows->k_head, least)) return rc;
+  if (int rc = uk::check_rows(what, "V", rows->v, rows->total, heads, rows->v_token, rows->v_head, least)) return rc;
   if (int rc = uk::check_device_ptr(cu, "cu_seqlens")) return rc;
   if (int rc = uk::check_device_ptr(lens, "seq_lens")) return rc;
   // as many tokens to a block as still give every SM four blocks

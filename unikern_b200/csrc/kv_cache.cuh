@@ -125,6 +125,9 @@ __device__ __forceinline__ uint32_t uk_half2_of(float x) {
 __device__ __forceinline__ float uk_exp_scale(uint32_t e) { return __uint_as_float(e == 0 ? 0x00400000u : e << 23); }
 
 namespace uk {
+// sequences of one call: indexes of 32 and blocks of 128 of them stay within 31
+// bits, and a kernel's pass over their lengths well within its bounded waits
+constexpr int MAX_SEQS = 1 << 24;
 // host checks of a cache and its block table (kv_cache.cu)
 int kv_view(const uk_kv_cache* cache, const int32_t* table, int64_t table_stride, int n_seq, int max_pages,
             const char* what, UkKvView* out);
