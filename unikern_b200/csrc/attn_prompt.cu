@@ -63,6 +63,7 @@ struct Args {
   // a tile is `tokens` query tokens by `heads` query heads of one key head, the
   // heads of a token side by side; `chunks` tiles make the key head's group
   int tokens, heads, chunks;
+  UkFastDiv by_tokens, by_heads, by_chunks, by_kv;  // by tokens, heads, chunks and heads_kv
 };
 
 __device__ __forceinline__ float4 row4(const uint16_t* row, int lane, int dim) {
@@ -153,7 +154,7 @@ struct Row {
   int token, head;
   bool on;
   __device__ __forceinline__ Row(const Args& a, const Tile& t, int i) {
-    token = i / a.heads;
+    token = (int)a.by_heads.div((uint32_t)i);
     head = i - token * a.heads;
     on = token < t.tokens && head < t.heads;
     token += t.first, head += t.head;
@@ -175,11 +176,24 @@ struct Item {
 // Within a level: sequences in order; in each the pairs of its tiles, the tiles
 // going from the last tokens to the first and through the group's heads, for
 // every key head.  A block's items come in rising order, so the search goes
-// on where the last one ended: 32 sequences at a time, a lane each.
+// on where the last one ended: 32 sequences at a time, a lane each.  (By the
+// machine's long division a step of it took 2 us: 80 prompts of 84 rows, 21 heads
+// over 7 of 64, 82 us.)
 struct Cursor {
   int level = 0, chunk = 0;
   int64_t before = 0;  // items before this level's chunk
 };
+
+// One warp: the first level that has items, from the longest sequence.
+__device__ int first_level(const Args& a) {
+  int most = 0;
+  for (int b = threadIdx.x & 31; b < a.n_seq; b += 32) {
+    const int64_t k0 = clamp64(__ldg(a.cu_k + b), 0, a.total_k), k1 = clamp64(__ldg(a.cu_k + b + 1), k0, a.total_k);
+    most = max(most, (int)(k1 - k0));
+  }
+  most = (__reduce_max_sync(0xffffffffu, most) + UN - 1) / UN;
+  return a.levels - (32 - __clz(most));
+}
 
 // One warp: item i, or false behind the list's end.
 __device__ bool find_item(const Args& a, int64_t item, Cursor& at, Item* out) {
@@ -193,7 +207,7 @@ __device__ bool find_item(const Args& a, int64_t item, Cursor& at, Item* out) {
         q0 = clamp64(__ldg(a.cu_q + b), 0, a.total_q), q1 = clamp64(__ldg(a.cu_q + b + 1), q0, a.total_q);
         k0 = clamp64(__ldg(a.cu_k + b), 0, a.total_k), k1 = clamp64(__ldg(a.cu_k + b + 1), k0, a.total_k);
       }
-      const int n = (int)(q1 - q0), m = (int)(k1 - k0), blocks = (n + a.tokens - 1) / a.tokens;
+      const int n = (int)(q1 - q0), m = (int)(k1 - k0), blocks = (int)a.by_tokens.div((uint32_t)(n + a.tokens - 1));
       // pairs whose first tile sees at least `units` runs of keys
       auto pairs = [&](int units) -> int64_t {
         int64_t tiles = blocks;
@@ -201,12 +215,12 @@ __device__ bool find_item(const Args& a, int64_t item, Cursor& at, Item* out) {
           const int64_t end = (int64_t)(units - 1) * UN;  // its last row sees more keys than that
           if (a.causal) {
             const int64_t x = end - m + n;
-            tiles = x >= n ? 0 : blocks - (x > 0 ? x / a.tokens : 0);
+            tiles = x >= n ? 0 : blocks - (x > 0 ? (int)a.by_tokens.div((uint32_t)x) : 0);
           } else if (m <= end) {
             tiles = 0;
           }
         }
-        return (tiles * a.chunks + a.tiles - 1) / a.tiles;
+        return (tiles * a.chunks + a.tiles - 1) >> (a.tiles - 1);  // by 1 or 2
       };
       const int64_t above = at.level == 0 ? 0 : pairs(1 << (a.levels - at.level));
       const int64_t here = pairs(at.level == a.levels ? 0 : 1 << (a.levels - 1 - at.level)) - above;
@@ -224,8 +238,9 @@ __device__ bool find_item(const Args& a, int64_t item, Cursor& at, Item* out) {
       }
       const int64_t x = item - at.before - (incl - mine);
       if (x >= 0 && x < mine) {
-        const int64_t pair = above + x / a.heads_kv;
-        out->g = (int)(x % a.heads_kv);
+        const int per_head = (int)a.by_kv.div((uint32_t)x);  // items are fewer than 2^31
+        const int64_t pair = above + per_head;
+        out->g = (int)x - per_head * a.heads_kv;
         out->q0 = (int)q0, out->k0 = (int)k0, out->n = n, out->m = m;
         out->first_block = 0;
 #pragma unroll
@@ -234,10 +249,10 @@ __device__ bool find_item(const Args& a, int64_t item, Cursor& at, Item* out) {
           Tile& tile = out->tile[t];
           tile.head = -1, tile.heads = 0, tile.first = 0, tile.tokens = 0, tile.units = 0;
           if (t >= a.tiles || e >= (int64_t)blocks * a.chunks) continue;
-          const int chunk = (int)(e % a.chunks);
+          const int at_block = (int)a.by_chunks.div((uint32_t)e), chunk = (int)e - at_block * a.chunks;
           tile.head = out->g * a.group + chunk * a.heads;
           tile.heads = min(a.heads, a.group - chunk * a.heads);
-          tile.first = (blocks - 1 - (int)(e / a.chunks)) * a.tokens;
+          tile.first = (blocks - 1 - at_block) * a.tokens;
           tile.tokens = min(a.tokens, n - tile.first);
           // one past the last key that its last token sees
           const int64_t end = a.causal ? (int64_t)m - n + tile.first + tile.tokens : m;
@@ -805,6 +820,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   Cursor cursor;
   bool any = false;
   if (warp == LOAD_WARP) {
+    if (a.levels > 0) cursor.level = first_level(a);
     any = find_item(a, kSplit ? blockIdx.x / a.split : blockIdx.x, cursor, &ctl->item[0]);
     __syncwarp();
     if (kSplit && lane == 0) {
@@ -995,7 +1011,7 @@ extern "C" int uk_cuda_attn_prompt_f16(const uint16_t* Q, int64_t q_token_stride
     if (int rc = uk::check_device_ptr(LSE, "LSE")) return rc;
   Args a{Q, K, V, O, q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride,
          o_token_stride, o_head_stride, LSE, cu_q, cu_k, n_seq, heads_q, heads_kv, heads_q / heads_kv, dim, causal,
-         total_q, total_k, scale2, 0, 2, 1, 0, 0, 0};
+         total_q, total_k, scale2, 0, 2, 1, 0, 0, 0, {}, {}, {}, {}};
   // a zero scale: any factor that no score can raise above rounding does the same
   // and leaves hidden scores at -inf
   if (a.scale2 == 0.f) a.scale2 = 1e-30f;
@@ -1014,6 +1030,8 @@ extern "C" int uk_cuda_attn_prompt_f16(const uint16_t* Q, int64_t q_token_stride
   a.chunks = (a.group + BM - 1) / BM;
   a.heads = (a.group + a.chunks - 1) / a.chunks;
   a.tokens = BM / a.heads;
+  a.by_tokens = UkFastDiv::make(a.tokens), a.by_heads = UkFastDiv::make(a.heads);
+  a.by_chunks = UkFastDiv::make(a.chunks), a.by_kv = UkFastDiv::make(heads_kv);
   // at most this many query blocks and pairs of tiles, whatever the lengths are
   const int64_t most = (total_q + (a.tokens - 1) * seqs) / a.tokens, q_blocks = most < total_q ? most : total_q;
   int64_t items = (q_blocks * a.chunks + seqs) / 2 * heads_kv;
@@ -1029,6 +1047,7 @@ extern "C" int uk_cuda_attn_prompt_f16(const uint16_t* Q, int64_t q_token_stride
     const int64_t blocks = total_k / n_seq / BN;
     while (a.split < 8 && tiles * a.split * 2 <= uk::sm_count() && blocks >= 8 * a.split) a.split *= 2;
   }
-  if (items > 0x7fffffff) return uk::fail(UK_EINVAL, "attn_prompt: %lld tiles exceed the grid", (long long)items);
+  // no fewer than items
+  if (tiles > 0x7fffffff) return uk::fail(UK_EINVAL, "attn_prompt: %lld tiles exceed the grid", (long long)tiles);
   return dim > 64 ? launch<128>(a, items, (cudaStream_t)stream) : launch<64>(a, items, (cudaStream_t)stream);
 }
