@@ -181,7 +181,7 @@ struct Item {
 // over 7 of 64, 82 us.)
 struct Cursor {
   int level = 0, chunk = 0;
-  int64_t before = 0;  // items before this level's chunk
+  uint32_t before = 0;  // items before this level's chunk; items are fewer than 2^31
 };
 
 // One warp: the first level that has items, from the longest sequence.
@@ -196,21 +196,22 @@ __device__ int first_level(const Args& a) {
 }
 
 // One warp: item i, or false behind the list's end.
-__device__ bool find_item(const Args& a, int64_t item, Cursor& at, Item* out) {
+__device__ bool find_item(const Args& a, uint32_t item, Cursor& at, Item* out) {
   const int lane = threadIdx.x & 31;
   if (item < at.before) at = Cursor{};
   for (; at.level <= a.levels; ++at.level, at.chunk = 0) {
     for (; at.chunk * 32 < a.n_seq; ++at.chunk) {
       const int b = at.chunk * 32 + lane;
-      int64_t q0 = 0, q1 = 0, k0 = 0, k1 = 0;
+      int q0 = 0, q1 = 0, k0 = 0, k1 = 0;
       if (b < a.n_seq) {
-        q0 = clamp64(__ldg(a.cu_q + b), 0, a.total_q), q1 = clamp64(__ldg(a.cu_q + b + 1), q0, a.total_q);
-        k0 = clamp64(__ldg(a.cu_k + b), 0, a.total_k), k1 = clamp64(__ldg(a.cu_k + b + 1), k0, a.total_k);
+        const int most_q = (int)a.total_q, most_k = (int)a.total_k;
+        q0 = min(max(__ldg(a.cu_q + b), 0), most_q), q1 = min(max(__ldg(a.cu_q + b + 1), q0), most_q);
+        k0 = min(max(__ldg(a.cu_k + b), 0), most_k), k1 = min(max(__ldg(a.cu_k + b + 1), k0), most_k);
       }
-      const int n = (int)(q1 - q0), m = (int)(k1 - k0), blocks = (int)a.by_tokens.div((uint32_t)(n + a.tokens - 1));
+      const int n = q1 - q0, m = k1 - k0, blocks = (int)a.by_tokens.div((uint32_t)(n + a.tokens - 1));
       // pairs whose first tile sees at least `units` runs of keys
-      auto pairs = [&](int units) -> int64_t {
-        int64_t tiles = blocks;
+      auto pairs = [&](int units) -> uint32_t {
+        uint32_t tiles = blocks;
         if (units > 0) {
           const int64_t end = (int64_t)(units - 1) * UN;  // its last row sees more keys than that
           if (a.causal) {
@@ -222,34 +223,32 @@ __device__ bool find_item(const Args& a, int64_t item, Cursor& at, Item* out) {
         }
         return (tiles * a.chunks + a.tiles - 1) >> (a.tiles - 1);  // by 1 or 2
       };
-      const int64_t above = at.level == 0 ? 0 : pairs(1 << (a.levels - at.level));
-      const int64_t here = pairs(at.level == a.levels ? 0 : 1 << (a.levels - 1 - at.level)) - above;
-      const int64_t mine = here * a.heads_kv;
-      int64_t incl = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t t = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += t;
-      }
-      const int64_t all = __shfl_sync(0xffffffffu, incl, 31);
-      if (item >= at.before + all) {
+      const uint32_t above = at.level == 0 ? 0 : pairs(1 << (a.levels - at.level));
+      const uint32_t here = pairs(at.level == a.levels ? 0 : 1 << (a.levels - 1 - at.level)) - above;
+      const uint32_t mine = here * a.heads_kv, all = __reduce_add_sync(0xffffffffu, mine);
+      if (item - at.before >= all) {
         at.before += all;
         continue;
       }
-      const int64_t x = item - at.before - (incl - mine);
-      if (x >= 0 && x < mine) {
-        const int per_head = (int)a.by_kv.div((uint32_t)x);  // items are fewer than 2^31
-        const int64_t pair = above + per_head;
-        out->g = (int)x - per_head * a.heads_kv;
-        out->q0 = (int)q0, out->k0 = (int)k0, out->n = n, out->m = m;
+      uint32_t incl = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t t = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += t;
+      }
+      const uint32_t x = item - at.before - (incl - mine);  // huge where the item lies in a lane before
+      if (x < mine) {
+        const uint32_t per_head = a.by_kv.div(x), pair = above + per_head;
+        out->g = (int)(x - per_head * a.heads_kv);
+        out->q0 = q0, out->k0 = k0, out->n = n, out->m = m;
         out->first_block = 0;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const int64_t e = pair * a.tiles + t;
+          const uint32_t e = pair * a.tiles + t;
           Tile& tile = out->tile[t];
           tile.head = -1, tile.heads = 0, tile.first = 0, tile.tokens = 0, tile.units = 0;
-          if (t >= a.tiles || e >= (int64_t)blocks * a.chunks) continue;
-          const int at_block = (int)a.by_chunks.div((uint32_t)e), chunk = (int)e - at_block * a.chunks;
+          if (t >= a.tiles || e >= (uint32_t)(blocks * a.chunks)) continue;
+          const int at_block = (int)a.by_chunks.div(e), chunk = (int)e - at_block * a.chunks;
           tile.head = out->g * a.group + chunk * a.heads;
           tile.heads = min(a.heads, a.group - chunk * a.heads);
           tile.first = (blocks - 1 - at_block) * a.tokens;
@@ -583,7 +582,7 @@ __device__ __forceinline__ void load_items(const Args& a, Ctl* ctl, uint8_t* sme
   using S = Smem<DP>;
   volatile int* abort = &ctl->abort;
   const int lane = threadIdx.x & 31;
-  int64_t block = blockIdx.x;
+  int block = blockIdx.x;
   uint32_t n = 0, fixed = 0, q_turn[2] = {0, 0};  // blocks put into the ring, V blocks zeroed, Q tiles loaded
   bool ok = true, asked = false;
   uint32_t answers = 0;
@@ -591,7 +590,7 @@ __device__ __forceinline__ void load_items(const Args& a, Ctl* ctl, uint8_t* sme
     Item& it = ctl->item[turn & 1u];
     if (!(ok = wait_warp(ctl, &ctl->item_empty[turn & 1u], ((turn >> 1) & 1u) ^ 1u, UK_FAULT_PRODUCER))) break;
     // the first item was looked up before the barriers were up
-    if (turn > 0) any = block >= 0 && find_item(a, block, cursor, &it);
+    if (turn > 0) any = block >= 0 && find_item(a, (uint32_t)block, cursor, &it);
     __syncwarp();
     if (lane == 0) {
       it.any = any;
