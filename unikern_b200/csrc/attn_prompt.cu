@@ -175,8 +175,8 @@ struct Item {
 // rest (blocks take items as they come free, so the last ones should be short).
 // Within a level: sequences in order; in each the pairs of its tiles, the tiles
 // going from the last tokens to the first and through the group's heads, for
-// every key head.  A block's items come in rising order, so the search goes
-// on where the last one ended: 32 sequences at a time, a lane each.  (By the
+// every key head.  A block's items come in nearly rising order, so the search goes
+// on from where the last one ended: 32 sequences at a time, a lane each.  (By the
 // machine's long division a step of it took 2 us: 80 prompts of 84 rows, 21 heads
 // over 7 of 64, 82 us.)
 struct Cursor {
@@ -195,73 +195,87 @@ __device__ int first_level(const Args& a) {
   return a.levels - (32 - __clz(most));
 }
 
+// A lane's sequence of a chunk of 32, and its items of a level.
+struct Lot {
+  int q0, k0, n, m, blocks;
+  uint32_t above, mine;  // pairs (of a key head) of the levels before; items
+};
+
+// One warp: the items of a level's chunk.
+__device__ __forceinline__ uint32_t count_items(const Args& a, int level, int chunk, Lot& lot) {
+  const int b = chunk * 32 + (threadIdx.x & 31);
+  int q0 = 0, q1 = 0, k0 = 0, k1 = 0;
+  if (b < a.n_seq) {
+    const int most_q = (int)a.total_q, most_k = (int)a.total_k;
+    q0 = min(max(__ldg(a.cu_q + b), 0), most_q), q1 = min(max(__ldg(a.cu_q + b + 1), q0), most_q);
+    k0 = min(max(__ldg(a.cu_k + b), 0), most_k), k1 = min(max(__ldg(a.cu_k + b + 1), k0), most_k);
+  }
+  const int n = q1 - q0, m = k1 - k0, blocks = (int)a.by_tokens.div((uint32_t)(n + a.tokens - 1));
+  // pairs whose first tile sees at least `units` runs of keys
+  auto pairs = [&](int units) -> uint32_t {
+    uint32_t tiles = blocks;
+    if (units > 0) {
+      const int64_t end = (int64_t)(units - 1) * UN;  // its last row sees more keys than that
+      if (a.causal) {
+        const int64_t x = end - m + n;
+        tiles = x >= n ? 0 : blocks - (x > 0 ? (int)a.by_tokens.div((uint32_t)x) : 0);
+      } else if (m <= end) {
+        tiles = 0;
+      }
+    }
+    return (tiles * a.chunks + a.tiles - 1) >> (a.tiles - 1);  // by 1 or 2
+  };
+  const uint32_t above = level == 0 ? 0 : pairs(1 << (a.levels - level));
+  const uint32_t here = pairs(level == a.levels ? 0 : 1 << (a.levels - 1 - level)) - above;
+  lot = Lot{q0, k0, n, m, blocks, above, here * a.heads_kv};
+  return __reduce_add_sync(0xffffffffu, lot.mine);
+}
+
 // One warp: item i, or false behind the list's end.
 __device__ bool find_item(const Args& a, uint32_t item, Cursor& at, Item* out) {
-  const int lane = threadIdx.x & 31;
-  if (item < at.before) at = Cursor{};
-  for (; at.level <= a.levels; ++at.level, at.chunk = 0) {
-    for (; at.chunk * 32 < a.n_seq; ++at.chunk) {
-      const int b = at.chunk * 32 + lane;
-      int q0 = 0, q1 = 0, k0 = 0, k1 = 0;
-      if (b < a.n_seq) {
-        const int most_q = (int)a.total_q, most_k = (int)a.total_k;
-        q0 = min(max(__ldg(a.cu_q + b), 0), most_q), q1 = min(max(__ldg(a.cu_q + b + 1), q0), most_q);
-        k0 = min(max(__ldg(a.cu_k + b), 0), most_k), k1 = min(max(__ldg(a.cu_k + b + 1), k0), most_k);
-      }
-      const int n = q1 - q0, m = k1 - k0, blocks = (int)a.by_tokens.div((uint32_t)(n + a.tokens - 1));
-      // pairs whose first tile sees at least `units` runs of keys
-      auto pairs = [&](int units) -> uint32_t {
-        uint32_t tiles = blocks;
-        if (units > 0) {
-          const int64_t end = (int64_t)(units - 1) * UN;  // its last row sees more keys than that
-          if (a.causal) {
-            const int64_t x = end - m + n;
-            tiles = x >= n ? 0 : blocks - (x > 0 ? (int)a.by_tokens.div((uint32_t)x) : 0);
-          } else if (m <= end) {
-            tiles = 0;
-          }
-        }
-        return (tiles * a.chunks + a.tiles - 1) >> (a.tiles - 1);  // by 1 or 2
-      };
-      const uint32_t above = at.level == 0 ? 0 : pairs(1 << (a.levels - at.level));
-      const uint32_t here = pairs(at.level == a.levels ? 0 : 1 << (a.levels - 1 - at.level)) - above;
-      const uint32_t mine = here * a.heads_kv, all = __reduce_add_sync(0xffffffffu, mine);
-      if (item - at.before >= all) {
-        at.before += all;
-        continue;
-      }
-      uint32_t incl = mine;
+  const int lane = threadIdx.x & 31, chunks = (a.n_seq + 31) / 32;
+  Lot lot;
+  // blocks taken over do not come quite in order
+  while (item < at.before) {
+    if (--at.chunk < 0) at.chunk = chunks - 1, --at.level;
+    at.before -= count_items(a, at.level, at.chunk, lot);
+  }
+  for (;;) {
+    if (at.level > a.levels) return false;
+    const uint32_t all = count_items(a, at.level, at.chunk, lot);
+    if (item - at.before < all) break;
+    at.before += all;
+    if (++at.chunk == chunks) at.chunk = 0, ++at.level;
+  }
+  uint32_t incl = lot.mine;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t t = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += t;
-      }
-      const uint32_t x = item - at.before - (incl - mine);  // huge where the item lies in a lane before
-      if (x < mine) {
-        const uint32_t per_head = a.by_kv.div(x), pair = above + per_head;
-        out->g = (int)(x - per_head * a.heads_kv);
-        out->q0 = q0, out->k0 = k0, out->n = n, out->m = m;
-        out->first_block = 0;
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t t = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += t;
+  }
+  const uint32_t x = item - at.before - (incl - lot.mine);  // huge where the item lies in a lane before
+  if (x < lot.mine) {
+    const uint32_t per_head = a.by_kv.div(x), pair = lot.above + per_head;
+    out->g = (int)(x - per_head * a.heads_kv);
+    out->q0 = lot.q0, out->k0 = lot.k0, out->n = lot.n, out->m = lot.m;
+    out->first_block = 0;
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const uint32_t e = pair * a.tiles + t;
-          Tile& tile = out->tile[t];
-          tile.head = -1, tile.heads = 0, tile.first = 0, tile.tokens = 0, tile.units = 0;
-          if (t >= a.tiles || e >= (uint32_t)(blocks * a.chunks)) continue;
-          const int at_block = (int)a.by_chunks.div(e), chunk = (int)e - at_block * a.chunks;
-          tile.head = out->g * a.group + chunk * a.heads;
-          tile.heads = min(a.heads, a.group - chunk * a.heads);
-          tile.first = (blocks - 1 - at_block) * a.tokens;
-          tile.tokens = min(a.tokens, n - tile.first);
-          // one past the last key that its last token sees
-          const int64_t end = a.causal ? (int64_t)m - n + tile.first + tile.tokens : m;
-          tile.units = end <= 0 ? 0 : (int)((end + UN - 1) / UN);
-        }
-      }
-      return true;
+    for (int t = 0; t < 2; ++t) {
+      const uint32_t e = pair * a.tiles + t;
+      Tile& tile = out->tile[t];
+      tile.head = -1, tile.heads = 0, tile.first = 0, tile.tokens = 0, tile.units = 0;
+      if (t >= a.tiles || e >= (uint32_t)(lot.blocks * a.chunks)) continue;
+      const int at_block = (int)a.by_chunks.div(e), chunk = (int)e - at_block * a.chunks;
+      tile.head = out->g * a.group + chunk * a.heads;
+      tile.heads = min(a.heads, a.group - chunk * a.heads);
+      tile.first = (lot.blocks - 1 - at_block) * a.tokens;
+      tile.tokens = min(a.tokens, lot.n - tile.first);
+      // one past the last key that its last token sees
+      const int64_t end = a.causal ? (int64_t)lot.m - lot.n + tile.first + tile.tokens : lot.m;
+      tile.units = end <= 0 ? 0 : (int)((end + UN - 1) / UN);
     }
   }
-  return false;
+  return true;
 }
 
 template <int DP>
@@ -586,6 +600,22 @@ __device__ __forceinline__ void load_items(const Args& a, Ctl* ctl, uint8_t* sme
   uint32_t n = 0, fixed = 0, q_turn[2] = {0, 0};  // blocks put into the ring, V blocks zeroed, Q tiles loaded
   bool ok = true, asked = false;
   uint32_t answers = 0;
+  auto ask = [&] {
+    if (lane == 0) {
+      uk_mbar_expect_tx(&ctl->next, 16);
+      uk_next_block_ask(ctl->answer, &ctl->next);
+    }
+    asked = true;
+  };
+  auto taken = [&] {  // the block asked for, -1: none is left
+    if (!(ok = wait_warp(ctl, &ctl->next, answers & 1u, UK_FAULT_PRODUCER))) return -1;
+    ++answers;
+    asked = false;
+    const int x = uk_next_block(ctl->answer);
+    uk_fence_proxy_async_smem();  // read before the next answer is written
+    __syncwarp();
+    return x;
+  };
   for (uint32_t turn = 0; ok; ++turn) {
     Item& it = ctl->item[turn & 1u];
     if (!(ok = wait_warp(ctl, &ctl->item_empty[turn & 1u], ((turn >> 1) & 1u) ^ 1u, UK_FAULT_PRODUCER))) break;
@@ -595,14 +625,17 @@ __device__ __forceinline__ void load_items(const Args& a, Ctl* ctl, uint8_t* sme
     if (lane == 0) {
       it.any = any;
       uk_mbar_arrive(&ctl->item_full[turn & 1u]);  // releases the item to the waiting warps
-      if (any && !kSplit) {
-        uk_mbar_expect_tx(&ctl->next, 16);
-        uk_next_block_ask(ctl->answer, &ctl->next);
-      }
     }
-    __syncwarp();
+    // Behind the list's end every block is empty, up to as many as there are
+    // items: they are taken here, each in less time than it takes to start one
+    // (1024 prompts of 64 rows, 32 heads over 8 of 128: 1240 us without this).
+    while (!any && !kSplit && block >= 0) {
+      ask();
+      block = taken();
+    }
     if (!any) break;
-    asked = !kSplit;
+    if (!kSplit) ask();
+    __syncwarp();
     const int blocks = it.blocks();
     for (int j = 0; j < 2 * blocks && ok; ++j) {
       if (j == 0) {
@@ -651,12 +684,7 @@ __device__ __forceinline__ void load_items(const Args& a, Ctl* ctl, uint8_t* sme
       }
     }
     if (!ok || kSplit) break;
-    if (!(ok = wait_warp(ctl, &ctl->next, answers & 1u, UK_FAULT_PRODUCER))) break;
-    ++answers;
-    asked = false;
-    block = uk_next_block(ctl->answer);
-    uk_fence_proxy_async_smem();  // read before the next answer is written
-    __syncwarp();
+    block = taken();
   }
   if (!ok || *abort) {  // what is in flight lands before this block's memory is given up
     if (asked) uk_mbar_wait(&ctl->next, answers & 1u, nullptr, WAIT_NS);
