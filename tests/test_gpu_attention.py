@@ -2,6 +2,7 @@
 prompts on the GPU, against the definition in 64 bits; bounds in attn_testutil."""
 import ctypes
 import math
+import random
 
 import pytest
 import torch
@@ -394,6 +395,29 @@ def test_prompt_many_sequences_and_heads():
     o, lse = torch.empty_like(q), torch.empty(cu_q[-1], 6, device="cuda")
     a.attn_prompt(q, k, v, i32(cu_q), i32(cu_k), o, lse=lse)
     check_prompt(q, k, v, cu_q, cu_k, o, lse, 0.25, True)
+
+
+@pytest.mark.parametrize("seqs,heads,group,causal", [(1000, 2, 4, True), (1024, 8, 4, True), (1025, 8, 1, True),
+                                                     (33, 16, 3, True), (700, 3, 7, False)])
+def test_prompt_lists_of_mixed_lengths(seqs, heads, group, causal):
+    """Hundreds of short prompts among long contexts and empty ones: every tile
+    is found once, whatever the order its block starts in."""
+    a = abi()
+    fault()
+    rng = random.Random(seqs)
+    nq = [rng.choice([0, 1, 7, 31, 32, 33, 64, 90]) for _ in range(seqs)]
+    nk = [n + rng.choice([0, 0, 0, 63, 200, 1100]) for n in nq]
+    nq[-1] = nk[-1] = 129
+    cu_q, cu_k = prefix(nq), prefix(nk)
+    q, k, v = (randn(cu_q[-1], heads * group, 32, seed=1), randn(cu_k[-1], heads, 32, seed=2),
+               randn(cu_k[-1], heads, 32, seed=3))
+    o, lse = torch.full_like(q, math.nan), torch.full((cu_q[-1], heads * group), math.nan, device="cuda")
+    a.attn_prompt(q, k, v, i32(cu_q), i32(cu_k), o, causal=causal, lse=lse)
+    assert fault() == 0
+    assert not o.isnan().any() and not lse.isnan().any()  # every row was written
+    for b in rng.sample(range(seqs), 12) + [seqs - 1]:
+        x, y = slice(cu_q[b], cu_q[b + 1]), slice(cu_k[b], cu_k[b + 1])
+        check_prompt(q[x], k[y], v[y], [0, nq[b]], [0, nk[b]], o[x], lse[x], 32 ** -0.5, causal)
 
 
 def test_prompt_long():
