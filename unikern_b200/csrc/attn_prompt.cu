@@ -588,6 +588,27 @@ __device__ __forceinline__ void join_shares(const Args& a, Ctl* ctl, uint8_t* ri
     if (ctl->odd[row / 32] >> (row % 32) & 1u) look_again(a, it, tile, row, it.all_units);
 }
 
+// Behind the list's end every block is empty, up to as many as there are items:
+// one warp takes them over, each in less time than it takes to start one (1024
+// prompts of 64 rows, 32 heads over 8 of 128: 367 us, 1340 without this).
+__device__ __noinline__ void drain_blocks(Ctl* ctl, uint32_t answers) {
+  for (int block = 0; block >= 0; ++answers) {
+    if ((threadIdx.x & 31) == 0) {
+      uk_mbar_expect_tx(&ctl->next, 16);
+      uk_next_block_ask(ctl->answer, &ctl->next);
+    }
+    __syncwarp();
+    // this block's memory is not given up before the answer is there
+    if (!__all_sync(0xffffffffu, uk_mbar_wait(&ctl->next, answers & 1u, nullptr, WAIT_NS))) {
+      raise_fault(ctl, UK_FAULT_PRODUCER);
+      return;
+    }
+    block = uk_next_block(ctl->answer);
+    uk_fence_proxy_async_smem();  // read before the next answer is written
+    __syncwarp();
+  }
+}
+
 // ---- items and loads, one warp ---------------------------------------------------------
 template <int DP, bool kSplit>
 __device__ __forceinline__ void load_items(const Args& a, Ctl* ctl, uint8_t* smem, uint8_t* ring,
@@ -600,22 +621,6 @@ __device__ __forceinline__ void load_items(const Args& a, Ctl* ctl, uint8_t* sme
   uint32_t n = 0, fixed = 0, q_turn[2] = {0, 0};  // blocks put into the ring, V blocks zeroed, Q tiles loaded
   bool ok = true, asked = false;
   uint32_t answers = 0;
-  auto ask = [&] {
-    if (lane == 0) {
-      uk_mbar_expect_tx(&ctl->next, 16);
-      uk_next_block_ask(ctl->answer, &ctl->next);
-    }
-    asked = true;
-  };
-  auto taken = [&] {  // the block asked for, -1: none is left
-    if (!(ok = wait_warp(ctl, &ctl->next, answers & 1u, UK_FAULT_PRODUCER))) return -1;
-    ++answers;
-    asked = false;
-    const int x = uk_next_block(ctl->answer);
-    uk_fence_proxy_async_smem();  // read before the next answer is written
-    __syncwarp();
-    return x;
-  };
   for (uint32_t turn = 0; ok; ++turn) {
     Item& it = ctl->item[turn & 1u];
     if (!(ok = wait_warp(ctl, &ctl->item_empty[turn & 1u], ((turn >> 1) & 1u) ^ 1u, UK_FAULT_PRODUCER))) break;
@@ -625,17 +630,17 @@ __device__ __forceinline__ void load_items(const Args& a, Ctl* ctl, uint8_t* sme
     if (lane == 0) {
       it.any = any;
       uk_mbar_arrive(&ctl->item_full[turn & 1u]);  // releases the item to the waiting warps
+      if (any && !kSplit) {
+        uk_mbar_expect_tx(&ctl->next, 16);
+        uk_next_block_ask(ctl->answer, &ctl->next);
+      }
     }
-    // Behind the list's end every block is empty, up to as many as there are
-    // items: they are taken here, each in less time than it takes to start one
-    // (1024 prompts of 64 rows, 32 heads over 8 of 128: 1240 us without this).
-    while (!any && !kSplit && block >= 0) {
-      ask();
-      block = taken();
-    }
-    if (!any) break;
-    if (!kSplit) ask();
     __syncwarp();
+    if (!any) {
+      if (!kSplit && block >= 0) drain_blocks(ctl, answers);
+      break;
+    }
+    asked = !kSplit;
     const int blocks = it.blocks();
     for (int j = 0; j < 2 * blocks && ok; ++j) {
       if (j == 0) {
@@ -684,7 +689,12 @@ __device__ __forceinline__ void load_items(const Args& a, Ctl* ctl, uint8_t* sme
       }
     }
     if (!ok || kSplit) break;
-    block = taken();
+    if (!(ok = wait_warp(ctl, &ctl->next, answers & 1u, UK_FAULT_PRODUCER))) break;
+    ++answers;
+    asked = false;
+    block = uk_next_block(ctl->answer);
+    uk_fence_proxy_async_smem();  // read before the next answer is written
+    __syncwarp();
   }
   if (!ok || *abort) {  // what is in flight lands before this block's memory is given up
     if (asked) uk_mbar_wait(&ctl->next, answers & 1u, nullptr, WAIT_NS);
