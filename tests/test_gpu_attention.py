@@ -163,6 +163,56 @@ def test_decode_scales(scale):
         check_decode(pool, q, o, lse, scale)
 
 
+def both_splits(pool):
+    """The block table as it is, and with far more room: two splits of the work."""
+    wide = torch.full((pool.table.shape[0], 70000 // pool.page_size), -1, dtype=torch.int32, device="cuda")
+    wide[:, :pool.table.shape[1]] = pool.table
+    return pool.table, wide
+
+
+@pytest.mark.parametrize("kind", ["f16", "e4m3"])
+@pytest.mark.parametrize("group,dim", [(4, 128), (4, 64), (12, 128), (12, 48)])
+def test_decode_values_of_all_magnitudes(kind, group, dim):
+    """Value rows from 2^-12 to 2^8 times normal ones in one sequence, each with
+    a scale of its own in the 8-bit cache: the small rows' share is as exact."""
+    a = abi()
+    lens = [700, 33, 2500]
+    pool = Pool(kind, "hnd", 2, dim, 16, lens, seed=3)
+    g = torch.Generator("cuda").manual_seed(4)
+    for b, n in enumerate(lens):
+        x = torch.randn(n, 2, dim, device="cuda", generator=g)
+        # columns that large rows leave to the small ones
+        x[:, :, dim // 2:] *= 2.0 ** -10
+        e = torch.randint(-12, 9, (n, 2, 1), device="cuda", generator=g)
+        pool.values[b] = (pool.values[b][0], pool.put(1, b, 0, (x * torch.exp2(e.float())).half()))
+    q = randn(len(lens), 2 * group, dim, seed=5)
+    for table in both_splits(pool):
+        o, lse = torch.empty_like(q), torch.empty(q.shape[:2], device="cuda")
+        a.attn_decode(q, pool.cache, table, pool.lens_t, o, lse=lse)
+        check_decode(pool, q, o, lse, dim ** -0.5)
+
+
+@pytest.mark.parametrize("kind", ["f16", "e4m3"])
+@pytest.mark.parametrize("n", [700, 16385])
+def test_decode_one_large_value_in_front_of_a_tail(kind, n):
+    """A first row of large values and weight in a few columns, zero in the
+    others, in front of a tail of small values whose weights lie 14.5 bits lower
+    and still make up much of the sum."""
+    a = abi()
+    pool = Pool(kind, "hnd", 1, 64, 16, [n], seed=1, fill=False)
+    k, v = torch.zeros(n, 1, 64, device="cuda"), randn(n, 1, 64, seed=2).float().abs() * 2.0 ** -8
+    k[0, 0, 0] = 14.5 * math.log(2) * 8  # times q = 1 and the scale 1 / 8
+    v[0] = 0
+    v[0, 0, :8] = 448 * 2.0 ** 3
+    pool.values[0] = (pool.put(0, 0, 0, k.half()), pool.put(1, 0, 0, v.half()))
+    q = torch.zeros(1, 4, 64, device="cuda", dtype=torch.float16)
+    q[..., 0] = 1
+    for table in both_splits(pool):
+        o, lse = torch.empty_like(q), torch.empty(1, 4, device="cuda")
+        a.attn_decode(q, pool.cache, table, pool.lens_t, o, lse=lse)
+        check_decode(pool, q, o, lse, 0.125)
+
+
 @pytest.mark.parametrize("kind", ["f16", "e4m3"])
 def test_decode_infinities_and_nan(kind):
     """Held NaN and infinities reach exactly the heads and columns they should;

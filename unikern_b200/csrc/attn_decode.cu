@@ -33,8 +33,11 @@
 //     the operand packs them, and the row index d is renamed.
 //   P^T (B operand): the S^T accumulator has position and head exchanged; an
 //     8 x 8 transpose between lanes (movmatrix) puts that right.
-// e4m3 rows are converted to binary16 in registers, exactly; the keys' scale
-// multiplies the score, the values' goes into the weight's exponent.
+// e4m3 rows are converted to binary16 in registers, exactly.  The keys' scale
+// multiplies the score; the values' multiplies the converted codes (exact, too:
+// a held value is a binary16 one).  In the weight's exponent instead, where it
+// costs fewer instructions, it would push the weights of rows of small values into
+// binary16's subnormals beside one row of large ones.
 // K of the next tile loads while the softmax and V product of this one run,
 // then V of the next; page ids load one tile earlier still.
 #include "kv_cache.cuh"
@@ -500,15 +503,14 @@ __global__ void __launch_bounds__(THREADS, NH == 1 ? 3 : 2) k_attn_decode(Args a
       }
       load_k(rows, p + CT);
 
-      // ---- scores, reference and weights.  e4m3: the value row's scale 2^ev
-      // goes into the weight's exponent, t = s + ev, and the codes enter the
-      // product unscaled; l takes 2^(t - m) 2^-ev in fp32.
-      float top[NH][2], inv_ev[NT][2];
-      float ek = 1.f, ev = 0.f, inv = 1.f;  // of this lane's position: scale * 2^ek, ev and 2^-ev
+      // ---- scores, reference and weights
+      float top[NH][2];
+      float ek = 1.f;    // of this lane's position: scale * 2^ek
+      uint32_t ev2 = 0;  // 2^ev of an even lane's position and of the next one, as halves
       if (!S::kF16) {
         ek = a.scale2 * uk_exp_scale(now_at.ek);
-        ev = __uint_as_float(0x4b000000u | now_at.ev) - 8388735.f;  // ev - 127, through 2^23
-        inv = uk_exp_scale(254u - now_at.ev);
+        const uint32_t own = uk_half2_of(uk_exp_scale(now_at.ev));
+        ev2 = __byte_perm(own, __shfl_xor_sync(0xffffffffu, own, 1), 0x7610);
       }
 #pragma unroll
       for (int w = 0; w < NH; ++w) top[w][0] = top[w][1] = -INFINITY;
@@ -516,20 +518,14 @@ __global__ void __launch_bounds__(THREADS, NH == 1 ? 3 : 2) k_attn_decode(Args a
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          float f = 1.f, add = 0.f;
-          if (!S::kF16) {
-            const int from = n * 16 + i * 8 + r;
-            f = __shfl_sync(0xffffffffu, ek, from);
-            add = __shfl_sync(0xffffffffu, ev, from);
-            inv_ev[n][i] = __shfl_sync(0xffffffffu, inv, from);
-          }
+          const float f = S::kF16 ? a.scale2 : __shfl_sync(0xffffffffu, ek, n * 16 + i * 8 + r);
           const bool on = now >> (2 * n + i) & 1u;
 #pragma unroll
           for (int w = 0; w < NH; ++w)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               float& v = s[n][w][2 * i + h];
-              v = on ? (S::kF16 ? v * a.scale2 : fmaf(v, f, add)) : -INFINITY;
+              v = on ? v * f : -INFINITY;
               top[w][h] = fmaxf(top[w][h], v);
             }
         }
@@ -567,8 +563,8 @@ __global__ void __launch_bounds__(THREADS, NH == 1 ? 3 : 2) k_attn_decode(Args a
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const float a0 = ex2(s[n][w][2 * i] - z0), a1 = ex2(s[n][w][2 * i + 1] - z1);
-            l[w][0] += S::kF16 ? a0 : a0 * inv_ev[n][i];
-            l[w][1] += S::kF16 ? a1 : a1 * inv_ev[n][i];
+            l[w][0] += a0;
+            l[w][1] += a1;
             pf[n][w][i] = transpose8(pack_half(a0, a1));
           }
       }
@@ -589,6 +585,8 @@ __global__ void __launch_bounds__(THREADS, NH == 1 ? 3 : 2) k_attn_decode(Args a
               for (int w = 0; w < NH; ++w) mma16816(acc[k * 4 + i][w], a0, a1, a2, a3, pf[n][w][0], pf[n][w][1]);
             }
         } else {
+          const uint32_t e0 = __shfl_sync(0xffffffffu, ev2, n * 16 + 2 * q);  // of positions 2q, 2q + 1
+          const uint32_t e1 = __shfl_sync(0xffffffffu, ev2, n * 16 + 8 + 2 * q);
 #pragma unroll
           for (int i = 0; i < S::VW; ++i)
 #pragma unroll
@@ -599,6 +597,8 @@ __global__ void __launch_bounds__(THREADS, NH == 1 ? 3 : 2) k_attn_decode(Args a
               uint32_t a0, a1, a2, a3;
               uk_e4m3x4_to_half2(y0, &a0, &a1);
               uk_e4m3x4_to_half2(y1, &a2, &a3);
+              a0 = uk_mul_half2(a0, e0), a1 = uk_mul_half2(a1, e0);
+              a2 = uk_mul_half2(a2, e1), a3 = uk_mul_half2(a3, e1);
 #pragma unroll
               for (int w = 0; w < NH; ++w)
                 mma16816(acc[2 * i + half][w], a0, a1, a2, a3, pf[n][w][0], pf[n][w][1]);
