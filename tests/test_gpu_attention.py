@@ -389,6 +389,21 @@ def test_prompt_scales(scale):
     check_prompt(q, k, v, [0, n], [0, n], o, lse, scale, True)
 
 
+@pytest.mark.parametrize("equal", [True, False])
+def test_prompt_row_by_row_over_a_long_context(equal):
+    """A negative scale takes the rows one by one: sums of 2^20 terms, of equal
+    ones behind a first key of its own weight and of random ones."""
+    a = abi()
+    n, m, dim = 6, 1 << 20, 8
+    q, k, v = randn(n, 1, dim, seed=1), randn(m, 1, dim, seed=2), randn(m, 1, dim, seed=3)
+    if equal:
+        q[:, 0, 0] = torch.linspace(-4, 1, n, device="cuda").half()
+        k[0], k[1:], v = 1.0, 0.0, v.abs() + 1
+    o, lse = torch.empty_like(q), torch.empty(n, 1, device="cuda")
+    a.attn_prompt(q, k, v, i32([0, n]), i32([0, m]), o, scale=-0.3, lse=lse)
+    check_prompt(q, k, v, [0, n], [0, m], o, lse, -0.3, True)
+
+
 def test_prompt_weak_tail():
     """A strong first key in front of many weak ones, whose weights together
     still count: they must not vanish in a narrow type."""

@@ -47,6 +47,7 @@ __device__ unsigned int g_attn_prompt_fault = 0;
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float GROW = 8.f;  // scores may pass the reference by 2^8 before it moves
 
 struct Args {
   const uint16_t *q, *k, *v;
@@ -86,17 +87,29 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 
+// A sum that carries what its additions round off (Kahan): those of equal terms
+// all round the same way (2^20 keys by plain sums: 0.4 % off).
+struct LongSum {
+  float s = 0.f, c = 0.f;
+  __device__ __forceinline__ void add(float x) {
+    const float y = x - c, t = s + y;
+    c = fabsf(t) < INFINITY ? (t - s) - y : 0.f;  // an infinity stays one
+    s = t;
+  }
+  __device__ __forceinline__ void scale(float f) { s *= f, c *= f; }
+};
+
 // One row by one warp, key by key, on CUDA cores: keys [k0, end).  A lane
 // holds four of the row's values.
 __device__ __noinline__ void attend_row(const Args& a, int64_t t, int h, int64_t k0, int64_t end) {
   const int lane = threadIdx.x & 31, g = h / a.group;
   const float4 q = row4(a.q + t * a.q_token + h * a.q_head, lane, a.dim);
-  float m = -INFINITY, l = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  float m = -INFINITY;
+  LongSum l, o[4];
   constexpr int U = 4;  // keys in flight
   for (int64_t j = k0; j < end; j += U) {
     float4 k[U], v[U];
-    float s[U], m2 = m;
+    float s[U], top = -INFINITY;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const bool on = j + u < end;
@@ -107,30 +120,37 @@ __device__ __noinline__ void attend_row(const Args& a, int64_t t, int h, int64_t
     for (int u = 0; u < U; ++u) {
       s[u] = uk_warp_sum(q.x * k[u].x + q.y * k[u].y + q.z * k[u].z + q.w * k[u].w) * a.scale2;
       if (j + u >= end) s[u] = -INFINITY;
-      m2 = fmaxf(m2, s[u]);
+      top = fmaxf(top, s[u]);
     }
-    const float z = m2 == -INFINITY ? 0.f : m2, f = m2 == -INFINITY ? 1.f : ex2(m - m2);
-    m = m2;
-    l *= f;
-    o = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+    if (top > m + GROW) {
+      const float f = ex2(m - top);
+      m = top;
+      l.scale(f);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) o[c].scale(f);
+    }
+    const float z = m == -INFINITY ? 0.f : m;
+    float e = 0.f;
+    float4 p = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const float e = ex2(s[u] - z);
-      l += e;
-      o = make_float4(fmaf(e, v[u].x, o.x), fmaf(e, v[u].y, o.y), fmaf(e, v[u].z, o.z), fmaf(e, v[u].w, o.w));
+      const float w = ex2(s[u] - z);
+      e += w;
+      p = make_float4(fmaf(w, v[u].x, p.x), fmaf(w, v[u].y, p.y), fmaf(w, v[u].z, p.z), fmaf(w, v[u].w, p.w));
     }
+    l.add(e);
+    o[0].add(p.x), o[1].add(p.y), o[2].add(p.z), o[3].add(p.w);
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = l.s == 0.f ? 0.f : 1.f / l.s;
   if (lane * 4 < a.dim)
     reinterpret_cast<uint2*>(a.o + t * a.o_token + h * a.o_head)[lane] =
-        make_uint2(pack_half(o.x * inv, o.y * inv), pack_half(o.z * inv, o.w * inv));
-  if (a.lse != nullptr && lane == 0) a.lse[t * a.heads_q + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
+        make_uint2(pack_half(o[0].s * inv, o[1].s * inv), pack_half(o[2].s * inv, o[3].s * inv));
+  if (a.lse != nullptr && lane == 0) a.lse[t * a.heads_q + h] = l.s == 0.f ? -INFINITY : (m + log2f(l.s)) * LN2;
 }
 
 // ---- what one CTA works on -----------------------------------------------------------
 constexpr int BM = 128, BN = 128;  // rows of a tile, keys of a block
 constexpr int UN = 64;             // keys of a softmax step (half a block)
-constexpr float GROW = 8.f;        // scores may pass the reference by 2^8 before it moves
 constexpr float SHIFT = 7.f;       // weights are held as 2^7 * 2^(s - m): up to 2^15, binary16 ends at 2^16
 // three warpgroups: two of softmax, one of the MMA and load warps (and an idle
 // one).  They launch with 168 registers a thread; the softmax takes 216 (a row
