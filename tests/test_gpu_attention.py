@@ -439,6 +439,24 @@ def test_prompt_rows_do_not_see_behind_their_mask():
                 assert torch.isfinite(lse).all()
 
 
+def test_prompt_rows_computed_again_behind_a_long_context():
+    """A NaN that only the last query may see, behind so many keys that the 127
+    rows before it in its tile take seconds to be computed again: the other warps
+    wait for them, and go on."""
+    a = abi()
+    fault()
+    n, m, heads, dim = 9600, 320000, 16, 8
+    q, k, v = randn(n, heads, dim, seed=1), randn(m, heads, dim, seed=2), randn(m, heads, dim, seed=3)
+    v[m - 1, 3, 5] = math.nan
+    o, lse = torch.full_like(q, 7.0), torch.full((n, heads), 7.0, device="cuda")
+    a.attn_prompt(q, k, v, i32([0, n]), i32([0, m]), o, lse=lse)
+    assert fault() == 0
+    assert torch.isnan(o[-1, 3, 5]) and torch.isnan(o).sum() == 1
+    rows = slice(n - 128, n - 1)
+    check_prompt(q[rows, 3:4], k[:m - 1, 3:4], v[:m - 1, 3:4], [0, 127], [0, m - 1], o[rows, 3:4], lse[rows, 3:4],
+                 dim ** -0.5, True)
+
+
 def test_prompt_bounds_of_the_length_arrays():
     """Row bounds outside the tensors are clamped, never read."""
     a = abi()

@@ -32,7 +32,9 @@
 // them holds a NaN or an infinity the row is computed again, key by key.
 //
 // Every mbarrier wait is bounded (uk_mbar_wait); a timeout sets the fault word
-// read by uk_cuda_pipeline_fault() and the CTA unwinds.
+// read by uk_cuda_pipeline_fault() and the CTA unwinds.  Rows that are computed
+// again may take longer than any limit (17.5 us a key for a warp's 32 rows): while
+// they do, a counter moves, and the waits for their warp are taken up again.
 #include <cudaTypedefs.h>
 
 #include <mutex>
@@ -88,7 +90,7 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 // A sum that carries what its additions round off (Kahan): those of equal terms
-// all round the same way (2^20 keys by plain sums: 0.4 % off).
+// all round the same way (2^20 keys by plain sums: 7 times the tests' bound off).
 struct LongSum {
   float s = 0.f, c = 0.f;
   __device__ __forceinline__ void add(float x) {
@@ -100,14 +102,16 @@ struct LongSum {
 };
 
 // One row by one warp, key by key, on CUDA cores: keys [k0, end).  A lane
-// holds four of the row's values.
-__device__ __noinline__ void attend_row(const Args& a, int64_t t, int h, int64_t k0, int64_t end) {
+// holds four of the row's values.  *beat (in shared memory, where there is one)
+// moves every few milliseconds.
+__device__ __noinline__ void attend_row(const Args& a, int64_t t, int h, int64_t k0, int64_t end, unsigned* beat) {
   const int lane = threadIdx.x & 31, g = h / a.group;
   const float4 q = row4(a.q + t * a.q_token + h * a.q_head, lane, a.dim);
   float m = -INFINITY;
   LongSum l, o[4];
   constexpr int U = 4;  // keys in flight
   for (int64_t j = k0; j < end; j += U) {
+    if (beat != nullptr && ((j - k0) & 4095) == 0 && lane == 0) atomicAdd(beat, 1u);
     float4 k[U], v[U];
     float s[U], top = -INFINITY;
 #pragma unroll
@@ -159,7 +163,7 @@ constexpr int NUM_THREADS = 384;
 constexpr int REGS_LAUNCH = 168, REGS_SOFTMAX = 216, REGS_OTHERS = 72;
 static_assert(2 * REGS_SOFTMAX + REGS_OTHERS <= 3 * REGS_LAUNCH, "registers of the block");
 constexpr int MMA_WARP = 8, LOAD_WARP = 10;  // MMA_WARP + t: tile t
-constexpr uint64_t WAIT_NS = 30000000000ull;  // 30 s: rows computed again may take long
+constexpr uint64_t WAIT_NS = 2000000000ull;  // 2 s: a pass over 2^25 keys, which a tile may have to wait for, takes 0.6 s
 
 struct Tile {
   int head;    // its first query head; -1: no tile
@@ -320,6 +324,7 @@ struct Ctl {
   alignas(16) uint8_t answer[16];
   uint32_t tmem;
   int abort;
+  unsigned beat;    // moves while rows are computed again
   unsigned odd[4];  // rows of a shared tile to look at again
   Item item[2];
 };
@@ -331,9 +336,26 @@ __device__ __forceinline__ void raise_fault(Ctl* ctl, unsigned bit) {
   ctl->abort = 1;
 }
 
+// uk_mbar_wait, but a wait that has run out is taken up once more, and again for
+// as long as `beat` moves meanwhile: its steps take some milliseconds, and there are
+// finitely many.
+__device__ __forceinline__ bool wait_beat(Ctl* ctl, uint64_t* bar, uint32_t parity, volatile int* abort) {
+  if (uk_mbar_try_wait(bar, parity)) return true;
+  uint64_t t0 = uk_globaltimer();
+  unsigned seen = 0;  // beat is never 0
+  for (uint32_t i = 1;; ++i) {
+    if (uk_mbar_try_wait(bar, parity)) return true;
+    if ((i & 255u) != 0) continue;
+    if (abort != nullptr && *abort) return false;
+    if (uk_globaltimer() - t0 <= WAIT_NS) continue;
+    const unsigned now = *(volatile unsigned*)&ctl->beat;
+    if (now == seen) return false;
+    seen = now, t0 = uk_globaltimer();
+  }
+}
 // a bounded wait by a whole warp: the same answer in every lane
 __device__ __forceinline__ bool wait_warp(Ctl* ctl, uint64_t* bar, uint32_t parity, unsigned bit) {
-  if (__all_sync(0xffffffffu, uk_mbar_wait(bar, parity, &ctl->abort, WAIT_NS))) return true;
+  if (__all_sync(0xffffffffu, wait_beat(ctl, bar, parity, &ctl->abort))) return true;
   if (!*(volatile int*)&ctl->abort) raise_fault(ctl, bit);
   return false;
 }
@@ -348,7 +370,8 @@ __device__ __forceinline__ int end_of(const Args& a, const Item& it, int token) 
 
 // A row with a finite sum that is not finite itself (one warp): it is computed
 // again where one of the keys between its mask and the end of its blocks is not.
-__device__ __noinline__ void look_again(const Args& a, const Item& it, const Tile& tile, int row, int units) {
+__device__ __noinline__ void look_again(const Args& a, const Item& it, const Tile& tile, int row, int units,
+                                        unsigned* beat) {
   const Row r(a, tile, row);
   const int lane = threadIdx.x & 31, from = end_of(a, it, r.token), to = min(units * UN, it.m);
   bool bad = false;
@@ -357,7 +380,7 @@ __device__ __noinline__ void look_again(const Args& a, const Item& it, const Til
     bad = __any_sync(0xffffffffu, !(fabsf(v.x) + fabsf(v.y) + fabsf(v.z) + fabsf(v.w) < INFINITY));
   }
   __syncwarp();  // the row's stores before come before these
-  if (bad) attend_row(a, (int64_t)it.q0 + r.token, r.head, it.k0, (int64_t)it.k0 + from);
+  if (bad) attend_row(a, (int64_t)it.q0 + r.token, r.head, it.k0, (int64_t)it.k0 + from, beat);
 }
 
 // A shared tile's sums in shared memory: 128 rows of DP floats (16-byte pieces
@@ -560,7 +583,7 @@ __device__ __forceinline__ bool softmax_tile(const Args& a, Ctl* ctl, const Item
   while (odd != 0) {
     const int r = __ffs(odd) - 1;
     odd &= odd - 1;
-    look_again(a, it, tile, quad * 32 + r, units);
+    look_again(a, it, tile, quad * 32 + r, units, &ctl->beat);
   }
   return true;
 }
@@ -605,7 +628,7 @@ __device__ __forceinline__ void join_shares(const Args& a, Ctl* ctl, uint8_t* ri
   }
   asm volatile("bar.sync 1, 256;" ::: "memory");
   for (int row = rank * rows + (int)(threadIdx.x >> 5); row < (rank + 1) * rows; row += 8)
-    if (ctl->odd[row / 32] >> (row % 32) & 1u) look_again(a, it, tile, row, it.all_units);
+    if (ctl->odd[row / 32] >> (row % 32) & 1u) look_again(a, it, tile, row, it.all_units, &ctl->beat);
 }
 
 // Behind the list's end every block is empty, up to as many as there are items:
@@ -824,7 +847,7 @@ __device__ __forceinline__ void issue_products(Ctl* ctl, int t, uint8_t* smem, u
   }
   // every product issued completes before TMEM and shared memory are given up
   commit(&ctl->teardown);
-  if (!__all_sync(0xffffffffu, uk_mbar_wait(&ctl->teardown, 0, nullptr, WAIT_NS)))
+  if (!__all_sync(0xffffffffu, wait_beat(ctl, &ctl->teardown, 0, nullptr)))  // the other tile's warp, too, has to get there
     atomicOr(&uk::g_attn_prompt_fault, UK_FAULT_TEARDOWN);
 }
 
@@ -864,6 +887,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     uk_mbar_init(&ctl->v_landed, 1);
     uk_mbar_init(&ctl->teardown, 2);
     ctl->abort = 0;
+    ctl->beat = 1;
     for (int i = 0; i < 4; ++i) ctl->odd[i] = 0;
     uk_fence_mbar_init();
     uk_tma_prefetch_desc(&tm_q);
@@ -938,7 +962,7 @@ __global__ void __launch_bounds__(256) k_attn_prompt_rows(const __grid_constant_
   if (b < 0) return;
   const int64_t q1 = clamp64(__ldg(a.cu_q + b + 1), 0, a.total_q);
   const int64_t k0 = clamp64(__ldg(a.cu_k + b), 0, a.total_k), k1 = clamp64(__ldg(a.cu_k + b + 1), k0, a.total_k);
-  attend_row(a, t, h, k0, a.causal ? k1 - (q1 - 1 - t) : k1);
+  attend_row(a, t, h, k0, a.causal ? k1 - (q1 - 1 - t) : k1, nullptr);
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
@@ -1041,8 +1065,7 @@ extern "C" int uk_cuda_attn_prompt_f16(const uint16_t* Q, int64_t q_token_stride
                                        int64_t total_k, int heads_q, int heads_kv, int dim, float scale, int causal,
                                        uint16_t* O, int64_t o_token_stride, int64_t o_head_stride, float* LSE,
                                        void* stream) {
-  // 2^25 keys: a tile's pass over them (0.4 s), and a warp's over each of its 32 rows
-  // when all have to be computed again (5 s), stay well within the kernel's bounded
+  // 2^25 keys: a tile's pass over them (0.6 s) stays well within the kernel's bounded
   // waits; queries: a tile's row numbers stay within 31 bits
   if (n_seq < 0 || n_seq > uk::MAX_SEQS || total_q < 0 || total_k < 0 || total_q > 0x7fffff00 || total_k > (1 << 25))
     return uk::fail(UK_EINVAL, "attn_prompt: n_seq %d (at most 2^24), total_q %lld (2^31 - 256), total_k %lld (2^25)",
