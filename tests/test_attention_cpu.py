@@ -189,3 +189,139 @@ int main() {
                    check=True, capture_output=True)
     r = subprocess.run([str(exe)], capture_output=True, text=True)
     assert r.returncode == 0, r.stdout
+
+
+def test_prompt_items_in_any_order(tmp_path):
+    """The blocks of the prompt attention, each with the numbers that it takes over
+    in an arbitrary order: every row of every head is worked on once, with all the
+    keys it sees, and no block gives up while numbers are left."""
+    src = tmp_path / "items.cu"
+    src.write_text(r'''
+#include "attn_prompt_items.cuh"
+#include <algorithm>
+#include <cstdio>
+#include <random>
+#include <vector>
+using namespace uk_prompt;
+
+struct Sim {  // what a warp does in find_item and drain_blocks, lane by lane
+  const Args& a;
+  uint32_t count(int level, int chunk) const {
+    uint32_t n = 0;
+    for (int lane = 0; lane < 32; ++lane) n += lot_of(a, level, chunk, lane).mine;
+    return n;
+  }
+  bool find(uint32_t item, Cursor& at, Item* out) const {
+    if (!find_chunk(a, item, at, [&](int l, int c) { return count(l, c); })) return false;
+    uint32_t x = item - at.before;
+    for (int lane = 0; lane < 32; ++lane) {
+      const Lot lot = lot_of(a, at.level, at.chunk, lane);
+      if (x < lot.mine) { place_item(a, lot, x, out); return true; }
+      x -= lot.mine;
+    }
+    return false;
+  }
+};
+
+int main() {
+  std::mt19937 rng(1);
+  auto pick = [&](int lo, int hi) { return lo + (int)(rng() % (unsigned)(hi - lo + 1)); };
+  for (int round = 0; round < 400; ++round) {
+    const int n_seq = round % 10 == 0 ? pick(1025, 1100) : round % 3 ? pick(1, 40) : pick(1, 300);
+    const int kv = pick(1, 5), group = round % 7 == 0 ? pick(100, 300) : pick(1, 9), sms = pick(1, 24);
+    std::vector<int32_t> cq{pick(0, 2)}, ck{pick(0, 2)};
+    for (int b = 0; b < n_seq; ++b) {
+      const int n = pick(0, 3) ? pick(0, 40) : pick(0, 400);
+      cq.push_back(cq.back() + n);
+      ck.push_back(ck.back() + std::max(0, n + (pick(0, 2) ? 0 : pick(-30, 3000))));
+    }
+    Args a{};
+    a.cu_q = cq.data(), a.cu_k = ck.data(), a.n_seq = n_seq, a.heads_q = kv * group, a.heads_kv = kv, a.group = group;
+    a.total_q = cq.back() + pick(0, 300), a.total_k = std::max(1, ck.back() + pick(0, 300)), a.causal = pick(0, 1);
+    if (a.total_q == 0) continue;
+    const int64_t grid = plan_items(&a, sms);
+    if (grid < 0) { std::puts("grid"); return 1; }
+    const Sim sim{a};
+    int most = 0;
+    for (int b = 0; b < n_seq; ++b) most = std::max(most, keys_of(a, b));
+
+    // the numbers nobody has got yet, handed out from the end of `left`
+    std::vector<int> left(grid);
+    for (int i = 0; i < grid; ++i) left[i] = i;
+    switch (round % 4) {
+      case 0: std::reverse(left.begin(), left.end()); break;  // rising
+      case 1: break;                                          // falling: those behind the list's end first
+      default: std::shuffle(left.begin(), left.end(), rng);
+    }
+    auto ask = [&] {
+      if (left.empty()) return -1;
+      const int x = left.back();
+      left.pop_back();
+      return x;
+    };
+    std::vector<uint8_t> seen((size_t)a.total_q * a.heads_q, 0);
+    int64_t worked = 0;
+    auto work = [&](const Item& it) {
+      ++worked;
+      if (it.tile[0].head < 0) return false;
+      for (const Tile& t : it.tile) {
+        if (t.head < 0) continue;
+        int end = 0;
+        for (int i = 0; i < BM; ++i) {
+          const Row r(a, t, i);
+          if (!r.on) continue;
+          if (r.token >= it.n || r.head / a.group != it.g) return false;
+          if (seen[(size_t)(it.q0 + r.token) * a.heads_q + r.head]++) return false;
+          end = std::max(end, a.causal ? it.m - it.n + 1 + r.token : it.m);
+        }
+        if (t.units != (end + UN - 1) / UN) return false;
+      }
+      return true;
+    };
+    struct Block { int number; Cursor at; bool any; Item it; };
+    std::vector<Block> running;
+    auto start = [&] {
+      Block b{ask(), {}, false, {}};
+      if (b.number < 0) return;
+      if (a.levels > 0) b.at.level = first_level_of(a, most);
+      b.any = sim.find(b.number, b.at, &b.it);
+      running.push_back(b);
+    };
+    for (int i = 0; i < sms; ++i) start();
+    while (!running.empty()) {
+      const size_t i = rng() % running.size();
+      Block& b = running[i];
+      if (!b.any && b.number >= 0 && a.split == 1) {
+        b.number = next_listed(b.at.before, ask);
+        if (b.number >= 0) {
+          Cursor fresh;
+          b.any = sim.find(b.number, fresh, &b.it);
+        }
+      }
+      if (!b.any) {  // leaves; another block starts in its place
+        running.erase(running.begin() + i);
+        start();
+        continue;
+      }
+      if (!work(b.it)) { std::printf("round %d: item %d\n", round, b.number); return 1; }
+      b.any = false;
+      if (a.split > 1) { b.number = -1; continue; }  // one tile a cluster
+      b.number = ask();
+      b.any = b.number >= 0 && sim.find(b.number, b.at, &b.it);
+    }
+    for (int t = 0; t < a.total_q; ++t)
+      for (int h = 0; h < a.heads_q; ++h)
+        if (seen[(size_t)t * a.heads_q + h] != (t >= cq[0] && t < cq.back())) {
+          std::printf("round %d: row %d head %d\n", round, t, h);
+          return 1;
+        }
+  }
+  return 0;
+}
+''')
+    from unikern_b200 import build
+    exe = tmp_path / "items"
+    subprocess.run([build.nvcc(), "-O1", "-std=c++17", "--expt-relaxed-constexpr", "-I", str(ROOT / "include"), "-I",
+                    str(build.CSRC), str(src), "-o", str(exe)], check=True, capture_output=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert r.returncode == 0, r.stdout

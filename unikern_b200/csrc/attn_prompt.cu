@@ -40,7 +40,7 @@
 #include <mutex>
 #include <utility>
 
-#include "kv_cache.cuh"
+#include "attn_prompt_items.cuh"
 
 namespace uk {
 __device__ unsigned int g_attn_prompt_fault = 0;
@@ -48,26 +48,10 @@ __device__ unsigned int g_attn_prompt_fault = 0;
 
 namespace {
 
+using namespace uk_prompt;
+
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float GROW = 8.f;  // scores may pass the reference by 2^8 before it moves
-
-struct Args {
-  const uint16_t *q, *k, *v;
-  uint16_t* o;
-  int64_t q_token, q_head, k_token, k_head, v_token, v_head, o_token, o_head;
-  float* lse;
-  const int32_t *cu_q, *cu_k;
-  int n_seq, heads_q, heads_kv, group, dim, causal;
-  int64_t total_q, total_k;
-  float scale2;
-  int levels;  // of the order of work
-  int tiles;   // of an item: 2, or 1 where pairs would leave SMs without work
-  int split;   // CTAs (a cluster) that share a tile's keys
-  // a tile is `tokens` query tokens by `heads` query heads of one key head, the
-  // heads of a token side by side; `chunks` tiles make the key head's group
-  int tokens, heads, chunks;
-  UkFastDiv by_tokens, by_heads, by_chunks, by_kv;  // by tokens, heads, chunks and heads_kv
-};
 
 __device__ __forceinline__ float4 row4(const uint16_t* row, int lane, int dim) {
   if (lane * 4 >= dim) return make_float4(0.f, 0.f, 0.f, 0.f);
@@ -76,8 +60,6 @@ __device__ __forceinline__ float4 row4(const uint16_t* row, int lane, int dim) {
   const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
   return make_float4(x.x, x.y, y.x, y.y);
 }
-
-__device__ __forceinline__ int64_t clamp64(int64_t x, int64_t lo, int64_t hi) { return x < lo ? lo : x > hi ? hi : x; }
 
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
@@ -153,8 +135,6 @@ __device__ __noinline__ void attend_row(const Args& a, int64_t t, int h, int64_t
 }
 
 // ---- what one CTA works on -----------------------------------------------------------
-constexpr int BM = 128, BN = 128;  // rows of a tile, keys of a block
-constexpr int UN = 64;             // keys of a softmax step (half a block)
 constexpr float SHIFT = 7.f;       // weights are held as 2^7 * 2^(s - m): up to 2^15, binary16 ends at 2^16
 // three warpgroups: two of softmax, one of the MMA and load warps (and an idle
 // one).  They launch with 168 registers a thread; the softmax takes 216 (a row
@@ -165,112 +145,22 @@ static_assert(2 * REGS_SOFTMAX + REGS_OTHERS <= 3 * REGS_LAUNCH, "registers of t
 constexpr int MMA_WARP = 8, LOAD_WARP = 10;  // MMA_WARP + t: tile t
 constexpr uint64_t WAIT_NS = 2000000000ull;  // 2 s: a pass over 2^25 keys, which a tile may have to wait for, takes 0.6 s
 
-struct Tile {
-  int head;    // its first query head; -1: no tile
-  int heads;   // query heads it has
-  int first;   // its first token within the sequence
-  int tokens;  // tokens it has
-  int units;   // runs of 64 keys that some row of it sees
-  __device__ __forceinline__ int blocks() const { return (units + 1) / 2; }
-};
-// row i of a tile: token i / a.heads of it, head i % a.heads
-struct Row {
-  int token, head;
-  bool on;
-  __device__ __forceinline__ Row(const Args& a, const Tile& t, int i) {
-    token = (int)a.by_heads.div((uint32_t)i);
-    head = i - token * a.heads;
-    on = token < t.tokens && head < t.heads;
-    token += t.first, head += t.head;
-  }
-};
-struct Item {
-  Tile tile[2];
-  int g;             // key head
-  int q0, k0, n, m;  // the sequence: its first rows, query and key counts
-  int any;           // 0: there is no further item
-  int first_block;   // the first block of keys that this CTA works on
-  int all_units;     // tile 0's runs of keys, of which tile[0].units are this CTA's
-  __device__ __forceinline__ int blocks() const { return max(tile[0].blocks(), tile[1].blocks()); }
-};
-
-// The list of items, by the work of a pair's first tile: first those of at least
-// 2^(levels - 1) runs of keys, then of half as many, and so on, at the end the
-// rest (blocks take items as they come free, so the last ones should be short).
-// Within a level: sequences in order; in each the pairs of its tiles, the tiles
-// going from the last tokens to the first and through the group's heads, for
-// every key head.  A block's items come in nearly rising order, so the search goes
-// on from where the last one ended: 32 sequences at a time, a lane each.  (By the
-// machine's long division a step of it took 2 us: 80 prompts of 84 rows, 21 heads
-// over 7 of 64, 82 us.)
-struct Cursor {
-  int level = 0, chunk = 0;
-  uint32_t before = 0;  // items before this level's chunk; items are fewer than 2^31
-};
-
 // One warp: the first level that has items, from the longest sequence.
 __device__ int first_level(const Args& a) {
   int most = 0;
-  for (int b = threadIdx.x & 31; b < a.n_seq; b += 32) {
-    const int64_t k0 = clamp64(__ldg(a.cu_k + b), 0, a.total_k), k1 = clamp64(__ldg(a.cu_k + b + 1), k0, a.total_k);
-    most = max(most, (int)(k1 - k0));
-  }
-  most = (__reduce_max_sync(0xffffffffu, most) + UN - 1) / UN;
-  return a.levels - (32 - __clz(most));
-}
-
-// A lane's sequence of a chunk of 32, and its items of a level.
-struct Lot {
-  int q0, k0, n, m, blocks;
-  uint32_t above, mine;  // pairs (of a key head) of the levels before; items
-};
-
-// One warp: the items of a level's chunk.
-__device__ __forceinline__ uint32_t count_items(const Args& a, int level, int chunk, Lot& lot) {
-  const int b = chunk * 32 + (threadIdx.x & 31);
-  int q0 = 0, q1 = 0, k0 = 0, k1 = 0;
-  if (b < a.n_seq) {
-    const int most_q = (int)a.total_q, most_k = (int)a.total_k;
-    q0 = min(max(__ldg(a.cu_q + b), 0), most_q), q1 = min(max(__ldg(a.cu_q + b + 1), q0), most_q);
-    k0 = min(max(__ldg(a.cu_k + b), 0), most_k), k1 = min(max(__ldg(a.cu_k + b + 1), k0), most_k);
-  }
-  const int n = q1 - q0, m = k1 - k0, blocks = (int)a.by_tokens.div((uint32_t)(n + a.tokens - 1));
-  // pairs whose first tile sees at least `units` runs of keys
-  auto pairs = [&](int units) -> uint32_t {
-    uint32_t tiles = blocks;
-    if (units > 0) {
-      const int64_t end = (int64_t)(units - 1) * UN;  // its last row sees more keys than that
-      if (a.causal) {
-        const int64_t x = end - m + n;
-        tiles = x >= n ? 0 : blocks - (x > 0 ? (int)a.by_tokens.div((uint32_t)x) : 0);
-      } else if (m <= end) {
-        tiles = 0;
-      }
-    }
-    return (tiles * a.chunks + a.tiles - 1) >> (a.tiles - 1);  // by 1 or 2
-  };
-  const uint32_t above = level == 0 ? 0 : pairs(1 << (a.levels - level));
-  const uint32_t here = pairs(level == a.levels ? 0 : 1 << (a.levels - 1 - level)) - above;
-  lot = Lot{q0, k0, n, m, blocks, above, here * a.heads_kv};
-  return __reduce_add_sync(0xffffffffu, lot.mine);
+  for (int b = threadIdx.x & 31; b < a.n_seq; b += 32) most = max(most, keys_of(a, b));
+  return first_level_of(a, __reduce_max_sync(0xffffffffu, most));
 }
 
 // One warp: item i, or false behind the list's end.
-__device__ bool find_item(const Args& a, uint32_t item, Cursor& at, Item* out) {
-  const int lane = threadIdx.x & 31, chunks = (a.n_seq + 31) / 32;
+__device__ __forceinline__ bool find_item(const Args& a, uint32_t item, Cursor& at, Item* out) {
+  const int lane = threadIdx.x & 31;
   Lot lot;
-  // blocks taken over do not come quite in order
-  while (item < at.before) {
-    if (--at.chunk < 0) at.chunk = chunks - 1, --at.level;
-    at.before -= count_items(a, at.level, at.chunk, lot);
-  }
-  for (;;) {
-    if (at.level > a.levels) return false;
-    const uint32_t all = count_items(a, at.level, at.chunk, lot);
-    if (item - at.before < all) break;
-    at.before += all;
-    if (++at.chunk == chunks) at.chunk = 0, ++at.level;
-  }
+  if (!find_chunk(a, item, at, [&](int level, int chunk) {
+        lot = lot_of(a, level, chunk, lane);
+        return __reduce_add_sync(0xffffffffu, lot.mine);
+      }))
+    return false;
   uint32_t incl = lot.mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -278,27 +168,7 @@ __device__ bool find_item(const Args& a, uint32_t item, Cursor& at, Item* out) {
     if (lane >= o) incl += t;
   }
   const uint32_t x = item - at.before - (incl - lot.mine);  // huge where the item lies in a lane before
-  if (x < lot.mine) {
-    const uint32_t per_head = a.by_kv.div(x), pair = lot.above + per_head;
-    out->g = (int)(x - per_head * a.heads_kv);
-    out->q0 = lot.q0, out->k0 = lot.k0, out->n = lot.n, out->m = lot.m;
-    out->first_block = 0;
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const uint32_t e = pair * a.tiles + t;
-      Tile& tile = out->tile[t];
-      tile.head = -1, tile.heads = 0, tile.first = 0, tile.tokens = 0, tile.units = 0;
-      if (t >= a.tiles || e >= (uint32_t)(lot.blocks * a.chunks)) continue;
-      const int at_block = (int)a.by_chunks.div(e), chunk = (int)e - at_block * a.chunks;
-      tile.head = out->g * a.group + chunk * a.heads;
-      tile.heads = min(a.heads, a.group - chunk * a.heads);
-      tile.first = (lot.blocks - 1 - at_block) * a.tokens;
-      tile.tokens = min(a.tokens, lot.n - tile.first);
-      // one past the last key that its last token sees
-      const int64_t end = a.causal ? (int64_t)lot.m - lot.n + tile.first + tile.tokens : lot.m;
-      tile.units = end <= 0 ? 0 : (int)((end + UN - 1) / UN);
-    }
-  }
+  if (x < lot.mine) place_item(a, lot, x, out);
   return true;
 }
 
@@ -324,7 +194,7 @@ struct Ctl {
   alignas(16) uint8_t answer[16];
   uint32_t tmem;
   int abort;
-  unsigned beat;    // moves while rows are computed again
+  unsigned beat;    // moves while rows are computed again or blocks taken over
   unsigned odd[4];  // rows of a shared tile to look at again
   Item item[2];
 };
@@ -631,25 +501,34 @@ __device__ __forceinline__ void join_shares(const Args& a, Ctl* ctl, uint8_t* ri
     if (ctl->odd[row / 32] >> (row % 32) & 1u) look_again(a, it, tile, row, it.all_units, &ctl->beat);
 }
 
-// Behind the list's end every block is empty, up to as many as there are items:
-// one warp takes them over, each in less time than it takes to start one (1024
-// prompts of 64 rows, 32 heads over 8 of 128: 367 us, 1340 without this).
-__device__ __noinline__ void drain_blocks(Ctl* ctl, uint32_t answers) {
-  for (int block = 0; block >= 0; ++answers) {
+// Most blocks of the grid can lie behind the list's end, up to as many as there are
+// items: a warp that has got one of them takes over others, each in less time than it
+// takes to start one (1024 prompts of 64 rows, 32 heads over 8 of 128: 367 us, 1340
+// without this).  Returns the number of one that is on the list after all, its item
+// looked up from the start, or -1; and how many answers there were.
+__device__ __noinline__ int2 drain_blocks(const Args& a, Ctl* ctl, uint32_t items, uint32_t answers, Item* out) {
+  uint32_t n = 0;
+  const int block = next_listed(items, [&] {
     if ((threadIdx.x & 31) == 0) {
       uk_mbar_expect_tx(&ctl->next, 16);
       uk_next_block_ask(ctl->answer, &ctl->next);
+      if (n % 1024 == 0) atomicAdd(&ctl->beat, 1u);
     }
     __syncwarp();
     // this block's memory is not given up before the answer is there
-    if (!__all_sync(0xffffffffu, uk_mbar_wait(&ctl->next, answers & 1u, nullptr, WAIT_NS))) {
+    if (!__all_sync(0xffffffffu, uk_mbar_wait(&ctl->next, (answers + n) & 1u, nullptr, WAIT_NS))) {
       raise_fault(ctl, UK_FAULT_PRODUCER);
-      return;
+      return -1;
     }
-    block = uk_next_block(ctl->answer);
+    ++n;
+    const int got = uk_next_block(ctl->answer);
     uk_fence_proxy_async_smem();  // read before the next answer is written
     __syncwarp();
-  }
+    return got;
+  });
+  Cursor cursor;
+  if (block >= 0) find_item(a, (uint32_t)block, cursor, out);
+  return make_int2(block, (int)n);
 }
 
 // ---- items and loads, one warp ---------------------------------------------------------
@@ -669,6 +548,11 @@ __device__ __forceinline__ void load_items(const Args& a, Ctl* ctl, uint8_t* sme
     if (!(ok = wait_warp(ctl, &ctl->item_empty[turn & 1u], ((turn >> 1) & 1u) ^ 1u, UK_FAULT_PRODUCER))) break;
     // the first item was looked up before the barriers were up
     if (turn > 0) any = block >= 0 && find_item(a, (uint32_t)block, cursor, &it);
+    if (!kSplit && !any && block >= 0) {
+      const int2 next = drain_blocks(a, ctl, cursor.before, answers, &it);
+      block = next.x, answers += next.y;
+      any = block >= 0;
+    }
     __syncwarp();
     if (lane == 0) {
       it.any = any;
@@ -679,10 +563,7 @@ __device__ __forceinline__ void load_items(const Args& a, Ctl* ctl, uint8_t* sme
       }
     }
     __syncwarp();
-    if (!any) {
-      if (!kSplit && block >= 0) drain_blocks(ctl, answers);
-      break;
-    }
+    if (!any) break;
     asked = !kSplit;
     const int blocks = it.blocks();
     for (int j = 0; j < 2 * blocks && ok; ++j) {
@@ -960,8 +841,8 @@ __global__ void __launch_bounds__(256) k_attn_prompt_rows(const __grid_constant_
   const int h = (int)(w - t * a.heads_q);
   const int b = t < a.total_q ? uk_find_seq<true>(a.cu_q, a.n_seq, t) : -1;
   if (b < 0) return;
-  const int64_t q1 = clamp64(__ldg(a.cu_q + b + 1), 0, a.total_q);
-  const int64_t k0 = clamp64(__ldg(a.cu_k + b), 0, a.total_k), k1 = clamp64(__ldg(a.cu_k + b + 1), k0, a.total_k);
+  const int q1 = bound(a.cu_q, b + 1, 0, (int)a.total_q);
+  const int64_t k0 = bound(a.cu_k, b, 0, (int)a.total_k), k1 = k0 + keys_of(a, b);
   attend_row(a, t, h, k0, a.causal ? k1 - (q1 - 1 - t) : k1, nullptr);
 }
 
@@ -1091,7 +972,7 @@ extern "C" int uk_cuda_attn_prompt_f16(const uint16_t* Q, int64_t q_token_stride
     if (int rc = uk::check_device_ptr(LSE, "LSE")) return rc;
   Args a{Q, K, V, O, q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride,
          o_token_stride, o_head_stride, LSE, cu_q, cu_k, n_seq, heads_q, heads_kv, heads_q / heads_kv, dim, causal,
-         total_q, total_k, scale2, 0, 2, 1, 0, 0, 0, {}, {}, {}, {}};
+         total_q, total_k, scale2};
   // a zero scale: any factor that no score can raise above rounding does the same
   // and leaves hidden scores at -inf
   if (a.scale2 == 0.f) a.scale2 = 1e-30f;
@@ -1101,33 +982,7 @@ extern "C" int uk_cuda_attn_prompt_f16(const uint16_t* Q, int64_t q_token_stride
     k_attn_prompt_rows<<<(unsigned)blocks, 256, 0, (cudaStream_t)stream>>>(a);
     return uk::check_launch("attn_prompt");
   }
-  // the order of work: a level per power of two of the keys a tile can see; with
-  // many sequences every level is a long search, and the order matters less
-  if (n_seq <= 1024)
-    while ((total_k + UN - 1) / UN >> a.levels) ++a.levels;
-  const int64_t seqs = n_seq < total_q ? n_seq : total_q;
-  // the heads of a group in as few tiles as hold them, a tile's rows filled up with tokens
-  a.chunks = (a.group + BM - 1) / BM;
-  a.heads = (a.group + a.chunks - 1) / a.chunks;
-  a.tokens = BM / a.heads;
-  a.by_tokens = UkFastDiv::make(a.tokens), a.by_heads = UkFastDiv::make(a.heads);
-  a.by_chunks = UkFastDiv::make(a.chunks), a.by_kv = UkFastDiv::make(heads_kv);
-  // at most this many query blocks and pairs of tiles, whatever the lengths are
-  const int64_t most = (total_q + (a.tokens - 1) * seqs) / a.tokens, q_blocks = most < total_q ? most : total_q;
-  int64_t items = (q_blocks * a.chunks + seqs) / 2 * heads_kv;
-  // Few tiles: where all of them can run at once, a tile per block instead of a
-  // pair (one alone takes two thirds of a pair's time), and its keys shared by a
-  // cluster of 2, 4 or 8 blocks while the SMs last and every one keeps four blocks
-  // of keys on average.  One B200, 32 heads over 8 of 128: 512 rows 17.9 us in
-  // pairs, 14.6 in single tiles (1024 rows, 256 tiles: 25.2 against 26.8); 200 rows
-  // behind 8000 keys 124 us in pairs, 92 in single tiles, 60 shared by two.
-  const int64_t tiles = q_blocks * a.chunks * heads_kv;
-  if (tiles <= uk::sm_count()) {
-    a.tiles = 1, items = tiles;
-    const int64_t blocks = total_k / n_seq / BN;
-    while (a.split < 8 && tiles * a.split * 2 <= uk::sm_count() && blocks >= 8 * a.split) a.split *= 2;
-  }
-  // no fewer than items
-  if (tiles > 0x7fffffff) return uk::fail(UK_EINVAL, "attn_prompt: %lld tiles exceed the grid", (long long)tiles);
+  const int64_t items = plan_items(&a, uk::sm_count());
+  if (items < 0) return uk::fail(UK_EINVAL, "attn_prompt: more tiles than a grid has blocks");
   return dim > 64 ? launch<128>(a, items, (cudaStream_t)stream) : launch<64>(a, items, (cudaStream_t)stream);
 }
