@@ -418,6 +418,100 @@ def test_prompt_weak_tail():
     check_prompt(q, k, v, [0, n], [0, n], o, lse, dim ** -0.5, True)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("n,heads,m", [
+    (9600, 4, 1 << 18),  # pairs of tiles
+    (9600, 1, 1 << 18),  # a tile per block
+    (100, 1, 1 << 20),   # a tile's keys shared by a cluster
+])
+def test_prompt_sums_over_long_contexts(n, heads, m, dim):
+    """Values that do not cancel under weights that are nearly equal: a sum that
+    is rounded the same way at every step drifts."""
+    a = abi()
+    fault()
+    q, k = torch.zeros(n, heads, dim, device="cuda").half(), torch.zeros(m, heads, dim, device="cuda").half()
+    q[:, :, 0] = torch.linspace(0.01, 3, n, device="cuda").half()[:, None]
+    k[:, :, 0] = randn(m, heads, seed=1, mul=0.1)
+    k[0, :, 0] = 9.0  # the reference is this key's score: the others' weights are no powers of two
+    v = randn(m, heads, dim, seed=2).abs() + 0.5
+    o, lse = torch.full_like(q, math.nan), torch.full((n, heads), math.nan, device="cuda")
+    a.attn_prompt(q, k, v, i32([0, n]), i32([0, m]), o, lse=lse)
+    assert fault() == 0
+    assert torch.isfinite(o).all() and torch.isfinite(lse).all()
+    for r in (0, n // 2, n - 40):
+        rows, end = slice(r, r + 40), m - n + r + 40
+        for h in (0, heads - 1):
+            check_prompt(q[rows, h:h + 1], k[:end, h:h + 1], v[:end, h:h + 1], [0, 40], [0, end], o[rows, h:h + 1],
+                         lse[rows, h:h + 1], dim ** -0.5, True)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("heads,group,dim", [(8, 4, 128), (8, 4, 64), (6, 1, 96), (12, 3, 40)])
+def test_prompt_long_contexts_among_short_ones(heads, group, dim, causal):
+    """Tiles whose keys are taken in several parts, in one, and around the border
+    between them, in one list."""
+    a = abi()
+    fault()
+    nq = [300, 700, 40, 130, 0, 1200, 257]
+    nk = [300, 33000, 70000, 32768, 50, 1200, 32769]
+    cu_q, cu_k = [3 + c for c in prefix(nq)], [5 + c for c in prefix(nk)]
+    q = randn(cu_q[-1] + 7, heads * group, dim, seed=1)
+    kv = randn(cu_k[-1] + 130, 2 * heads, dim, seed=2)
+    kv[cu_k[-1]:] = math.nan
+    k, v = kv[:, :heads], kv[:, heads:]
+    o, lse = torch.full_like(q, 7.0), torch.full(q.shape[:2], 7.0, device="cuda")
+    a.attn_prompt(q, k, v, i32(cu_q), i32(cu_k), o, causal=causal, lse=lse)
+    assert fault() == 0
+    for x in (o, lse):
+        assert (x[:3] == 7).all() and (x[cu_q[-1]:] == 7).all()
+    for b, (n, m) in enumerate(zip(nq, nk)):
+        for h in (0, heads * group - 1):
+            for r in range(0, n, max(1, n - 60)):  # the first rows and the last ones
+                rows = slice(cu_q[b] + r, cu_q[b] + min(n, r + 60))
+                cnt = rows.stop - rows.start
+                end = m - n + r + cnt if causal else m
+                ks = slice(cu_k[b], cu_k[b] + end)
+                check_prompt(q[rows, h:h + 1], k[ks, h // group:h // group + 1], v[ks, h // group:h // group + 1],
+                             [0, cnt], [0, end], o[rows, h:h + 1], lse[rows, h:h + 1], dim ** -0.5, causal)
+    again = torch.full_like(q, 7.0)
+    a.attn_prompt(q, k, v, i32(cu_q), i32(cu_k), again, causal=causal)
+    assert same_bits(again, o)
+
+
+@pytest.mark.parametrize("heads,group,dim,n", [(8, 4, 128, 700), (8, 4, 64, 700), (1, 2, 128, 40)])
+def test_prompt_long_contexts_with_infinities_and_nan(heads, group, dim, n):
+    """In the first part, in the middle and behind the mask of all rows but the last."""
+    a = abi()
+    fault()
+    m = 70000
+    q, k, v = randn(n, heads * group, dim, seed=1), randn(m, heads, dim, seed=2), randn(m, heads, dim, seed=3)
+    v[3, 0, 1], v[40000, 0, 2], v[40001, 0, 3], v[m - 1, 0, 4] = math.inf, -math.inf, math.nan, math.nan
+    k[:, 0, :], q[:, :group] = k[:, 0, :].abs(), -q[:, :group].abs()
+    k[50000, 0, 0] = math.inf  # a score of -inf: no weight
+    o, lse = torch.full_like(q, 7.0), torch.full(q.shape[:2], 7.0, device="cuda")
+    a.attn_prompt(q, k, v, i32([0, n]), i32([0, m]), o, lse=lse)
+    assert fault() == 0
+    x = o[:, :group]
+    assert (x[..., 1] == math.inf).all() and (x[..., 2] == -math.inf).all() and torch.isnan(x[..., 3]).all()
+    assert torch.isfinite(x[:-1, :, 4]).all() and torch.isnan(x[-1, :, 4]).all()
+    assert torch.isfinite(lse).all() and torch.isfinite(x[..., 5:]).all() and torch.isfinite(o[:, group:]).all()
+    cols = [0] + list(range(4, dim))
+    sane = v.clone()
+    sane[[3, 40000, 40001], 0, 1:4] = 0.0
+    for r in (0, n - 30):
+        rows, end = slice(r, r + 29), m - n + r + 29
+        for h in (0, heads * group - 1):
+            g = h // group
+            qq, kk = q[rows, h].double(), k[:end, g].double()
+            kk[50000] = torch.where(torch.isinf(kk[50000]), torch.full_like(kk[50000], 1e6), kk[50000])
+            seen = torch.arange(end, device="cuda")[None] <= torch.arange(29, device="cuda")[:, None] + end - 29
+            ro, rl, to, _ = attention_f64(qq, kk, sane[:end, g], dim ** -0.5, seen)
+            kk[50000] = 0  # takes no part in the scores' bound
+            _, _, to, tl = attention_f64(qq, kk, sane[:end, g], dim ** -0.5, seen)
+            assert_close(o[rows, h][:, cols], ro[:, cols], to[:, cols], "rows from %d, head %d: o" % (r, h))
+            assert_close(lse[rows, h], rl, tl, "rows from %d, head %d: lse" % (r, h))
+
+
 def test_prompt_rows_do_not_see_behind_their_mask():
     """Infinities, NaN and the lowest value at later keys reach no earlier row;
     at keys that are seen they do."""

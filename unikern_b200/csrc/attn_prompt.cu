@@ -25,6 +25,12 @@
 // at 256 and 384.  A run's S is issued behind the product that reads the P in its
 // place, and the tensor core runs one thread's products in order.
 //
+// More than PART runs of keys are taken in parts, behind each of which the softmax
+// warps take out of O what it holds to 11 bits, O / l as binary16 (kept in the
+// row's place in the output), and leave the rest: the tensor core goes on adding to a
+// small number, and nothing is lost.  (The CTAs of a cluster share their rows: they
+// keep the sums in the unused tile's TMEM, in 32 bits, and leave zero.)
+//
 // What lies behind a row's mask: scores are replaced before the maximum, V rows
 // behind the sequence's last key are zeroed in shared memory (a zero weight
 // times a NaN would be one), and where a finite sum meets a row of O that is
@@ -135,6 +141,11 @@ __device__ __noinline__ void attend_row(const Args& a, int64_t t, int h, int64_t
 }
 
 // ---- what one CTA works on -----------------------------------------------------------
+// runs of keys whose products the tensor core adds up in one go: its sums are
+// truncated, 1e-7 of the sum for every 16 keys (2e-4 over 512 runs, 32768 keys; in one
+// go 8e-4 over 131072, 7e-3 over 2^20).  Calls of at most as many keys in all run
+// without the code for parts: 11 x 900 rows of dim 64 39.6 us, 41.1 with it.
+constexpr int PART = 512;
 constexpr float SHIFT = 7.f;       // weights are held as 2^7 * 2^(s - m): up to 2^15, binary16 ends at 2^16
 // three warpgroups: two of softmax, one of the MMA and load warps (and an idle
 // one).  They launch with 168 registers a thread; the softmax takes 216 (a row
@@ -231,7 +242,7 @@ __device__ __forceinline__ bool wait_warp(Ctl* ctl, uint64_t* bar, uint32_t pari
 }
 // ---- the softmax of a tile ------------------------------------------------------------
 // *turn: runs of 64 keys of this tile's slot that came before, even and odd ones;
-// *ends: items that had any.
+// *ends: parts of items.
 // One past the last key that a token of the sequence sees.
 __device__ __forceinline__ int end_of(const Args& a, const Item& it, int token) {
   const int64_t end = a.causal ? (int64_t)it.m - it.n + 1 + token : it.m;
@@ -266,7 +277,7 @@ struct Shared {
   __device__ __forceinline__ float* piece(int row, int c) const { return o + row * DP + (c ^ (row & 7)) * 4; }
 };
 
-template <int DP, bool kSplit>
+template <int DP, bool kSplit, bool kParts>
 __device__ __forceinline__ bool softmax_tile(const Args& a, Ctl* ctl, const Item& it, int t, uint32_t tmem,
                                              uint8_t* ring, uint32_t (&turn)[2], uint32_t* ends) {
   const Tile& tile = it.tile[t];
@@ -274,14 +285,17 @@ __device__ __forceinline__ bool softmax_tile(const Args& a, Ctl* ctl, const Item
   const int lane = threadIdx.x & 31, quad = (threadIdx.x >> 5) & 3;
   const int i = quad * 32 + lane;  // row of the tile
   const uint32_t lanes = (uint32_t)(quad * 32) << 16;
-  const uint32_t s_at = tmem + lanes + t * BN, o_at = tmem + lanes + 256 + t * 128;
+  const uint32_t s_at = tmem + lanes + t * BN, o_at = tmem + lanes + 256 + t * 128, sum_at = tmem + lanes + 384;
   const Row row(a, tile, i);
   // one past the last key that this row and that the tile's first token see
   const int end = end_of(a, it, row.token), clear = end_of(a, it, tile.first);
   const uint64_t scale2 = uk_f2(a.scale2, a.scale2);
   const int units = tile.units;
 
-  float m = -INFINITY, l = 0.f;
+  const int64_t token = (int64_t)it.q0 + row.token;
+  uint16_t* const own = row.on ? a.o + token * a.o_token + row.head * a.o_head : nullptr;
+  float m = -INFINITY, l = 0.f, lost = 0.f;  // lost: what the additions to l have rounded off (Kahan)
+  float part = 0.f;                          // what the numbers of the parts before are multiples of
   auto step = [&](int u, int h, uint32_t runs) {  // run u, of parity h; runs: of this tile's slot before it
     if (!wait_warp(ctl, &ctl->s_full[t][h], turn[h] & 1u, UK_FAULT_EPILOGUE)) return false;
     ++turn[h];
@@ -317,7 +331,8 @@ __device__ __forceinline__ bool softmax_tile(const Args& a, Ctl* ctl, const Item
       const float m2 = fmaxf(m, mt);
       const float f = m2 == -INFINITY ? 1.f : ex2(m - m2);
       m = m2;
-      l *= f;
+      l *= f, lost *= f;
+      if (kParts) part *= f;
       if (u > 0) {
         // the run before this one may still be on its way into O
         if (!wait_warp(ctl, &ctl->pv_done[t], (runs - 1) & 1u, UK_FAULT_EPILOGUE)) return false;
@@ -358,15 +373,79 @@ __device__ __forceinline__ bool softmax_tile(const Args& a, Ctl* ctl, const Item
     if (lane == 0) uk_mbar_arrive(&ctl->p_full[t][h]);
     float l0, l1;
     uk_f2_split(uk_f2_add(sum[0], sum[1]), &l0, &l1);
-    l += l0 + l1;
+    const float add = l0 + l1 - lost, sum_l = l + add;
+    lost = sum_l - l - add;
+    l = sum_l;
     return true;
   };
-  for (int u = 0; u < units; ++u)
-    if (!step(u, u & 1, turn[0] + turn[1])) return false;
+  // adds to 16 columns of O what was taken out of them
+  auto add_parts = [&](int c, uint32_t* o) {
+    uint32_t x[16];
+    if constexpr (kSplit) {
+      uk_tmem_ld16(sum_at + c * 16, x);
+      uk_tmem_ld_wait();
+    } else {
+      uint4 w[2] = {};
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        if (own != nullptr && c * 16 + k * 8 < a.dim) w[k] = reinterpret_cast<const uint4*>(own + c * 16)[k];
+      const uint32_t h[8] = {w[0].x, w[0].y, w[0].z, w[0].w, w[1].x, w[1].y, w[1].z, w[1].w};
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&h[k]));
+        x[2 * k] = __float_as_uint(y.x), x[2 * k + 1] = __float_as_uint(y.y);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(fmaf(__uint_as_float(x[k]), part, __uint_as_float(o[k])));
+  };
+  // behind a part, before run u
+  auto end_part = [&](int u) {
+    if (!wait_warp(ctl, &ctl->o_full[t], *ends & 1u, UK_FAULT_EPILOGUE)) return false;
+    uk_tc_fence_after();
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+#pragma unroll 1
+    for (int c = 0; c < DP / 16; ++c) {
+      uint32_t o[16];
+      uk_tmem_ld16(o_at + c * 16, o);
+      uk_tmem_ld_wait();
+      if (u > PART) add_parts(c, o);
+      if constexpr (kSplit) {
+        uk_tmem_st16(sum_at + c * 16, o);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) o[k] = 0;
+      } else {
+        uint32_t w[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          float x[2] = {__uint_as_float(o[2 * k]), __uint_as_float(o[2 * k + 1])};
+          w[k] = pack_half(fminf(fmaxf(x[0] * inv, -65504.f), 65504.f), fminf(fmaxf(x[1] * inv, -65504.f), 65504.f));
+          const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+          o[2 * k] = __float_as_uint(fmaf(-l, y.x, x[0])), o[2 * k + 1] = __float_as_uint(fmaf(-l, y.y, x[1]));
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          if (own != nullptr && c * 16 + k * 8 < a.dim)
+            reinterpret_cast<uint4*>(own + c * 16)[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+      }
+      uk_tmem_st16(o_at + c * 16, o);
+    }
+    part = kSplit ? 1.f : l;
+    uk_tmem_st_wait();
+    uk_tc_fence_before();
+    __syncwarp();
+    if (lane == 0) uk_mbar_arrive(&ctl->o_empty[t]);
+    ++*ends;
+    return true;
+  };
+  for (int u = 0; u < units;) {
+    if (kParts && u > 0 && !end_part(u)) return false;
+    for (const int stop = kParts ? min(u + PART, units) : units; u < stop; ++u)
+      if (!step(u, u & 1, turn[0] + turn[1])) return false;
+  }
 
   // ---- O / l, the log of the sum
   const bool mine = row.on;
-  const int64_t token = (int64_t)it.q0 + row.token;
   if (units > 0) {
     if (!wait_warp(ctl, &ctl->o_full[t], *ends & 1u, UK_FAULT_EPILOGUE)) return false;
     uk_tc_fence_after();
@@ -382,6 +461,7 @@ __device__ __forceinline__ bool softmax_tile(const Args& a, Ctl* ctl, const Item
       if (units > 0) {
         uk_tmem_ld32(o_at + c * 32, o);
         uk_tmem_ld_wait();
+        if (kParts && units > PART) add_parts(2 * c, o), add_parts(2 * c + 1, o + 16);
       }
 #pragma unroll
       for (int k = 0; k < 8; ++k)
@@ -397,10 +477,9 @@ __device__ __forceinline__ bool softmax_tile(const Args& a, Ctl* ctl, const Item
   // between their rows turns 32 lines touched by every store into 8 (the
   // store path takes a line per cycle: 2000 cycles a tile pair at dim 64).
   const int j4 = lane & 3;
-  const uint64_t own = mine ? (uint64_t)(a.o + token * a.o_token + row.head * a.o_head) : 0;
   uint16_t* out[4];  // of the group's four rows
 #pragma unroll
-  for (int k = 0; k < 4; ++k) out[k] = (uint16_t*)__shfl_sync(0xffffffffu, own, (lane & ~3) + k);
+  for (int k = 0; k < 4; ++k) out[k] = (uint16_t*)__shfl_sync(0xffffffffu, (uint64_t)own, (lane & ~3) + k);
 #pragma unroll
   for (int c = 0; c < DP / 32; ++c) {
     uint32_t w[4][4];
@@ -410,6 +489,7 @@ __device__ __forceinline__ bool softmax_tile(const Args& a, Ctl* ctl, const Item
       uint32_t o[32];
       uk_tmem_ld32(o_at + c * 32, o);
       uk_tmem_ld_wait();
+      if (kParts && units > PART) add_parts(2 * c, o), add_parts(2 * c + 1, o + 16);
 #pragma unroll
       for (int k = 0; k < 16; ++k) {
         const uint64_t v = uk_f2_fma(uk_f2(__uint_as_float(o[2 * k]), __uint_as_float(o[2 * k + 1])), inv2, zero2);
@@ -636,7 +716,7 @@ __device__ __forceinline__ void load_items(const Args& a, Ctl* ctl, uint8_t* sme
 // to be moved there).  The tensor core takes few products ahead, so while this
 // warp waits for the softmax it would run dry; the other tile's warp feeds it
 // then (one warp for both tiles left it idle 40 % of the time).
-template <int DP, bool kSplit>
+template <int DP, bool kSplit, bool kParts>
 __device__ __forceinline__ void issue_products(Ctl* ctl, int t, uint8_t* smem, uint8_t* ring, uint32_t tmem) {
   using S = Smem<DP>;
   constexpr uint32_t IDESC_S = uk_idesc_f16_ab(BM, UN, 0, 0), IDESC_O = uk_idesc_f16_ab(BM, DP, 0, 1);
@@ -652,7 +732,7 @@ __device__ __forceinline__ void issue_products(Ctl* ctl, int t, uint8_t* smem, u
   };
   auto commit = [&](uint64_t* bar) { uk_umma_commit_if(leader, bar); };
   uint32_t slot = 0, phase = 0;              // the ring's next block
-  uint32_t turn[2] = {0, 0}, ends = 0;       // even and odd runs, items of this tile so far
+  uint32_t turn[2] = {0, 0}, items = 0, ends = 0;  // of this tile so far: even and odd runs, items, parts of items
   auto next_slot = [&] {
     if (++slot == S::STAGES) slot = 0, phase ^= 1u;
   };
@@ -681,7 +761,8 @@ __device__ __forceinline__ void issue_products(Ctl* ctl, int t, uint8_t* smem, u
     // is there: an early return would stand for the other warp's.
     if (blocks > 0 && !(ok = wait(&ctl->kv_full[slot], phase))) break;
     if (own > 0) {  // the scores of the first block
-      if (!(ok = wait(&ctl->q_full[t], ends))) break;
+      if (!(ok = wait(&ctl->q_full[t], items))) break;
+      ++items;
       scores(0, slot);
       if (own > 1) scores(1, slot);
       if (own <= 2) commit(&ctl->q_empty[t]);
@@ -703,7 +784,7 @@ __device__ __forceinline__ void issue_products(Ctl* ctl, int t, uint8_t* smem, u
       for (int h = 0; h < 2; ++h) {
         const int u = 2 * j + h;
         if (!ok || u >= own) continue;
-        if (u == 0 && !(ok = wait(&ctl->o_empty[t], ends ^ 1u))) continue;
+        if ((kParts ? u % PART == 0 : u == 0) && !(ok = wait(&ctl->o_empty[t], ends ^ 1u))) continue;
         if (!(ok = wait(&ctl->p_full[t][h], turn[h]))) continue;
         ++turn[h];
 #pragma unroll
@@ -715,7 +796,7 @@ __device__ __forceinline__ void issue_products(Ctl* ctl, int t, uint8_t* smem, u
           scores(h, sk);
           if (u + 3 == own) commit(&ctl->q_empty[t]);
         }
-        if (u + 1 == own) {
+        if (u + 1 == own || (kParts && (u + 1) % PART == 0)) {
           commit(&ctl->o_full[t]);
           ++ends;
         }
@@ -733,8 +814,8 @@ __device__ __forceinline__ void issue_products(Ctl* ctl, int t, uint8_t* smem, u
 }
 
 // kSplit: a cluster of a.split CTAs per tile, each with a share of its keys, and
-// one tile per block (no next item).
-template <int DP, bool kSplit>
+// one tile per block (no next item).  kParts: tiles may see more than PART runs.
+template <int DP, bool kSplit, bool kParts>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
     k_attn_prompt(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                   const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ Args a) {
@@ -808,14 +889,14 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     for (uint32_t item = 0;; ++item) {
       if (!wait_warp(ctl, &ctl->item_full[item & 1u], (item >> 1) & 1u, UK_FAULT_EPILOGUE)) break;
       const Item& it = ctl->item[item & 1u];
-      if (!it.any || !softmax_tile<DP, kSplit>(a, ctl, it, warp >> 2, tmem, ring, turn, &ends) || kSplit) break;
+      if (!it.any || !softmax_tile<DP, kSplit, kParts>(a, ctl, it, warp >> 2, tmem, ring, turn, &ends) || kSplit) break;
       __syncwarp();
       if (lane == 0) uk_mbar_arrive(&ctl->item_empty[item & 1u]);
     }
   } else {
     uk_regs_down<REGS_OTHERS>();
     if (warp == LOAD_WARP) load_items<DP, kSplit>(a, ctl, smem, ring, tm_q, tm_k, tm_v, cursor, any);
-    else if (warp < MMA_WARP + 2) issue_products<DP, kSplit>(ctl, warp - MMA_WARP, smem, ring, tmem);
+    else if (warp < MMA_WARP + 2) issue_products<DP, kSplit, kParts>(ctl, warp - MMA_WARP, smem, ring, tmem);
   }
   __syncwarp();
   uk_tc_fence_before();
@@ -886,7 +967,7 @@ int make_map(CUtensorMap* m, const char* name, const uint16_t* base, int dim, in
   return UK_OK;
 }
 
-template <int DP>
+template <int DP, bool kSplit, bool kParts>
 int launch(const Args& a, int64_t items, cudaStream_t st) {
   CUtensorMap q, k, v;
   if (int rc = make_map(&q, "Q", a.q, a.dim, a.total_q, a.heads_q, a.q_token, a.q_head, a.tokens, a.heads)) return rc;
@@ -896,15 +977,13 @@ int launch(const Args& a, int64_t items, cudaStream_t st) {
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !attr_done[dev]) {
-    const int bytes = (int)Smem<DP>::BYTES;
-    cudaError_t e = cudaFuncSetAttribute(k_attn_prompt<DP, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(k_attn_prompt<DP, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    const cudaError_t e = cudaFuncSetAttribute(k_attn_prompt<DP, kSplit, kParts>,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Smem<DP>::BYTES);
     if (e != cudaSuccess) return uk::fail(UK_ECUDA, "attn_prompt: smem attribute: %s", cudaGetErrorString(e));
     if (dev >= 0 && dev < 64) attr_done[dev] = true;
   }
-  if (a.split == 1) {
-    k_attn_prompt<DP, false><<<(unsigned)items, NUM_THREADS, Smem<DP>::BYTES, st>>>(q, k, v, a);
+  if constexpr (!kSplit) {
+    k_attn_prompt<DP, false, kParts><<<(unsigned)items, NUM_THREADS, Smem<DP>::BYTES, st>>>(q, k, v, a);
     return uk::check_launch("attn_prompt");
   }
   cudaLaunchConfig_t cfg{};
@@ -919,12 +998,18 @@ int launch(const Args& a, int64_t items, cudaStream_t st) {
   attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, k_attn_prompt<DP, true>, q, k, v, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, k_attn_prompt<DP, kSplit, kParts>, q, k, v, a);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return uk::fail(UK_ECUDA, "attn_prompt: %s", cudaGetErrorString(e));
   }
   return UK_OK;
+}
+
+template <int DP>
+int launch(const Args& a, int64_t items, cudaStream_t st) {
+  if (a.total_k > PART * UN) return a.split > 1 ? launch<DP, true, true>(a, items, st) : launch<DP, false, true>(a, items, st);
+  return a.split > 1 ? launch<DP, true, false>(a, items, st) : launch<DP, false, false>(a, items, st);
 }
 
 }  // namespace
