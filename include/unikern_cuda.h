@@ -320,7 +320,10 @@ int uk_cuda_decode_rmsnorm_gemm_f16(const float* X, const float* gamma, float ep
  *               is within [-24, 15].
  * Any page_size >= 1; dim a multiple of 8 (e4m3: of 16) from 8 to 128; pools
  * 16-byte aligned, strides multiples of 16 bytes; max_pages * page_size below
- * 2^31 - 4096; up to 2^24 sequences in a call.
+ * 2^31 - 4096; up to 2^24 sequences in a call.  uk_cuda_attn_decode_f16 refuses
+ * pools that span 2^32 - 1 times the largest power of two, up to 4096 bytes, which
+ * divides all strides (16-byte units: 64 GiB), but takes UK_KV_F16 pools with a
+ * page_size that is a multiple of 16 up to 4 TiB.
  * Page ids and lengths are device memory and are not trusted: a page id outside
  * the pool or a position beyond max_pages pages is treated as absent (nothing is
  * written there; it reads as zeros; attention does not see it) and sets bit 64

@@ -309,6 +309,37 @@ def test_decode_offsets_past_32_bits(kind, page):
     assert rc == 2
 
 
+@pytest.mark.parametrize("kind,page,taken", [("f16", 16, True), ("f16", 48, True), ("f16", 8, False),
+                                             ("e4m3", 16, False)])
+def test_decode_pools_of_small_units(kind, page, taken):
+    """A pool of more than 2^32 of the units that its strides have in common: the
+    form that finds groups of 16 positions by 64-bit offsets takes it.  (Only the
+    pages that the table names exist.)"""
+    a = abi()
+    dim, heads, n = 24 if kind == "f16" else 48, 3, 100
+    pool = Pool(kind, "hnd", heads, dim, page, [n], seed=1)
+    q = randn(1, heads * 2, dim, seed=2)
+    o, lse = torch.empty_like(q), torch.empty(1, heads * 2, device="cuda")
+    far = a.KvCacheStruct(*[getattr(pool.cache.struct, f[0]) for f in a.KvCacheStruct._fields_])
+    far.pages = (1 << 36) // (far.page_stride * (2 if kind == "f16" else 1)) + 2
+    ws = a.attn_decode_workspace(pool.cache, heads * 2)
+    t = pool.table
+    rc = a.lib().uk_cuda_attn_decode_f16(q.data_ptr(), q.stride(0), q.stride(1), ctypes.byref(far), t.data_ptr(),
+                                         t.stride(0), t.shape[1], pool.lens_t.data_ptr(), 1, heads * 2, dim ** -0.5,
+                                         o.data_ptr(), o.stride(0), o.stride(1), lse.data_ptr(), ws.data_ptr(),
+                                         ws.numel(), None)
+    assert rc == (0 if taken else 2)
+    if taken:
+        check_decode(pool, q, o, lse, dim ** -0.5)
+    # strides whose extent does not even fit 64 bits
+    far.page_stride = 1 << 60
+    rc = a.lib().uk_cuda_attn_decode_f16(q.data_ptr(), q.stride(0), q.stride(1), ctypes.byref(far), t.data_ptr(),
+                                         t.stride(0), t.shape[1], pool.lens_t.data_ptr(), 1, heads * 2, dim ** -0.5,
+                                         o.data_ptr(), o.stride(0), o.stride(1), lse.data_ptr(), ws.data_ptr(),
+                                         ws.numel(), None)
+    assert rc == 2
+
+
 # ---- packed prompts -------------------------------------------------------------------
 
 def check_prompt(q, k, v, cu_q, cu_k, o, lse, scale, causal):

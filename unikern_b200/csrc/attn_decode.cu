@@ -922,10 +922,13 @@ int launch(const Args& a, const UkKvView& c, int ctas, cudaStream_t st) {
   return launch_join<DP, NH>(a, c.dim, ctas, st);
 }
 
+// every group of 16 positions in one page (kWhole)
+bool whole_groups(const UkKvView& c) { return c.kind == UK_KV_F16 && c.page_size % 16 == 0; }
+
 template <int KIND, int DP, int NH>
 int launch(const Args& a, const UkKvView& c, int ctas, cudaStream_t st) {
   if constexpr (KIND == UK_KV_F16)
-    if (c.page_size % 16 == 0) return launch<KIND, DP, NH, true>(a, c, ctas, st);
+    if (whole_groups(c)) return launch<KIND, DP, NH, true>(a, c, ctas, st);
   return launch<KIND, DP, NH, false>(a, c, ctas, st);
 }
 
@@ -982,10 +985,13 @@ extern "C" int uk_cuda_attn_decode_f16(const uint16_t* Q, int64_t q_seq_stride, 
   if (c.page_size > 1) strides |= c.token_bytes;
   if (c.heads > 1) strides |= c.head_bytes;
   a.unit = (int)(strides & -strides);
-  const int64_t far = (c.pages - 1) * c.page_bytes + (c.page_size - 1) * c.token_bytes + (c.heads - 1) * c.head_bytes;
-  if (c.pages > 0 && far / a.unit >= 0xffffffffll)
-    return uk::fail(UK_EINVAL, "attn_decode: a pool of %lld bytes with strides of multiples of %d bytes only",
-                    (long long)far, a.unit);
+  // (in 128 bits: nothing bounds the strides).  Whole groups go by 64-bit offsets:
+  // there the limit only catches strides that cannot be meant, 4 TiB from end to end.
+  const __int128 far = (__int128)(c.pages - 1) * c.page_bytes + (__int128)(c.page_size - 1) * c.token_bytes +
+                       (__int128)(c.heads - 1) * c.head_bytes;
+  if (c.pages > 0 && far / a.unit >= 0xffffffffll && (!whole_groups(c) || far >= (__int128)1 << 42))
+    return uk::fail(UK_EINVAL, "attn_decode: a pool of %.3g bytes with strides of multiples of %d bytes only",
+                    (double)far, a.unit);
   a.parts = reinterpret_cast<float*>(a.recs + ctas);
   const cudaStream_t st = (cudaStream_t)stream;
   switch ((cache->kind == UK_KV_E4M3 ? 4 : 0) + (dp == 128 ? 2 : 0) + (nh - 1)) {
