@@ -146,6 +146,44 @@ def test_decode_long(kind):
     check_decode(pool, q, o, lse, dim ** -0.5)
 
 
+@pytest.mark.parametrize("kind,page,heads,group,dim,seqs,n", [
+    ("f16", 64, 8, 4, 16, 64, 1 << 20), ("e4m3", 64, 8, 4, 16, 64, 1 << 20), ("f16", 40, 2, 12, 64, 230, 150001),
+    ("e4m3", 32, 2, 20, 128, 230, 140000), ("f16", 16, 8, 1, 128, 56, 200000)])
+def test_decode_sums_over_long_contexts(kind, page, heads, group, dim, seqs, n):
+    """So many long sequences that a block sums whole ones up (all of them in the
+    same pages), some shorter ones between them; values that do not cancel under
+    weights that are nearly equal: a sum that is rounded the same way at every step
+    drifts."""
+    a = abi()
+    fault()
+    pool = Pool(kind, "hnd", heads, dim, page, [n], seed=1, fill=False)
+    k = torch.zeros(n, heads, dim, device="cuda")
+    k[:, :, 0] = randn(n, heads, seed=1, mul=0.1)
+    k[0, :, 0] = 9.0
+    k, v = pool.put(0, 0, 0, k.half()), pool.put(1, 0, 0, randn(n, heads, dim, seed=2).abs() + 0.5)
+    lens = [n] * seqs
+    lens[3:9] = [70000, 0, 32768, 32769, 5, 98305]
+    lens[-2] = 65536
+    q = torch.zeros(seqs, heads * group, dim, device="cuda").half()
+    q[:, :, 0] = torch.linspace(0.01, 3, seqs, device="cuda").half()[:, None]
+    o, lse = torch.full_like(q, math.nan), torch.full(q.shape[:2], math.nan, device="cuda")
+    table = pool.table.repeat(seqs, 1)
+    a.attn_decode(q, pool.cache, table, i32(lens), o, lse=lse)
+    assert fault() == 0
+    assert torch.isfinite(o).all() and torch.isfinite(lse[[b for b in range(seqs) if lens[b]]]).all()
+    for b in [0, 1, 3, 4, 5, 6, 7, 8, seqs // 2, seqs - 3, seqs - 2, seqs - 1]:
+        m = lens[b]
+        for g in (0, heads - 1):
+            rows = slice(g * group, (g + 1) * group)
+            seen = torch.ones(group, m, dtype=torch.bool, device="cuda")
+            ro, rl, to, tl = attention_f64(q[b, rows], k[:m, g], v[:m, g], dim ** -0.5, seen)
+            assert_close(o[b, rows], ro, to, "sequence %d heads of %d: o" % (b, g))
+            assert_close(lse[b, rows], rl, tl, "sequence %d heads of %d: lse" % (b, g))
+    again = torch.full_like(q, math.nan)
+    a.attn_decode(q, pool.cache, table, i32(lens), again)
+    assert same_bits(again, o)
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.3, 1.0, 40.0])
 def test_decode_scales(scale):
     """Uniform weights, negative scales, and scores of some hundreds that rise

@@ -52,6 +52,9 @@ constexpr int WARPS = 4, THREADS = WARPS * 32;
 constexpr int MAX_CTAS = 1024;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float GROW = 8.f;   // scores may pass the reference by 2^8 before it moves
+// positions that are summed up in one go: the tensor core's sums are truncated, and l
+// is a plain one (one sequence of 2^20 positions per CTA in one go: 1e-3 too small)
+constexpr int PART = 1 << 15;
 constexpr float SHIFT = 7.f;  // weights are held as 2^7 * 2^(s - m): up to 2^15, binary16 ends at 2^16
 
 struct Args {
@@ -64,7 +67,7 @@ struct Args {
   int n_seq, heads_q, group;  // group = query heads per key head
   int chunks;                 // runs of 8 NH query heads per key head
   float scale2;               // scale * log2 e
-  float* parts;               // [ctas][2][part_floats]
+  float* parts;               // [ctas][2][part_floats]; also holds a pair's sum between its PARTs
   // a pair cut by the end of its first CTA's run: {b, pair, first CTA, last
   // CTA}, b = -1: none; one per pair where there are no more pairs than CTAs
   // (by_pair), else one per CTA
@@ -222,6 +225,7 @@ __global__ void __launch_bounds__(THREADS, NH == 1 ? 3 : 2) k_attn_decode(Args a
   constexpr int CT = S::CT, WT = S::WT, NT = S::NT;
   __shared__ float sm_m[WARPS][8 * NH], sm_l[WARPS][8 * NH];
   __shared__ __align__(16) float sm_o[WARPS][8 * NH][DP + 2];
+  __shared__ float part_m[2][8 * NH], part_l[2][8 * NH];  // of the PARTs of a pair so far; by turns
   __shared__ float sum_m[kCluster ? 8 * NH : 1], sum_l[kCluster ? 8 * NH : 1];  // of this CTA's four warps
   __shared__ __align__(16) float sum_o[kCluster ? 8 * NH : 1][kCluster ? DP : 4];
 
@@ -272,11 +276,13 @@ __global__ void __launch_bounds__(THREADS, NH == 1 ? 3 : 2) k_attn_decode(Args a
   }
 
   int64_t x = x0;
+  int turn = 0;
   for (bool more = true; more;) {
     // the place of the pair's first tile, and its tiles here
     const int64_t start = kCluster ? 0 : before * pairs + (int64_t)pair * (nt + START) + START;
-    const int t0 = x > start ? (int)(x - start) : 0, t1 = (int)min((int64_t)nt, x1 - start);
-    if (!kCluster && t1 <= t0) break;  // only places in front of it
+    const int t0 = x > start ? (int)(x - start) : 0, end = (int)min((int64_t)nt, x1 - start);
+    if (!kCluster && end <= t0) break;  // only places in front of it
+    const int t1 = kCluster ? end : min(end, t0 + PART / CT);  // the rest follows in the next turn
     const int g = pair / a.chunks, h0 = g * a.group + (pair % a.chunks) * 8 * NH;
     const int heads = min(8 * NH, (g + 1) * a.group - h0);  // query heads of this run
 
@@ -628,7 +634,8 @@ __global__ void __launch_bounds__(THREADS, NH == 1 ? 3 : 2) k_attn_decode(Args a
         }
       }
     __syncthreads();
-    const bool entered = t0 > 0, leaves = t1 < nt;
+    const bool entered = x0 > start, leaves = end < nt;
+    const bool goes_on = t1 < end, went_on = t0 > 0 && x > x0;  // the pair's PARTs here behind and before this one
     float* part = a.parts + ((int64_t)blockIdx.x * 2 + (entered ? 0 : 1)) * part_floats(DP, NH);
     constexpr int LANES = DP / 8;  // threads per head, 8 values each
     for (int i = threadIdx.x; i < heads * LANES; i += THREADS) {
@@ -647,12 +654,23 @@ __global__ void __launch_bounds__(THREADS, NH == 1 ? 3 : 2) k_attn_decode(Args a
 #pragma unroll
         for (int k = 0; k < 8; ++k) o[k] += sm_o[w][head][d + k] * f;
       }
+      if (!kCluster && went_on) {  // what this thread left of the PARTs before
+        const float m0 = part_m[turn][head], m2 = fmaxf(mm, m0);
+        const float f = mm == m2 ? 1.f : ex2(mm - m2), f0 = m0 == m2 ? 1.f : ex2(m0 - m2);
+        const float4* src = reinterpret_cast<const float4*>(part + 16 * NH + head * DP + d);
+        const float4 u = src[0], v = src[1];
+        mm = m2, ll = ll * f + part_l[turn][head] * f0;
+        o[0] = o[0] * f + u.x * f0, o[1] = o[1] * f + u.y * f0, o[2] = o[2] * f + u.z * f0, o[3] = o[3] * f + u.w * f0;
+        o[4] = o[4] * f + v.x * f0, o[5] = o[5] * f + v.y * f0, o[6] = o[6] * f + v.z * f0, o[7] = o[7] * f + v.w * f0;
+      }
       if (kCluster) {
         if (d == 0) sum_m[head] = mm, sum_l[head] = ll;
         *reinterpret_cast<float4*>(&sum_o[head][d]) = make_float4(o[0], o[1], o[2], o[3]);
         *reinterpret_cast<float4*>(&sum_o[head][d + 4]) = make_float4(o[4], o[5], o[6], o[7]);
-      } else if (entered || leaves) {
-        if (d == 0) {
+      } else if (entered || leaves || goes_on) {
+        if (d == 0 && goes_on) {
+          part_m[turn ^ 1][head] = mm, part_l[turn ^ 1][head] = ll;
+        } else if (d == 0) {
           part[head] = mm;
           part[8 * NH + head] = ll;
         }
@@ -703,7 +721,8 @@ __global__ void __launch_bounds__(THREADS, NH == 1 ? 3 : 2) k_attn_decode(Args a
       uk_cluster_sync();  // no CTA leaves while another reads its shared memory
       return;
     }
-    if (!entered) {
+    turn ^= 1;
+    if (!entered && !goes_on) {
       if (leaves) rec = make_int4(b, pair, blockIdx.x, (int)line.owner(start + nt - 1));
       if (a.by_pair && threadIdx.x == 0) a.recs[b * pairs + pair] = leaves ? rec : make_int4(-1, 0, 0, 0);
     }
@@ -711,7 +730,7 @@ __global__ void __launch_bounds__(THREADS, NH == 1 ? 3 : 2) k_attn_decode(Args a
 
     x = start + t1;
     more = x < x1;
-    if (more && ++pair == pairs) {
+    if (more && !goes_on && ++pair == pairs) {
       pair = 0;
       before += nt + START;
       do {
