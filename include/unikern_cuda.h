@@ -379,7 +379,8 @@ int uk_cuda_kv_gather_f16(const uk_kv_cache* cache, const int32_t* block_table, 
  * heads_q up to 65535.  O overlaps neither Q nor the cache.
  * Scores, softmax statistics and sums are fp32; the softmax weights enter the
  * value product as binary16, one rounding into O.  A NaN or an infinity among
- * the values seen makes that column's outputs NaN or infinite.
+ * the values seen makes that column's outputs NaN or infinite; an average of
+ * finite values is finite (65504 where the roundings lead above it).
  * Deterministic.  The workspace (its size depends on the current device, the
  * heads and dim, not on lengths or n_seq) may be reused by later calls on the
  * same stream; calls that can overlap need one each. */

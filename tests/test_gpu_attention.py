@@ -675,6 +675,53 @@ def test_prompt_long():
     check_prompt(q, k, v, [0, n], [0, n], o, lse, dim ** -0.5, True)
 
 
+@pytest.mark.parametrize("n,heads,group,dim,m", [(700, 8, 4, 128, 900), (300, 2, 3, 64, 700), (40, 1, 4, 64, 5000),
+                                                 (700, 8, 4, 64, 40000), (20, 2, 4, 64, 600)])
+def test_prompt_averages_of_the_largest_values(n, heads, group, dim, m):
+    """Columns that hold 65504 at every key, seen with weights that round up: the
+    average does not become an infinity.  (Scores 3 bits above the reference.)"""
+    a = abi()
+    fault()
+    q, k = torch.zeros(n, heads * group, dim, device="cuda").half(), torch.zeros(m, heads, dim, device="cuda").half()
+    q[:, :, 0] = 1.0 + randn(n, heads * group, seed=1, mul=0.1).abs()
+    k[128:, :, 0] = 3.0 * math.log(2) * math.sqrt(dim)
+    v = randn(m, heads, dim, seed=2)
+    v[:, :, 0], v[:, :, 1], v[:, :, 8] = 65504.0, -65504.0, 65504.0
+    for scale in (dim ** -0.5, -dim ** -0.5):
+        o, lse = torch.empty_like(q), torch.empty(n, heads * group, device="cuda")
+        a.attn_prompt(q, k, v, i32([0, n]), i32([0, m]), o, scale=scale, lse=lse)
+        assert torch.isfinite(o).all()
+        rows = slice(n - 20, n)
+        check_prompt(q[rows], k, v, [0, 20], [0, m], o[rows], lse[rows], scale, True)
+
+
+@pytest.mark.parametrize("n,page", [(900, 16), (900, 5), (20000, 16)])
+def test_decode_averages_of_the_largest_values(n, page):
+    """The same over a cache, whole sequences and ones cut in parts."""
+    a = abi()
+    heads, group, dim, seqs = 2, 16, 64, 40
+    pool = Pool("f16", "hnd", heads, dim, page, [n], seed=1, fill=False)
+    k = torch.zeros(n, heads, dim, device="cuda")
+    k[256:, :, 0] = 3.0 * math.log(2) * math.sqrt(dim)
+    v = randn(n, heads, dim, seed=2)
+    v[:, :, 0], v[:, :, 1], v[:, :, 8] = 65504.0, -65504.0, 65504.0
+    k, v = pool.put(0, 0, 0, k.half()), pool.put(1, 0, 0, v)
+    for count in (1, seqs):
+        q = torch.zeros(count, heads * group, dim, device="cuda").half()
+        q[:, :, 0] = 1.0 + randn(count, heads * group, seed=1, mul=0.1).abs()
+        for table in both_splits(pool):
+            o, lse = torch.empty_like(q), torch.empty(q.shape[:2], device="cuda")
+            a.attn_decode(q, pool.cache, table.repeat(count, 1), i32([n] * count), o, lse=lse)
+            assert torch.isfinite(o).all()
+            seen = torch.ones(group, n, dtype=torch.bool, device="cuda")
+            for b in (0, count - 1):
+                for g in range(heads):
+                    rows = slice(g * group, (g + 1) * group)
+                    ro, rl, to, tl = attention_f64(q[b, rows], k[:, g], v[:, g], dim ** -0.5, seen)
+                    assert_close(o[b, rows], ro, to, "sequence %d heads of %d: o" % (b, g))
+                    assert_close(lse[b, rows], rl, tl, "sequence %d heads of %d: lse" % (b, g))
+
+
 # ---- together -------------------------------------------------------------------------
 
 @pytest.mark.parametrize("kind", ["f16", "e4m3"])

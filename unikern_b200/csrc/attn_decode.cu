@@ -681,8 +681,8 @@ __global__ void __launch_bounds__(THREADS, NH == 1 ? 3 : 2) k_attn_decode(Args a
         const float inv = ll == 0.f ? 0.f : 1.f / ll;
         if (d < c.dim)
           *reinterpret_cast<uint4*>(a.o + b * a.o_seq + (int64_t)(h0 + head) * a.o_head + d) =
-              make_uint4(pack_half(o[0] * inv, o[1] * inv), pack_half(o[2] * inv, o[3] * inv),
-                         pack_half(o[4] * inv, o[5] * inv), pack_half(o[6] * inv, o[7] * inv));
+              make_uint4(uk_pack_average(o[0] * inv, o[1] * inv), uk_pack_average(o[2] * inv, o[3] * inv),
+                         uk_pack_average(o[4] * inv, o[5] * inv), uk_pack_average(o[6] * inv, o[7] * inv));
         if (a.lse != nullptr && d == 0)
           a.lse[(int64_t)b * a.heads_q + h0 + head] = ll == 0.f ? -INFINITY : (mm - SHIFT + log2f(ll)) * LN2;
       }
@@ -713,8 +713,8 @@ __global__ void __launch_bounds__(THREADS, NH == 1 ? 3 : 2) k_attn_decode(Args a
         const float inv = ll == 0.f ? 0.f : 1.f / ll;
         if (d < c.dim)
           *reinterpret_cast<uint4*>(a.o + b * a.o_seq + (int64_t)(h0 + head) * a.o_head + d) =
-              make_uint4(pack_half(o[0] * inv, o[1] * inv), pack_half(o[2] * inv, o[3] * inv),
-                         pack_half(o[4] * inv, o[5] * inv), pack_half(o[6] * inv, o[7] * inv));
+              make_uint4(uk_pack_average(o[0] * inv, o[1] * inv), uk_pack_average(o[2] * inv, o[3] * inv),
+                         uk_pack_average(o[4] * inv, o[5] * inv), uk_pack_average(o[6] * inv, o[7] * inv));
         if (a.lse != nullptr && d == 0)
           a.lse[(int64_t)b * a.heads_q + h0 + head] = ll == 0.f ? -INFINITY : (mm - SHIFT + log2f(ll)) * LN2;
       }
@@ -798,7 +798,7 @@ __global__ void __launch_bounds__(256) k_attn_join_few(Args a, int dim) {
   const float inv = l == 0.f ? 0.f : 1.f / l;
   if (d4 * 4 < dim)
     reinterpret_cast<uint2*>(a.o + b * a.o_seq + (int64_t)h * a.o_head)[d4] =
-        make_uint2(pack_half(o.x * inv, o.y * inv), pack_half(o.z * inv, o.w * inv));
+        make_uint2(uk_pack_average(o.x * inv, o.y * inv), uk_pack_average(o.z * inv, o.w * inv));
   if (a.lse != nullptr && d4 == 0)
     a.lse[(int64_t)b * a.heads_q + h] = l == 0.f ? -INFINITY : (m - SHIFT + log2f(l)) * LN2;
 }
@@ -853,7 +853,7 @@ __global__ void __launch_bounds__(512) k_attn_join_many(Args a, int dim) {
     const float inv = ll == 0.f ? 0.f : 1.f / ll;
     if (d4 * 4 < dim)
       reinterpret_cast<uint2*>(a.o + b * a.o_seq + (int64_t)h * a.o_head)[d4] =
-          make_uint2(pack_half(o.x * inv, o.y * inv), pack_half(o.z * inv, o.w * inv));
+          make_uint2(uk_pack_average(o.x * inv, o.y * inv), uk_pack_average(o.z * inv, o.w * inv));
     if (a.lse != nullptr && d4 == 0)
       a.lse[(int64_t)b * a.heads_q + h] = ll == 0.f ? -INFINITY : (mm - SHIFT + log2f(ll)) * LN2;
   }

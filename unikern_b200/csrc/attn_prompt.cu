@@ -136,7 +136,7 @@ __device__ __noinline__ void attend_row(const Args& a, int64_t t, int h, int64_t
   const float inv = l.s == 0.f ? 0.f : 1.f / l.s;
   if (lane * 4 < a.dim)
     reinterpret_cast<uint2*>(a.o + t * a.o_token + h * a.o_head)[lane] =
-        make_uint2(pack_half(o[0].s * inv, o[1].s * inv), pack_half(o[2].s * inv, o[3].s * inv));
+        make_uint2(uk_pack_average(o[0].s * inv, o[1].s * inv), uk_pack_average(o[2].s * inv, o[3].s * inv));
   if (a.lse != nullptr && lane == 0) a.lse[t * a.heads_q + h] = l.s == 0.f ? -INFINITY : (m + log2f(l.s)) * LN2;
 }
 
@@ -277,6 +277,48 @@ struct Shared {
   __device__ __forceinline__ float* piece(int row, int c) const { return o + row * DP + (c ^ (row & 7)) * 4; }
 };
 
+// 16 values of a row of the output, as far as `left` of it go; zeros without a row
+__device__ __forceinline__ void load_halves(const uint16_t* row, int left, uint32_t (&x)[16]) {
+  uint4 w[2] = {};
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    if (k * 8 < left) w[k] = reinterpret_cast<const uint4*>(row)[k];
+  const uint32_t h[8] = {w[0].x, w[0].y, w[0].z, w[0].w, w[1].x, w[1].y, w[1].z, w[1].w};
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&h[k]));
+    x[2 * k] = __float_as_uint(y.x), x[2 * k + 1] = __float_as_uint(y.y);
+  }
+}
+
+// A warp's rows of O times inv, each stored by its own thread: where they were taken
+// out in parts (part: what the halves that lie in `own` are multiples of), and where a
+// value is not finite.  True where that is so.
+template <int DP>
+__device__ __noinline__ bool store_own(uint32_t o_at, float inv, uint16_t* own, float part, int dim) {
+  float odd = 0.f;
+#pragma unroll 1
+  for (int c = 0; c < DP / 16; ++c) {
+    uint32_t o[16], x[16], w[8];
+    uk_tmem_ld16(o_at + c * 16, o);
+    const int left = own != nullptr ? dim - c * 16 : 0;
+    load_halves(own + c * 16, part != 0.f ? left : 0, x);
+    uk_tmem_ld_wait();
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float y0 = fmaf(__uint_as_float(x[2 * k]), part, __uint_as_float(o[2 * k])) * inv;
+      const float y1 = fmaf(__uint_as_float(x[2 * k + 1]), part, __uint_as_float(o[2 * k + 1])) * inv;
+      odd = fmaf(y0, 0.f, fmaf(y1, 0.f, odd));
+      w[k] = uk_pack_average(y0, y1);
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if (k * 8 < left)
+        reinterpret_cast<uint4*>(own + c * 16)[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+  }
+  return odd != 0.f;
+}
+
 template <int DP, bool kSplit, bool kParts>
 __device__ __forceinline__ bool softmax_tile(const Args& a, Ctl* ctl, const Item& it, int t, uint32_t tmem,
                                              uint8_t* ring, uint32_t (&turn)[2], uint32_t* ends) {
@@ -385,16 +427,7 @@ __device__ __forceinline__ bool softmax_tile(const Args& a, Ctl* ctl, const Item
       uk_tmem_ld16(sum_at + c * 16, x);
       uk_tmem_ld_wait();
     } else {
-      uint4 w[2] = {};
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-        if (own != nullptr && c * 16 + k * 8 < a.dim) w[k] = reinterpret_cast<const uint4*>(own + c * 16)[k];
-      const uint32_t h[8] = {w[0].x, w[0].y, w[0].z, w[0].w, w[1].x, w[1].y, w[1].z, w[1].w};
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&h[k]));
-        x[2 * k] = __float_as_uint(y.x), x[2 * k + 1] = __float_as_uint(y.y);
-      }
+      load_halves(own + c * 16, own != nullptr ? a.dim - c * 16 : 0, x);
     }
 #pragma unroll
     for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(fmaf(__uint_as_float(x[k]), part, __uint_as_float(o[k])));
@@ -419,7 +452,7 @@ __device__ __forceinline__ bool softmax_tile(const Args& a, Ctl* ctl, const Item
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           float x[2] = {__uint_as_float(o[2 * k]), __uint_as_float(o[2 * k + 1])};
-          w[k] = pack_half(fminf(fmaxf(x[0] * inv, -65504.f), 65504.f), fminf(fmaxf(x[1] * inv, -65504.f), 65504.f));
+          w[k] = uk_pack_finite(x[0] * inv, x[1] * inv);  // an infinity or a NaN stays in the rest
           const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
           o[2 * k] = __float_as_uint(fmaf(-l, y.x, x[0])), o[2 * k + 1] = __float_as_uint(fmaf(-l, y.y, x[1]));
         }
@@ -472,50 +505,62 @@ __device__ __forceinline__ bool softmax_tile(const Args& a, Ctl* ctl, const Item
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const uint64_t inv2 = uk_f2(inv, inv), zero2 = uk_f2(0.f, 0.f);
-  uint64_t odd2 = zero2;  // NaN once a value of the row is not finite
-  // Stores go by groups of four lanes: a 4 x 4 transpose of 16-byte pieces
-  // between their rows turns 32 lines touched by every store into 8 (the
-  // store path takes a line per cycle: 2000 cycles a tile pair at dim 64).
-  const int j4 = lane & 3;
-  uint16_t* out[4];  // of the group's four rows
+  unsigned odd;  // rows of the warp with a finite sum, but a value that is not
+  if (kParts && units > PART) {
+    const bool bad = store_own<DP>(o_at, inv, own, part, a.dim);
+    odd = __ballot_sync(0xffffffffu, mine && bad && l - l == 0.f);
+  } else {
+    uint64_t odd2 = zero2;  // NaN once a value of the row is not finite
+    // Stores go by groups of four lanes: a 4 x 4 transpose of 16-byte pieces
+    // between their rows turns 32 lines touched by every store into 8 (the
+    // store path takes a line per cycle: 2000 cycles a tile pair at dim 64).
+    const int j4 = lane & 3;
+    uint16_t* out[4];  // of the group's four rows
 #pragma unroll
-  for (int k = 0; k < 4; ++k) out[k] = (uint16_t*)__shfl_sync(0xffffffffu, (uint64_t)own, (lane & ~3) + k);
+    for (int k = 0; k < 4; ++k) out[k] = (uint16_t*)__shfl_sync(0xffffffffu, (uint64_t)own, (lane & ~3) + k);
 #pragma unroll
-  for (int c = 0; c < DP / 32; ++c) {
-    uint32_t w[4][4];
+    for (int c = 0; c < DP / 32; ++c) {
+      uint32_t w[4][4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) w[k][0] = w[k][1] = w[k][2] = w[k][3] = 0;
-    if (units > 0) {
-      uint32_t o[32];
-      uk_tmem_ld32(o_at + c * 32, o);
-      uk_tmem_ld_wait();
-      if (kParts && units > PART) add_parts(2 * c, o), add_parts(2 * c + 1, o + 16);
+      for (int k = 0; k < 4; ++k) w[k][0] = w[k][1] = w[k][2] = w[k][3] = 0;
+      if (units > 0) {
+        uint32_t o[32];
+        uk_tmem_ld32(o_at + c * 32, o);
+        uk_tmem_ld_wait();
 #pragma unroll
-      for (int k = 0; k < 16; ++k) {
-        const uint64_t v = uk_f2_fma(uk_f2(__uint_as_float(o[2 * k]), __uint_as_float(o[2 * k + 1])), inv2, zero2);
-        odd2 = uk_f2_fma(v, zero2, odd2);
-        float x, y;
-        uk_f2_split(v, &x, &y);
-        w[k / 4][k % 4] = pack_half(x, y);
-      }
-    }
-#pragma unroll
-    for (int bit = 1; bit < 4; bit *= 2)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (k & bit) continue;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const bool up = lane & bit;
-          const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? w[k][e] : w[k + bit][e], bit);
-          if (up) w[k][e] = got;
-          else w[k + bit][e] = got;
+        for (int k = 0; k < 16; ++k) {
+          const uint64_t v = uk_f2_fma(uk_f2(__uint_as_float(o[2 * k]), __uint_as_float(o[2 * k + 1])), inv2, zero2);
+          odd2 = uk_f2_fma(v, zero2, odd2);
+          float x, y;
+          uk_f2_split(v, &x, &y);
+          w[k / 4][k % 4] = uk_pack_finite(x, y);
         }
       }
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (out[k] != nullptr && c * 32 + j4 * 8 < a.dim)
-        *reinterpret_cast<uint4*>(out[k] + c * 32 + j4 * 8) = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
+      for (int bit = 1; bit < 4; bit *= 2)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (k & bit) continue;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const bool up = lane & bit;
+            const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? w[k][e] : w[k + bit][e], bit);
+            if (up) w[k][e] = got;
+            else w[k + bit][e] = got;
+          }
+        }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (out[k] != nullptr && c * 32 + j4 * 8 < a.dim)
+          *reinterpret_cast<uint4*>(out[k] + c * 32 + j4 * 8) = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
+    }
+    float odd0, odd1;
+    uk_f2_split(odd2, &odd0, &odd1);
+    odd = __ballot_sync(0xffffffffu, mine && odd0 + odd1 != 0.f && l - l == 0.f);
+    if (odd != 0) {  // infinities go out as such
+      __syncwarp();
+      store_own<DP>(o_at, inv, odd >> lane & 1u ? own : nullptr, 0.f, a.dim);
+    }
   }
   if (units > 0) {
     uk_tc_fence_before();
@@ -526,10 +571,7 @@ __device__ __forceinline__ bool softmax_tile(const Args& a, Ctl* ctl, const Item
   if (mine && a.lse != nullptr)
     a.lse[token * a.heads_q + row.head] = l == 0.f ? -INFINITY : (m - SHIFT + log2f(l)) * LN2;
 
-  // rows that may have met what their mask hides: a finite sum, but not a finite row
-  float odd0, odd1;
-  uk_f2_split(odd2, &odd0, &odd1);
-  unsigned odd = __ballot_sync(0xffffffffu, mine && odd0 + odd1 != 0.f && l - l == 0.f);
+  // they may have met what their mask hides
   while (odd != 0) {
     const int r = __ffs(odd) - 1;
     odd &= odd - 1;
@@ -571,7 +613,7 @@ __device__ __forceinline__ void join_shares(const Args& a, Ctl* ctl, uint8_t* ri
     }
     const int64_t token = (int64_t)it.q0 + r.token;
     *reinterpret_cast<uint4*>(a.o + token * a.o_token + r.head * a.o_head + d) = make_uint4(
-        pack_half(o[0], o[1]), pack_half(o[2], o[3]), pack_half(o[4], o[5]), pack_half(o[6], o[7]));
+        uk_pack_average(o[0], o[1]), uk_pack_average(o[2], o[3]), uk_pack_average(o[4], o[5]), uk_pack_average(o[6], o[7]));
     if (a.lse != nullptr && d == 0)
       a.lse[token * a.heads_q + r.head] = l == 0.f ? -INFINITY : (mm - SHIFT + log2f(l)) * LN2;
     if (odd && l - l == 0.f) atomicOr(&ctl->odd[row / 32], 1u << (row % 32));

@@ -121,6 +121,21 @@ __device__ __forceinline__ uint32_t uk_half2_of(float x) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// Two attention outputs as halves.  They are averages of binary16 values, so a
+// finite one that lies above 65504 is so by rounding (of the weights) alone and
+// becomes 65504; an infinity stays one.
+__device__ __forceinline__ uint32_t uk_pack_finite(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint32_t uk_pack_average(float lo, float hi) {
+  uint32_t r = uk_pack_finite(lo, hi);
+  if (fabsf(lo) == INFINITY) r = (r & 0xffff8000u) | 0x7c00u;
+  if (fabsf(hi) == INFINITY) r = (r & 0x8000ffffu) | 0x7c000000u;
+  return r;
+}
+
 // 2^(e - 127) for an exponent byte (0 counts as 2^-127: not written by the append)
 __device__ __forceinline__ float uk_exp_scale(uint32_t e) { return __uint_as_float(e == 0 ? 0x00400000u : e << 23); }
 
