@@ -602,6 +602,62 @@ def test_prompt_rows_do_not_see_behind_their_mask():
                 assert torch.isfinite(lse).all()
 
 
+@pytest.mark.parametrize("heads,group,dim,n", [(2, 4, 128, 700), (3, 1, 72, 1500), (1, 2, 64, 3000)])
+def test_prompt_nan_from_a_key_on(heads, group, dim, n):
+    """All values NaN from a key on, some columns from another one on, infinities
+    among them: rows before are exact, columns that only hidden keys spoil too."""
+    a = abi()
+    fault()
+    q, k, v = randn(n, heads * group, dim, seed=1), randn(n, heads, dim, seed=2), randn(n, heads, dim, seed=3)
+    at = {0: n // 2 + 3, 7: n // 2 - 50, 11: n - 1}  # the first key that spoils a column
+    rest = n // 2 + 20
+    for c, j in at.items():
+        v[j:, 0, c] = math.nan
+    v[n // 2 - 5, 0, 2] = math.inf
+    v[rest:, 0, [c for c in range(dim) if c not in (2, *at)]] = math.nan
+    o, lse = torch.empty_like(q), torch.empty(n, heads * group, device="cuda")
+    a.attn_prompt(q, k, v, i32([0, n]), i32([0, n]), o, lse=lse)
+    assert fault() == 0
+    first = torch.tensor([at.get(c, n if c == 2 else rest) for c in range(dim)], device="cuda")
+    gone = torch.arange(n, device="cuda")[:, None] >= first
+    assert torch.equal(torch.isnan(o[:, :group]), gone[:, None].expand(n, group, dim))
+    assert torch.equal(o[:, :group, 2] == math.inf, (torch.arange(n, device="cuda") >= n // 2 - 5)[:, None].expand(n, group))
+    assert torch.isfinite(lse).all() and torch.isfinite(o[:, group:]).all()
+    # each column against the definition over keys that hold nothing spoilt but what it sees
+    sane = torch.where(torch.isfinite(v), v, torch.zeros_like(v))
+    seen = torch.arange(n, device="cuda")[None] <= torch.arange(n, device="cuda")[:, None]
+    for h in (0, heads * group - 1):
+        ro, rl, to, tl = attention_f64(q[:, h], k[:, h // group], sane[:, h // group], dim ** -0.5, seen)
+        got = o[:, h].double()
+        fine = torch.isfinite(got)
+        assert ((got - ro).abs() <= to)[fine].all()
+        assert_close(lse[:, h], rl, tl, "head %d: lse" % h)
+
+
+def test_prompt_of_nan_is_not_computed_again():
+    """Where every value is NaN no row is looked at key by key (a thousand times the
+    time of a prompt of numbers; 5 times it without)."""
+    a = abi()
+    n = 8192
+    q, k, v = (randn(n, h, 128, seed=h) for h in (8, 2, 2))
+    o, cu = torch.empty_like(q), i32([0, n])
+
+    def took():
+        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.attn_prompt(q, k, v, cu, cu, o)
+        torch.cuda.synchronize()
+        start.record()
+        a.attn_prompt(q, k, v, cu, cu, o)
+        end.record()
+        torch.cuda.synchronize()
+        return start.elapsed_time(end)
+
+    clean = took()
+    v.fill_(math.nan)
+    assert took() < 60 * clean
+    assert torch.isnan(o).all()
+
+
 def test_prompt_rows_computed_again_behind_a_long_context():
     """A NaN that only the last query may see, behind so many keys that the 127
     rows before it in its tile take seconds to be computed again: the other warps
