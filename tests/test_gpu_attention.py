@@ -148,7 +148,8 @@ def test_decode_long(kind):
 
 @pytest.mark.parametrize("kind,page,heads,group,dim,seqs,n", [
     ("f16", 64, 8, 4, 16, 64, 1 << 20), ("e4m3", 64, 8, 4, 16, 64, 1 << 20), ("f16", 40, 2, 12, 64, 230, 150001),
-    ("e4m3", 32, 2, 20, 128, 230, 140000), ("f16", 16, 8, 1, 128, 56, 200000)])
+    ("e4m3", 32, 2, 20, 128, 230, 140000), ("f16", 16, 8, 1, 128, 56, 200000), ("f16", 64, 2, 4, 16, 10, 1 << 20),
+    ("e4m3", 16, 1, 9, 64, 12, 1600000)])
 def test_decode_sums_over_long_contexts(kind, page, heads, group, dim, seqs, n):
     """So many long sequences that a block sums whole ones up (all of them in the
     same pages), some shorter ones between them; values that do not cancel under

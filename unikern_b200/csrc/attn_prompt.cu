@@ -40,7 +40,7 @@
 // Every mbarrier wait is bounded (uk_mbar_wait); a timeout sets the fault word
 // read by uk_cuda_pipeline_fault() and the CTA unwinds.  Rows that are computed
 // again may take longer than any limit (17.5 us a key for a warp's 32 rows): while
-// they do, a counter moves, and the waits for their warp are taken up again.
+// they are, the time limit is put off again and again.
 #include <cudaTypedefs.h>
 
 #include <mutex>
@@ -77,6 +77,9 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 
+constexpr uint64_t WAIT_NS = 2000000000ull;  // 2 s
+__device__ __forceinline__ void put_off(volatile uint64_t* limit) { *limit = uk_globaltimer() + WAIT_NS; }
+
 // A sum that carries what its additions round off (Kahan): those of equal terms
 // all round the same way (2^20 keys by plain sums: 7 times the tests' bound off).
 struct LongSum {
@@ -90,16 +93,17 @@ struct LongSum {
 };
 
 // One row by one warp, key by key, on CUDA cores: keys [k0, end).  A lane
-// holds four of the row's values.  *beat (in shared memory, where there is one)
-// moves every few milliseconds.
-__device__ __noinline__ void attend_row(const Args& a, int64_t t, int h, int64_t k0, int64_t end, unsigned* beat) {
+// holds four of the row's values.  *limit (where there is one), the
+// time limit of other warps' waits, is put off every few milliseconds.
+__device__ __noinline__ void attend_row(const Args& a, int64_t t, int h, int64_t k0, int64_t end,
+                                        volatile uint64_t* limit) {
   const int lane = threadIdx.x & 31, g = h / a.group;
   const float4 q = row4(a.q + t * a.q_token + h * a.q_head, lane, a.dim);
   float m = -INFINITY;
   LongSum l, o[4];
   constexpr int U = 4;  // keys in flight
   for (int64_t j = k0; j < end; j += U) {
-    if (beat != nullptr && ((j - k0) & 4095) == 0 && lane == 0) atomicAdd(beat, 1u);
+    if (limit != nullptr && ((j - k0) & 4095) == 0 && lane == 0) put_off(limit);
     float4 k[U], v[U];
     float s[U], top = -INFINITY;
 #pragma unroll
@@ -154,7 +158,6 @@ constexpr int NUM_THREADS = 384;
 constexpr int REGS_LAUNCH = 168, REGS_SOFTMAX = 216, REGS_OTHERS = 72;
 static_assert(2 * REGS_SOFTMAX + REGS_OTHERS <= 3 * REGS_LAUNCH, "registers of the block");
 constexpr int MMA_WARP = 8, LOAD_WARP = 10;  // MMA_WARP + t: tile t
-constexpr uint64_t WAIT_NS = 2000000000ull;  // 2 s: a pass over 2^25 keys, which a tile may have to wait for, takes 0.6 s
 
 // One warp: the first level that has items, from the longest sequence.
 __device__ int first_level(const Args& a) {
@@ -205,7 +208,7 @@ struct Ctl {
   alignas(16) uint8_t answer[16];
   uint32_t tmem;
   int abort;
-  unsigned beat;    // moves while rows are computed again or blocks taken over
+  uint64_t limit;   // of the waits: a time
   unsigned odd[4];  // rows of a shared tile to look at again
   Item item[2];
 };
@@ -215,28 +218,22 @@ static_assert(Smem<128>::BYTES <= 232448 && Smem<64>::BYTES <= 232448, "shared m
 __device__ __forceinline__ void raise_fault(Ctl* ctl, unsigned bit) {
   atomicOr(&uk::g_attn_prompt_fault, bit);
   ctl->abort = 1;
+  *(volatile uint64_t*)&ctl->limit = 0;
 }
 
-// uk_mbar_wait, but a wait that has run out is taken up once more, and again for
-// as long as `beat` moves meanwhile: its steps take some milliseconds, and there are
-// finitely many.
-__device__ __forceinline__ bool wait_beat(Ctl* ctl, uint64_t* bar, uint32_t parity, volatile int* abort) {
+// Waits end at the block's common time limit.  It is put off when the load warp comes
+// to a new item and every 64 blocks of keys, and every few milliseconds while rows
+// are computed again or blocks taken over, of which there are finitely many.
+__device__ __forceinline__ bool wait_until(const Ctl* ctl, uint64_t* bar, uint32_t parity) {
   if (uk_mbar_try_wait(bar, parity)) return true;
-  uint64_t t0 = uk_globaltimer();
-  unsigned seen = 0;  // beat is never 0
   for (uint32_t i = 1;; ++i) {
     if (uk_mbar_try_wait(bar, parity)) return true;
-    if ((i & 255u) != 0) continue;
-    if (abort != nullptr && *abort) return false;
-    if (uk_globaltimer() - t0 <= WAIT_NS) continue;
-    const unsigned now = *(volatile unsigned*)&ctl->beat;
-    if (now == seen) return false;
-    seen = now, t0 = uk_globaltimer();
+    if ((i & 255u) == 0 && uk_globaltimer() > *(const volatile uint64_t*)&ctl->limit) return false;
   }
 }
-// a bounded wait by a whole warp: the same answer in every lane
+// by a whole warp: the same answer in every lane
 __device__ __forceinline__ bool wait_warp(Ctl* ctl, uint64_t* bar, uint32_t parity, unsigned bit) {
-  if (__all_sync(0xffffffffu, wait_beat(ctl, bar, parity, &ctl->abort))) return true;
+  if (__all_sync(0xffffffffu, wait_until(ctl, bar, parity))) return true;
   if (!*(volatile int*)&ctl->abort) raise_fault(ctl, bit);
   return false;
 }
@@ -255,7 +252,7 @@ __device__ __forceinline__ int end_of(const Args& a, const Item& it, int token) 
 // are looked at: from the first NaN of a model on, all are.  8192 rows of NaN, 32
 // heads over 8 of 128: 2.4 ms, all of them computed again 551.)
 __device__ __noinline__ void look_again(const Args& a, const Item& it, const Tile& tile, int row, int units,
-                                        unsigned* beat) {
+                                        volatile uint64_t* limit) {
   const Row r(a, tile, row);
   const int lane = threadIdx.x & 31, from = end_of(a, it, r.token), to = min(units * UN, it.m);
   const uint16_t* v0 = a.v + (int64_t)it.k0 * a.v_token + it.g * a.v_head;
@@ -286,7 +283,7 @@ __device__ __noinline__ void look_again(const Args& a, const Item& it, const Til
   }
   __syncwarp();  // the row's stores before come before these
   if (__any_sync(0xffffffffu, bad != 0))
-    attend_row(a, (int64_t)it.q0 + r.token, r.head, it.k0, (int64_t)it.k0 + from, beat);
+    attend_row(a, (int64_t)it.q0 + r.token, r.head, it.k0, (int64_t)it.k0 + from, limit);
 }
 
 // A shared tile's sums in shared memory: 128 rows of DP floats (16-byte pieces
@@ -600,7 +597,7 @@ __device__ __forceinline__ bool softmax_tile(const Args& a, Ctl* ctl, const Item
   while (odd != 0) {
     const int r = __ffs(odd) - 1;
     odd &= odd - 1;
-    look_again(a, it, tile, quad * 32 + r, units, &ctl->beat);
+    look_again(a, it, tile, quad * 32 + r, units, &ctl->limit);
   }
   return true;
 }
@@ -645,7 +642,7 @@ __device__ __forceinline__ void join_shares(const Args& a, Ctl* ctl, uint8_t* ri
   }
   asm volatile("bar.sync 1, 256;" ::: "memory");
   for (int row = rank * rows + (int)(threadIdx.x >> 5); row < (rank + 1) * rows; row += 8)
-    if (ctl->odd[row / 32] >> (row % 32) & 1u) look_again(a, it, tile, row, it.all_units, &ctl->beat);
+    if (ctl->odd[row / 32] >> (row % 32) & 1u) look_again(a, it, tile, row, it.all_units, &ctl->limit);
 }
 
 // Most blocks of the grid can lie behind the list's end, up to as many as there are
@@ -659,7 +656,7 @@ __device__ __noinline__ int2 drain_blocks(const Args& a, Ctl* ctl, uint32_t item
     if ((threadIdx.x & 31) == 0) {
       uk_mbar_expect_tx(&ctl->next, 16);
       uk_next_block_ask(ctl->answer, &ctl->next);
-      if (n % 1024 == 0) atomicAdd(&ctl->beat, 1u);
+      if (n % 1024 == 0) put_off(&ctl->limit);
     }
     __syncwarp();
     // this block's memory is not given up before the answer is there
@@ -692,6 +689,7 @@ __device__ __forceinline__ void load_items(const Args& a, Ctl* ctl, uint8_t* sme
   uint32_t answers = 0;
   for (uint32_t turn = 0; ok; ++turn) {
     Item& it = ctl->item[turn & 1u];
+    if (lane == 0 && !*abort) put_off(&ctl->limit);
     if (!(ok = wait_warp(ctl, &ctl->item_empty[turn & 1u], ((turn >> 1) & 1u) ^ 1u, UK_FAULT_PRODUCER))) break;
     // the first item was looked up before the barriers were up
     if (turn > 0) any = block >= 0 && find_item(a, (uint32_t)block, cursor, &it);
@@ -732,6 +730,7 @@ __device__ __forceinline__ void load_items(const Args& a, Ctl* ctl, uint8_t* sme
         if (!ok) break;
       }
       const int s = n % S::STAGES, at = (it.first_block + (j >> 1)) * BN;  // K and V blocks alternate
+      if ((j & 127) == 127 && lane == 0 && !*abort) put_off(&ctl->limit);
       if (!(ok = wait_warp(ctl, &ctl->kv_empty[s], ((n / S::STAGES) & 1u) ^ 1u, UK_FAULT_PRODUCER))) break;
       const bool fix = (j & 1) && at + BN > it.m;
       uint8_t* dst = ring + (size_t)s * S::TILE;
@@ -876,8 +875,12 @@ __device__ __forceinline__ void issue_products(Ctl* ctl, int t, uint8_t* smem, u
   }
   // every product issued completes before TMEM and shared memory are given up
   commit(&ctl->teardown);
-  if (!__all_sync(0xffffffffu, wait_beat(ctl, &ctl->teardown, 0, nullptr)))  // the other tile's warp, too, has to get there
+  // (the other tile's warp, too, has to get there)
+  while (!__all_sync(0xffffffffu, uk_mbar_wait(&ctl->teardown, 0, nullptr, WAIT_NS))) {
+    if (!__any_sync(0xffffffffu, uk_globaltimer() > *(volatile uint64_t*)&ctl->limit)) continue;
     atomicOr(&uk::g_attn_prompt_fault, UK_FAULT_TEARDOWN);
+    break;
+  }
 }
 
 // kSplit: a cluster of a.split CTAs per tile, each with a share of its keys, and
@@ -916,7 +919,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     uk_mbar_init(&ctl->v_landed, 1);
     uk_mbar_init(&ctl->teardown, 2);
     ctl->abort = 0;
-    ctl->beat = 1;
+    put_off(&ctl->limit);
     for (int i = 0; i < 4; ++i) ctl->odd[i] = 0;
     uk_fence_mbar_init();
     uk_tma_prefetch_desc(&tm_q);
@@ -1098,8 +1101,9 @@ extern "C" int uk_cuda_attn_prompt_f16(const uint16_t* Q, int64_t q_token_stride
                                        int64_t total_k, int heads_q, int heads_kv, int dim, float scale, int causal,
                                        uint16_t* O, int64_t o_token_stride, int64_t o_head_stride, float* LSE,
                                        void* stream) {
-  // 2^25 keys: a tile's pass over them (0.6 s) stays well within the kernel's bounded
-  // waits; queries: a tile's row numbers stay within 31 bits
+  // 2^25 keys: a tile's pass over them takes 0.6 s, and weights below 2^-32 of the
+  // largest, which binary16 does not hold, are at most 2^-7 of the sum; queries: a
+  // tile's row numbers stay within 31 bits
   if (n_seq < 0 || n_seq > uk::MAX_SEQS || total_q < 0 || total_k < 0 || total_q > 0x7fffff00 || total_k > (1 << 25))
     return uk::fail(UK_EINVAL, "attn_prompt: n_seq %d (at most 2^24), total_q %lld (2^31 - 256), total_k %lld (2^25)",
                     n_seq, (long long)total_q, (long long)total_k);

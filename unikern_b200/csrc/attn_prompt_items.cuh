@@ -114,11 +114,10 @@ __host__ __device__ __forceinline__ int first_level_of(const Args& a, int most) 
 
 __host__ __device__ __forceinline__ int bound(const int32_t* cu, int i, int lo, int hi) {
 #ifdef __CUDA_ARCH__
-  const int x = __ldg(cu + i);
+  return min(max(__ldg(cu + i), lo), hi);
 #else
-  const int x = cu[i];
+  return cu[i] < lo ? lo : cu[i] > hi ? hi : cu[i];
 #endif
-  return x < lo ? lo : x > hi ? hi : x;
 }
 // keys of sequence b
 __host__ __device__ __forceinline__ int keys_of(const Args& a, int b) {
