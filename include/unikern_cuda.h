@@ -316,8 +316,12 @@ int uk_cuda_decode_rmsnorm_gemm_f16(const float* X, const float* gamma, float ep
  *   UK_KV_F16   rows of binary16.
  *   UK_KV_E4M3  rows of 8-bit e4m3 codes (4 exponent and 3 mantissa bits, no
  *               infinity) and one exponent byte e per row, in k_exp / v_exp
- *               [pages][heads][page_size]: value = code * 2^(e - 127).  e - 127
- *               is within [-24, 15].
+ *               [pages][heads][page_size]: value = code * 2^(e - 127).  The
+ *               append writes e - 127 from -15 to 8 and only values that
+ *               binary16 holds.  A caller's own bytes are taken with e - 127
+ *               from -24 to 15; a value that binary16 does not hold is read
+ *               rounded to it (above 65504: infinite), but for keys in the
+ *               decode attention's scores, which take it unrounded.
  * Any page_size >= 1; dim a multiple of 8 (e4m3: of 16) from 8 to 128; pools
  * 16-byte aligned, strides multiples of 16 bytes; max_pages * page_size below
  * 2^31 - 4096; up to 2^24 sequences in a call.  uk_cuda_attn_decode_f16 refuses
@@ -360,8 +364,8 @@ int uk_cuda_kv_append_f16(const uint16_t* K, int64_t k_token_stride, int64_t k_h
                           const int32_t* seq_lens, int n_seq, void* stream);
 
 /* The inverse: the last cu_out[b + 1] - cu_out[b] of the seq_lens[b] positions
- * of each sequence, as packed binary16 rows K, V [total][heads][dim] (exact
- * values of the codes).  Positions below 0 and absent pages give zeros; rows
+ * of each sequence, as packed binary16 rows K, V [total][heads][dim] (the
+ * values held).  Positions below 0 and absent pages give zeros; rows
  * outside cu_out[0] .. cu_out[n_seq] - 1 are left as they were. */
 int uk_cuda_kv_gather_f16(const uk_kv_cache* cache, const int32_t* block_table, int64_t table_stride, int max_pages,
                           const int32_t* cu_out, const int32_t* seq_lens, int n_seq, uint16_t* K,
@@ -377,10 +381,12 @@ int uk_cuda_kv_gather_f16(const uk_kv_cache* cache, const int32_t* block_table, 
  * out).  A sequence of length zero gives zeros and -inf.  Q, O binary16
  * [n_seq][heads_q][dim], strides in elements (multiples of 8, 16-byte aligned);
  * heads_q up to 65535.  O overlaps neither Q nor the cache.
- * Scores, softmax statistics and sums are fp32; the softmax weights enter the
- * value product as binary16, one rounding into O.  A NaN or an infinity among
- * the values seen makes that column's outputs NaN or infinite; an average of
- * finite values is finite (65504 where the roundings lead above it).
+ * Scores, softmax statistics and sums are fp32 (also over long contexts, whose
+ * sums are taken in parts); the softmax weights enter the value product as
+ * binary16 (11 bits; those below 2^-21 of the largest in steps of 2^-32 of it,
+ * at most 2^-11 of the sum over 2^21 positions), one rounding into O.  A NaN or
+ * an infinity among the values seen makes that column's outputs NaN or infinite;
+ * an average of finite values is finite (65504 where the roundings lead above it).
  * Deterministic.  The workspace (its size depends on the current device, the
  * heads and dim, not on lengths or n_seq) may be reused by later calls on the
  * same stream; calls that can overlap need one each. */
@@ -404,8 +410,11 @@ int uk_cuda_attn_decode_f16(const uint16_t* Q, int64_t q_seq_stride, int64_t q_h
  * as they were.  cu_q and cu_k are device memory, non-decreasing within
  * [0, total_q] and [0, total_k]; values outside are clamped.  Up to
  * 2^24 sequences, 2^31 - 256 query and 2^25 key rows, 65535 query heads.  O does
- * not overlap Q, K or V.  fp32 scores, statistics and sums; the softmax weights enter the value
- * product as binary16.  A negative scale runs row by row on CUDA cores.
+ * not overlap Q, K or V; its rows hold intermediate numbers meanwhile.  Scores,
+ * statistics, sums and weights as above.  Two things run row by row on CUDA
+ * cores, 17.5 us a key for 32 rows: a negative scale, and rows whose mask hides a
+ * NaN or an infinity among the next 191 keys while the last 128 keys they see
+ * hold no NaN in the same columns.
  * Deterministic. */
 int uk_cuda_attn_prompt_f16(const uint16_t* Q, int64_t q_token_stride, int64_t q_head_stride, const uint16_t* K,
                             int64_t k_token_stride, int64_t k_head_stride, const uint16_t* V, int64_t v_token_stride,

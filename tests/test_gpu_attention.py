@@ -279,6 +279,40 @@ def test_decode_infinities_and_nan(kind):
     check_decode(pool, q, o, lse, 32 ** -0.5)
 
 
+def test_exponents_of_the_callers_own():
+    """Exponent bytes that the append does not write: values are rounded to binary16
+    by the gather and in the value product, keys enter the scores as they are."""
+    a = abi()
+    fault()
+    heads, dim, n = 2, 64, 700
+    pool = Pool("e4m3", "hnd", heads, dim, 16, [n], seed=1)
+    g = torch.Generator("cuda").manual_seed(5)
+    page, off = pool.where(0, 0, n)
+    held = []
+    for which in range(2):
+        e = torch.randint(-24, 16, (n, heads), device="cuda", generator=g)
+        if which == 0:
+            e = e.clamp(max=-3)  # scores of ordinary size
+        x = torch.randn(n, heads, dim, device="cuda", generator=g)
+        x = torch.where(e[..., None] > 8, x.clamp(-1.75, 1.75), x * 16)
+        code = x.to(torch.float8_e4m3fn)
+        (pool.k, pool.v)[which].view(torch.uint8)[page, off] = code.view(torch.uint8)
+        pool.exps[which].transpose(1, 2)[page, off] = (e + 127).to(torch.uint8)
+        held.append(code.double() * torch.exp2(e.double())[..., None])
+    rounded = [h.half() for h in held]  # exact in fp32 on the way: four significant bits
+    out = [torch.empty(n, heads, dim, dtype=torch.float16, device="cuda") for _ in "kv"]
+    a.kv_gather(pool.cache, pool.table, i32([0, n]), pool.lens_t, *out)
+    assert same_bits(out[0], rounded[0]) and same_bits(out[1], rounded[1])
+    assert torch.isfinite(rounded[1]).all()
+    pool.values[0] = (held[0], rounded[1].double())
+    q = randn(1, heads * 4, dim, seed=2)
+    for table in both_splits(pool):
+        o, lse = torch.empty_like(q), torch.empty(q.shape[:2], device="cuda")
+        a.attn_decode(q, pool.cache, table, pool.lens_t, o, lse=lse)
+        check_decode(pool, q, o, lse, dim ** -0.5)
+    assert fault() == 0
+
+
 def test_decode_absent_pages():
     a = abi()
     fault()
