@@ -8,12 +8,13 @@
 // The work is bound by the tensor cores (4 dim flops per visible pair and head)
 // and, nearly as much, by the exponentials (one per pair and head; the MUFU
 // makes 16 per cycle and SM, a 128 x 128 tile's take as long as its two
-// products at dim 128); long prompts run into the power limit first (8192 rows,
-// 32 heads over 8 of 128: 1370 MHz).  A tile has 128 rows: the heads of a key
-// head's group, side by side for each of as many tokens as fit (32 for groups of
-// 4), so short sequences fill it too.  A CTA (one per SM) works on two tiles of
-// one key head at a time, so that one tile's products run while the other's
-// softmax does:
+// products at dim 128); the two wait for one another (8192 rows, 32 heads over 8 of
+// 128: 3150 cycles for two tiles by 128 keys, 2048 of them products), and long
+// prompts run into the power limit (1520 MHz: 517 us, 442 before the limit acts).
+// A tile has 128 rows: the heads of a key head's group, side by side for each of as
+// many tokens as fit (32 for groups of 4), so short sequences fill it too.  A CTA
+// (one per SM) works on two tiles of one key head at a time, so that one tile's
+// products run while the other's softmax does:
 //   warp 10      loads (TMA): both Q tiles, then K and V blocks of 128 keys through
 //                a ring in shared memory; finds the next pair of tiles meanwhile;
 //   warps 8, 9   issue tcgen05.mma, a tile each: S = Q K^T for runs of 64 keys,
@@ -150,7 +151,10 @@ __device__ __noinline__ void attend_row(const Args& a, int64_t t, int h, int64_t
 // go 8e-4 over 131072, 7e-3 over 2^20).  Calls of at most as many keys in all run
 // without the code for parts: 11 x 900 rows of dim 64 39.6 us, 41.1 with it.
 constexpr int PART = 512;
-constexpr float SHIFT = 7.f;       // weights are held as 2^7 * 2^(s - m): up to 2^15, binary16 ends at 2^16
+// Weights enter the product as binary16, 2^7 * 2^(s - m): up to 2^15 (binary16 ends
+// at 2^16), normal down to 2^-21 of the reference's.  Each is off by 2^-11 at most;
+// 32-bit operands would halve the products' rate.
+constexpr float SHIFT = 7.f;
 // three warpgroups: two of softmax, one of the MMA and load warps (and an idle
 // one).  They launch with 168 registers a thread; the softmax takes 216 (a row
 // of 128 scores stays in registers) and the others keep 72.
@@ -647,7 +651,7 @@ __device__ __forceinline__ void join_shares(const Args& a, Ctl* ctl, uint8_t* ri
 
 // Most blocks of the grid can lie behind the list's end, up to as many as there are
 // items: a warp that has got one of them takes over others, each in less time than it
-// takes to start one (1024 prompts of 64 rows, 32 heads over 8 of 128: 367 us, 1340
+// takes to start one (1024 prompts of 64 rows, 32 heads over 8 of 128: 357 us, 1340
 // without this).  Returns the number of one that is on the list after all, its item
 // looked up from the start, or -1; and how many answers there were.
 __device__ __noinline__ int2 drain_blocks(const Args& a, Ctl* ctl, uint32_t items, uint32_t answers, Item* out) {
