@@ -38,7 +38,7 @@
 // not, the few masked keys of its last blocks are looked through; if one of
 // them holds a NaN or an infinity the row is computed again, key by key.
 //
-// Every mbarrier wait is bounded (uk_mbar_wait); a timeout sets the fault word
+// Every mbarrier wait is bounded (wait_until, uk_mbar_wait); a timeout sets the fault word
 // read by uk_cuda_pipeline_fault() and the CTA unwinds.  Rows that are computed
 // again may take longer than any limit (17.5 us a key for a warp's 32 rows): while
 // they are, the time limit is put off again and again.
@@ -1082,7 +1082,8 @@ int launch(const Args& a, int64_t items, cudaStream_t st) {
 
 template <int DP>
 int launch(const Args& a, int64_t items, cudaStream_t st) {
-  if (a.total_k > PART * UN) return a.split > 1 ? launch<DP, true, true>(a, items, st) : launch<DP, false, true>(a, items, st);
+  if (a.total_k > PART * UN)
+    return a.split > 1 ? launch<DP, true, true>(a, items, st) : launch<DP, false, true>(a, items, st);
   return a.split > 1 ? launch<DP, true, false>(a, items, st) : launch<DP, false, false>(a, items, st);
 }
 
